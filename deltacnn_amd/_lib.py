@@ -84,6 +84,43 @@ class AddItem(ctypes.Structure):
         ("batch", c_int32), ("height", c_int32), ("width", c_int32), ("channels", c_int32), ("scale", c_int32)]
 
 
+class RotaryArgs(ctypes.Structure):
+    """struct dc_rotary_args."""
+    _fields_ = [
+        ("tokens", c_int32), ("q_heads", c_int32), ("kv_heads", c_int32), ("dim", c_int32),
+        ("q", c_void_p), ("q_token_stride", c_int64), ("q_head_stride", c_int64),
+        ("out", c_void_p), ("out_token_stride", c_int64), ("out_head_stride", c_int64),
+        ("positions", c_void_p), ("axes", c_int32), ("sections", c_int32 * 4), ("frequencies", c_void_p),
+        ("interleaved", c_int32), ("inverse", c_int32), ("k", c_void_p), ("v", c_void_p),
+        ("k_token_stride", c_int64), ("k_head_stride", c_int64), ("v_token_stride", c_int64), ("v_head_stride", c_int64),
+        ("keys", c_void_p), ("values", c_void_p), ("weights", c_void_p), ("stamps", c_void_p),
+        ("token_stamps", c_void_p), ("page_table", c_void_p), ("slots", c_void_p), ("starts", c_void_p),
+        ("streams", c_int32), ("num_pages", c_int32), ("page_size", c_int32), ("max_pages", c_int32),
+        ("lens", c_void_p), ("new_lens", c_void_p)]
+
+
+class AttentionArgs(ctypes.Structure):
+    """struct dc_attention_args."""
+    _fields_ = [
+        ("tokens", c_int32), ("q_heads", c_int32), ("kv_heads", c_int32), ("dim", c_int32),
+        ("q", c_void_p), ("q_token_stride", c_int64), ("q_head_stride", c_int64),
+        ("out", c_void_p), ("out_token_stride", c_int64), ("out_head_stride", c_int64),
+        ("lse", c_void_p), ("keys", c_void_p), ("values", c_void_p),
+        ("page_table", c_void_p), ("lens", c_void_p), ("starts", c_void_p),
+        ("streams", c_int32), ("num_pages", c_int32), ("page_size", c_int32), ("max_pages", c_int32),
+        ("causal_block", c_int32), ("scale", c_float), ("weights", c_void_p), ("decay", c_float),
+        ("workspace", c_void_p), ("workspace_bytes", c_int64)]
+
+
+class SlotsArgs(ctypes.Structure):
+    """struct dc_slots_args."""
+    _fields_ = [
+        ("weights", c_void_p), ("stamps", c_void_p), ("keep_from", c_void_p),
+        ("page_table", c_void_p), ("lens", c_void_p), ("starts", c_void_p),
+        ("streams", c_int32), ("tokens", c_int32), ("kv_heads", c_int32), ("num_pages", c_int32),
+        ("page_size", c_int32), ("max_pages", c_int32), ("budget", c_int32), ("slots", c_void_p), ("new_lens", c_void_p)]
+
+
 CONV_GROUP_MAX = 8
 
 _P = c_void_p
@@ -118,6 +155,10 @@ _SIGNATURES = {
     "dc_upsample": (c_int, [_P, _P, _P, _P, c_int32, c_int32, c_int32, c_int32, c_int32, c_int, _P]),
     "dc_concat": (c_int, [_P, _P, _P, _P, _P, _P, c_int32, c_int32, c_int32, c_int, _P]),
     "dc_mul_add": (c_int, [_P, _P, _P, _P, _P, _P, c_int32, c_int32, c_int, _P]),
+    "dc_rotary": (c_int, [POINTER(RotaryArgs), c_int, _P]),
+    "dc_paged_attention": (c_int, [POINTER(AttentionArgs), c_int, _P]),
+    "dc_paged_attention_workspace": (c_int64, [POINTER(AttentionArgs), c_int]),
+    "dc_cache_slots": (c_int, [POINTER(SlotsArgs), _P]),
 }
 
 _lib = None

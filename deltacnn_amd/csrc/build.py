@@ -14,8 +14,9 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
 LIB = os.path.join(PKG, "libdeltacnn_hip.so")
-SOURCES = ["dc_abi.cpp", "elementwise.hip", "conv.hip", "convres.hip", "pwconv.hip", "pwpair.hip", "pool.hip", "block.hip", "linear.hip"]
-HEADERS = ["common.hpp", "tile.hpp", "epilogue.hpp", os.path.join("..", "..", "include", "deltacnn_hip.h")]
+SOURCES = ["dc_abi.cpp", "elementwise.hip", "conv.hip", "convres.hip", "pwconv.hip", "pwpair.hip", "pool.hip", "block.hip", "linear.hip",
+           "rotary.hip", "attention.hip", "slots.hip"]
+HEADERS = ["common.hpp", "tile.hpp", "epilogue.hpp", "cache.hpp", os.path.join("..", "..", "include", "deltacnn_hip.h")]
 # -ffp-contract=off: every operation of the bit-exact elementwise operators rounds on its own.
 # packed-fp32-ops disabled: hipcc must not form v_pk_*_f32 from ordinary float code.
 FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-ffp-contract=off",

@@ -954,4 +954,175 @@ int dc_mul_add(const void *input, const int32_t *mask, void *out, int32_t *mask_
                                      dtype, (hipStream_t)stream), "dc_mul_add");
 }
 
+namespace {
+
+// Bytes that rows [tokens][heads][dim] with these strides span.
+size_t rows_span(int32_t tokens, int32_t heads, int32_t dim, int64_t token_stride, int64_t head_stride, int dtype) {
+    return (size_t(tokens - 1) * token_stride + size_t(heads - 1) * head_stride + dim) * esize(dtype);
+}
+
+int check_rows(const char *fn, const char *what, const void *p, int32_t heads, int32_t dim, int64_t token_stride,
+               int64_t head_stride, int dtype) {
+    if (p == nullptr) return fail(DC_ERR_NULL, "%s: %s is NULL", fn, what);
+    if (reinterpret_cast<uintptr_t>(p) % esize(dtype)) return fail(DC_ERR_ALIGN, "%s: %s is not aligned to its elements", fn, what);
+    // heads of a token and tokens must not overlap: either may be the outer dimension
+    if (token_stride < dim || (heads > 1 && head_stride < dim))
+        return fail(DC_ERR_SHAPE, "%s: %s strides %lld, %lld below dim=%d", fn, what, (long long)token_stride, (long long)head_stride, dim);
+    return DC_OK;
+}
+
+int check_pool(const char *fn, int32_t streams, int32_t num_pages, int32_t page_size, int32_t max_pages, int32_t tokens,
+               const int32_t *page_table, const int32_t *starts) {
+    if (streams <= 0 || num_pages <= 0 || page_size <= 0 || max_pages <= 0)
+        return fail(DC_ERR_SHAPE, "%s: streams=%d, num_pages=%d, page_size=%d, max_pages=%d must be positive", fn, streams,
+                    num_pages, page_size, max_pages);
+    if (streams > 65535) return fail(DC_ERR_UNSUPPORTED, "%s: streams=%d exceeds 65535", fn, streams);
+    if ((int64_t)max_pages * page_size > (1 << 30))
+        return fail(DC_ERR_UNSUPPORTED, "%s: more than 2^30 slots in a stream", fn);
+    if (starts == nullptr && tokens % streams != 0)
+        return fail(DC_ERR_SHAPE, "%s: %d tokens do not divide over %d streams (pass starts)", fn, tokens, streams);
+    if (page_table == nullptr) return fail(DC_ERR_NULL, "%s: page_table is NULL", fn);
+    if (reinterpret_cast<uintptr_t>(page_table) % 4 || reinterpret_cast<uintptr_t>(starts) % 4)
+        return fail(DC_ERR_ALIGN, "%s: page_table and starts are int32", fn);
+    return DC_OK;
+}
+
+int check_heads(const char *fn, int32_t tokens, int32_t q_heads, int32_t kv_heads, int32_t dim) {
+    if (tokens <= 0 || q_heads <= 0 || dim <= 0 || kv_heads <= 0)
+        return fail(DC_ERR_SHAPE, "%s: tokens=%d, heads=%d/%d, dim=%d must be positive", fn, tokens, q_heads, kv_heads, dim);
+    if (tokens > (1 << 24) || q_heads > 1024 || kv_heads > 256)
+        return fail(DC_ERR_UNSUPPORTED, "%s: more than 2^24 tokens, 1024 query heads or 256 kv heads", fn);
+    return DC_OK;
+}
+
+int check_attention(const dc_attention_args *a, int dtype) {
+    const char *fn = "dc_paged_attention";
+    if (a == nullptr) return fail(DC_ERR_NULL, "%s: args is NULL", fn);
+    DC_REQUIRE_DTYPE("dc_paged_attention");
+    int rc = check_heads(fn, a->tokens, a->q_heads, a->kv_heads, a->dim);
+    if (rc != DC_OK) return rc;
+    if (a->q_heads % a->kv_heads != 0)
+        return fail(DC_ERR_SHAPE, "%s: %d query heads do not share %d kv heads evenly", fn, a->q_heads, a->kv_heads);
+    if (a->dim % 8 != 0 || a->dim > 256) return fail(DC_ERR_UNSUPPORTED, "%s: dim=%d is no multiple of 8 up to 256", fn, a->dim);
+    if ((rc = check_pool(fn, a->streams, a->num_pages, a->page_size, a->max_pages, a->tokens, a->page_table, a->starts)) != DC_OK) return rc;
+    if (a->causal_block < 0) return fail(DC_ERR_SHAPE, "%s: causal_block=%d is negative", fn, a->causal_block);
+    if (!(a->scale == a->scale) || !(a->decay == a->decay)) return fail(DC_ERR_UNSUPPORTED, "%s: scale and decay must not be NaN", fn);
+    return DC_OK;
+}
+
+}  // namespace
+
+int dc_rotary(const dc_rotary_args *a, int dtype, void *stream) {
+    dc::kernel_log_reset();
+    const char *fn = "dc_rotary";
+    if (a == nullptr) return fail(DC_ERR_NULL, "%s: args is NULL", fn);
+    DC_REQUIRE_DTYPE("dc_rotary");
+    int rc = check_heads(fn, a->tokens, a->q_heads, a->keys != nullptr ? a->kv_heads : 1, a->dim);
+    if (rc != DC_OK) return rc;
+    if (a->dim > 1024) return fail(DC_ERR_UNSUPPORTED, "%s: dim=%d exceeds 1024", fn, a->dim);
+    if (a->axes < 1 || a->axes > 4) return fail(DC_ERR_SHAPE, "%s: axes=%d is not 1 .. 4", fn, a->axes);
+    int64_t turned = 0;
+    for (int i = 0; i < a->axes; ++i) {
+        if (a->sections[i] < 0 || a->sections[i] % 2 != 0)
+            return fail(DC_ERR_SHAPE, "%s: section %d of axis %d must be even and not negative", fn, a->sections[i], i);
+        turned += a->sections[i];
+    }
+    if (turned < 2 || turned > a->dim) return fail(DC_ERR_SHAPE, "%s: sections turn %lld of %d elements", fn, (long long)turned, a->dim);
+    if ((rc = check_rows(fn, "q", a->q, a->q_heads, a->dim, a->q_token_stride, a->q_head_stride, dtype)) != DC_OK) return rc;
+    if ((rc = check_rows(fn, "out", a->out, a->q_heads, a->dim, a->out_token_stride, a->out_head_stride, dtype)) != DC_OK) return rc;
+    DC_REQUIRE_PTR("dc_rotary", a->positions);
+    DC_REQUIRE_PTR("dc_rotary", a->frequencies);
+    DC_REQUIRE_ALIGNED("dc_rotary", a->positions, 4);
+    DC_REQUIRE_ALIGNED("dc_rotary", a->frequencies, 8);
+    const Span q(a->q, rows_span(a->tokens, a->q_heads, a->dim, a->q_token_stride, a->q_head_stride, dtype));
+    const Span out(a->out, rows_span(a->tokens, a->q_heads, a->dim, a->out_token_stride, a->out_head_stride, dtype));
+    if (q.meets(out) && a->q != a->out) {  // columns of one wider buffer may interleave, nothing else
+        const int64_t width = (int64_t)(a->q_heads - 1) * a->q_head_stride + a->dim, ts = a->q_token_stride;
+        const int64_t off = (static_cast<const char *>(a->q) - static_cast<const char *>(a->out)) / (int64_t)esize(dtype);
+        const int64_t column = ((off % ts) + ts) % ts;
+        if (ts != a->out_token_stride || a->q_head_stride != a->out_head_stride || column < width || column + width > ts)
+            return fail(DC_ERR_UNSUPPORTED, "%s: out overlaps q without being q", fn);
+    }
+    if (a->q == a->out && (a->q_token_stride != a->out_token_stride || a->q_head_stride != a->out_head_stride))
+        return fail(DC_ERR_UNSUPPORTED, "%s: out overlaps q without being q", fn);
+    if (a->keys != nullptr) {
+        if ((rc = check_pool(fn, a->streams, a->num_pages, a->page_size, a->max_pages, a->tokens, a->page_table, a->starts)) != DC_OK) return rc;
+        if ((rc = check_rows(fn, "k", a->k, a->kv_heads, a->dim, a->k_token_stride, a->k_head_stride, dtype)) != DC_OK) return rc;
+        if ((rc = check_rows(fn, "v", a->v, a->kv_heads, a->dim, a->v_token_stride, a->v_head_stride, dtype)) != DC_OK) return rc;
+        DC_REQUIRE_PTR("dc_rotary", a->values);
+        DC_REQUIRE_PTR("dc_rotary", a->slots);
+        DC_REQUIRE_ALIGNED("dc_rotary", a->keys, esize(dtype));
+        DC_REQUIRE_ALIGNED("dc_rotary", a->values, esize(dtype));
+        DC_REQUIRE_ALIGNED("dc_rotary", a->weights, 4);
+        DC_REQUIRE_ALIGNED("dc_rotary", a->stamps, 4);
+        DC_REQUIRE_ALIGNED("dc_rotary", a->token_stamps, 4);
+        DC_REQUIRE_ALIGNED("dc_rotary", a->slots, 4);
+        DC_REQUIRE_ALIGNED("dc_rotary", a->lens, 4);
+        if (a->lens != nullptr) DC_REQUIRE_PTR("dc_rotary", a->new_lens);
+        DC_REQUIRE_ALIGNED("dc_rotary", a->new_lens, 4);
+    }
+    return finish(dc::launch_rotary(*a, dtype, (hipStream_t)stream), fn);
+}
+
+int64_t dc_paged_attention_workspace(const dc_attention_args *a, int dtype) {
+    int rc = check_attention(a, dtype);
+    return rc != DC_OK ? rc : dc::paged_attention_workspace(*a, dtype);
+}
+
+int dc_paged_attention(const dc_attention_args *a, int dtype, void *stream) {
+    dc::kernel_log_reset();
+    const char *fn = "dc_paged_attention";
+    int rc = check_attention(a, dtype);
+    if (rc != DC_OK) return rc;
+    if ((rc = check_rows(fn, "q", a->q, a->q_heads, a->dim, a->q_token_stride, a->q_head_stride, dtype)) != DC_OK) return rc;
+    if ((rc = check_rows(fn, "out", a->out, a->q_heads, a->dim, a->out_token_stride, a->out_head_stride, dtype)) != DC_OK) return rc;
+    DC_REQUIRE_PTR("dc_paged_attention", a->keys);
+    DC_REQUIRE_PTR("dc_paged_attention", a->values);
+    DC_REQUIRE_PTR("dc_paged_attention", a->lens);
+    DC_REQUIRE_ALIGNED("dc_paged_attention", a->q, 16);
+    DC_REQUIRE_ALIGNED("dc_paged_attention", a->keys, 16);
+    DC_REQUIRE_ALIGNED("dc_paged_attention", a->values, 16);
+    DC_REQUIRE_ALIGNED("dc_paged_attention", a->lse, 4);
+    DC_REQUIRE_ALIGNED("dc_paged_attention", a->lens, 4);
+    DC_REQUIRE_ALIGNED("dc_paged_attention", a->weights, 4);
+    const int64_t vec = 16 / int64_t(esize(dtype));
+    if (a->q_token_stride % vec || a->q_head_stride % vec)
+        return fail(DC_ERR_ALIGN, "%s: rows of q are not aligned to 16 bytes", fn);
+    const Span q(a->q, rows_span(a->tokens, a->q_heads, a->dim, a->q_token_stride, a->q_head_stride, dtype));
+    const Span out(a->out, rows_span(a->tokens, a->q_heads, a->dim, a->out_token_stride, a->out_head_stride, dtype));
+    const size_t pool = size_t(a->num_pages) * a->kv_heads * a->page_size * a->dim * esize(dtype);
+    if (out.meets(q) || out.meets(Span(a->keys, pool)) || out.meets(Span(a->values, pool)))
+        return fail(DC_ERR_UNSUPPORTED, "%s: out overlaps an operand", fn);
+    const int64_t need = dc::paged_attention_workspace(*a, dtype);
+    if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need))
+        return fail(DC_ERR_NULL, "%s: needs %lld bytes of workspace", fn, (long long)need);
+    if (need > 0) DC_REQUIRE_ALIGNED("dc_paged_attention", a->workspace, 16);
+    return finish(dc::launch_paged_attention(*a, dtype, (hipStream_t)stream), fn);
+}
+
+int dc_cache_slots(const dc_slots_args *a, void *stream) {
+    dc::kernel_log_reset();
+    const char *fn = "dc_cache_slots";
+    if (a == nullptr) return fail(DC_ERR_NULL, "%s: args is NULL", fn);
+    int rc = check_heads(fn, a->tokens, 1, a->kv_heads, 1);
+    if (rc != DC_OK) return rc;
+    if ((rc = check_pool(fn, a->streams, a->num_pages, a->page_size, a->max_pages, a->tokens, a->page_table, a->starts)) != DC_OK) return rc;
+    if (a->budget <= 0 || a->budget > (int64_t)a->max_pages * a->page_size)
+        return fail(DC_ERR_SHAPE, "%s: budget=%d is not 1 .. %lld, the slots of a stream", fn, a->budget, (long long)a->max_pages * a->page_size);
+    DC_REQUIRE_PTR("dc_cache_slots", a->weights);
+    DC_REQUIRE_PTR("dc_cache_slots", a->lens);
+    DC_REQUIRE_PTR("dc_cache_slots", a->slots);
+    DC_REQUIRE_PTR("dc_cache_slots", a->new_lens);
+    if (a->stamps != nullptr) DC_REQUIRE_PTR("dc_cache_slots", a->keep_from);
+    DC_REQUIRE_ALIGNED("dc_cache_slots", a->weights, 4);
+    DC_REQUIRE_ALIGNED("dc_cache_slots", a->stamps, 4);
+    DC_REQUIRE_ALIGNED("dc_cache_slots", a->keep_from, 4);
+    DC_REQUIRE_ALIGNED("dc_cache_slots", a->lens, 4);
+    DC_REQUIRE_ALIGNED("dc_cache_slots", a->slots, 4);
+    DC_REQUIRE_ALIGNED("dc_cache_slots", a->new_lens, 4);
+    if (Span(a->lens, size_t(a->streams) * 4).meets(Span(a->new_lens, size_t(a->streams) * 4)))
+        return fail(DC_ERR_UNSUPPORTED, "%s: new_lens overlaps lens", fn);
+    return finish(dc::launch_cache_slots(*a, (hipStream_t)stream), fn);
+}
+
 }  // extern "C"

@@ -720,3 +720,234 @@ def sparse_concatenate(a, b, out=None):
           P=_pixels(a), C=a.shape[1], Cb=b.shape[1], esize=a.element_size(), in_mask=mask_a,
           in_mask_b=mask_b, out_mask=mask_out, keep=(a, b, out_t))
     return out_t, mask_out
+
+
+# ---- attention over the frames of a video stream (include/deltacnn_hip.h) ----
+
+def _expect(ok, message):
+    if not ok:
+        raise _lib.DeltaCNNError(-2, message)
+
+
+def _resident(name, device, **tensors):
+    """Every operand lives on the device of the call, and nothing asks for a gradient."""
+    for what, t in tensors.items():
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise _lib.DeltaCNNError(-4, f"{name}: {what} must be a tensor on the GPU")
+        _expect(t.device == device, f"{name}: {what} lives on {t.device}, the call on {device}")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise _lib.DeltaCNNError(-3, f"{name}: {what} asks for a gradient (the operator has none: call it under torch.no_grad())")
+
+
+def _words(name, what, t, shape, dtype=torch.int32):
+    if t is not None:
+        _expect(t.dtype == dtype and tuple(t.shape) == tuple(shape) and t.is_contiguous(),
+                f"{name}: {what} must be a dense {str(dtype)[6:]} tensor {tuple(shape)}, got {str(t.dtype)[6:]} {tuple(t.shape)}")
+
+
+def _rows(name, what, t, dtype=None, dim=None):
+    """Strides of [tokens][heads][dim] rows whose elements are dense; a dimension of one element may
+    have any stride in torch, and gets the dense one here."""
+    _expect(t.dim() == 3 and 0 not in t.shape, f"{name}: {what} must be [tokens, heads, dim], got {tuple(t.shape)}")
+    _expect(dtype is None or t.dtype == dtype, f"{name}: {what} is {str(t.dtype)[6:]}, expected {str(dtype)[6:]}")
+    _expect(dim is None or t.shape[2] == dim, f"{name}: {what} has {t.shape[2]} elements a head, expected {dim}")
+    tokens, heads, d = t.shape
+    _expect(t.stride(2) == 1 or d == 1, f"{name}: the elements of a head of {what} must be dense")
+    head = t.stride(1) if heads > 1 else d
+    return (t.stride(0) if tokens > 1 else max(heads * head, d)), head
+
+
+def _pool(name, keys, values, page_table, dtype):
+    _expect(keys.dim() == 4 and keys.is_contiguous() and 0 not in keys.shape,
+            f"{name}: keys must be a dense [pages, kv_heads, page_size, dim] tensor, got {tuple(keys.shape)}")
+    _expect(values.shape == keys.shape and values.is_contiguous(), f"{name}: values {tuple(values.shape)} do not match keys {tuple(keys.shape)}")
+    _expect(keys.dtype == dtype and values.dtype == dtype, f"{name}: the cache holds {str(keys.dtype)[6:]}, the call has {str(dtype)[6:]}")
+    _table(name, page_table)
+    return keys.shape
+
+
+def _table(name, page_table):
+    _expect(page_table.dim() == 2 and 0 not in page_table.shape and page_table.dtype == torch.int32 and page_table.is_contiguous(),
+            f"{name}: page_table must be a dense int32 [streams, pages of a stream] tensor")
+
+
+def rotary_frequencies(sections: Sequence[int], base: float = 10000.0, device=None) -> torch.Tensor:
+    """Angular frequencies of :func:`rotary` and :func:`rotary_append`: a ladder of its own for each
+    axis, ``base ** (-2 i / n)`` for pair ``i`` of the ``n`` rotated elements of that axis, as the
+    float64 tensor the operators take (a far position times a rounded frequency is a wrong angle)."""
+    _expect(len(sections) > 0 and all(int(n) >= 0 and int(n) % 2 == 0 for n in sections), f"rotary_frequencies: sections {tuple(sections)} must be even")
+    rows = [float(base) ** (-torch.arange(0, int(n), 2, dtype=torch.float64) / int(n)) for n in sections if int(n) > 0]
+    return torch.cat(rows).to(device) if rows else torch.empty(0, dtype=torch.float64, device=device)
+
+
+def _rotary_args(name, q, positions, frequencies, sections, interleaved, out):
+    sections = [int(n) for n in sections]
+    _expect(1 <= len(sections) <= 4, f"{name}: 1 .. 4 axes, got sections {tuple(sections)}")
+    a = _lib.RotaryArgs()
+    a.tokens, a.q_heads, a.dim = q.shape[0], q.shape[1], q.shape[2]
+    a.q_token_stride, a.q_head_stride = _rows(name, "q", q)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _expect(out.shape == q.shape, f"{name}: out {tuple(out.shape)} does not match q {tuple(q.shape)}")
+    a.out_token_stride, a.out_head_stride = _rows(name, "out", out, q.dtype)
+    _words(name, "positions", positions, (q.shape[0], len(sections)))
+    _words(name, "frequencies", frequencies, (sum(sections) // 2,), torch.float64)
+    a.q, a.out, a.positions, a.frequencies = q.data_ptr(), out.data_ptr(), positions.data_ptr(), frequencies.data_ptr()
+    a.axes = len(sections)
+    for i, n in enumerate(sections):
+        a.sections[i] = n
+    a.interleaved = int(bool(interleaved))
+    return a, out
+
+
+def rotary(x, positions, frequencies, sections, *, interleaved=False, inverse=False, out=None):
+    """Rotary positions with one to four axes (time, height, width, ..) on ``x`` [tokens, heads, dim],
+    which may be a view with dense elements: of the first ``sum(sections)`` elements of a head, pair
+    ``p`` -- ``(2 p, 2 p + 1)`` if ``interleaved``, else ``(p, p + sum(sections) / 2)`` -- turns by
+    ``positions[t, axis of p] * frequencies[p]``; axis ``a`` has ``sections[a] / 2`` pairs.
+    ``positions`` is int32 [tokens, axes], ``frequencies`` float64 (:func:`rotary_frequencies`).
+    ``inverse`` turns back, which is also how a gradient passes through.  ``out`` may be ``x``."""
+    lib = _lib.load()
+    _expect(isinstance(x, torch.Tensor) and x.dim() == 3, "rotary: x must be [tokens, heads, dim]")
+    _resident("rotary", x.device, x=x, positions=positions, frequencies=frequencies, out=out)
+    dt = _dtype(x)
+    a, out = _rotary_args("rotary", x, positions, frequencies, sections, interleaved, out)
+    a.inverse = int(bool(inverse))
+    with torch.cuda.device(x.device):
+        _call("rotary", lib.dc_rotary, (ctypes.byref(a), dt, _stream()), tokens=x.shape[0], q_heads=x.shape[1], kv_heads=0,
+              dim=x.shape[2], axes=len(sections), esize=x.element_size(), keep=(a, x, positions, frequencies, out))
+    return out
+
+
+def rotary_append(q, k, v, positions, frequencies, sections, keys, values, page_table, slots, *, starts=None, weights=None,
+                  stamps=None, token_stamps=None, lens=None, new_lens=None, interleaved=False, out=None):
+    """:func:`rotary` on the queries and keys of new tokens, and the write of the turned keys and the
+    values into a paged cache, in one launch.  Returns the turned queries (``out``; may be ``q``).
+
+    ``q`` [T, q_heads, dim], ``k`` and ``v`` [T, kv_heads, dim] may be views of one projection's output.
+    ``keys`` / ``values`` [pages, kv_heads, page_size, dim] and ``page_table`` [streams, pages of a
+    stream] are the cache; ``slots`` [kv_heads, T] (from :func:`cache_slots`) says where each token
+    goes in its stream, no slot twice.  ``starts`` [streams + 1] gives the first token of every stream
+    (default: T / streams each).  The slots' ``weights`` become 0 and their ``stamps`` the tokens'
+    (``token_stamps`` [T], default: the position on the first axis); ``lens`` receives ``new_lens``.
+    A token whose slot is negative, or lies in a page outside the pool, is not stored."""
+    lib = _lib.load()
+    name = "rotary_append"
+    _expect(isinstance(q, torch.Tensor) and q.dim() == 3, f"{name}: q must be [tokens, heads, dim]")
+    _resident(name, q.device, q=q, k=k, v=v, positions=positions, frequencies=frequencies, keys=keys, values=values,
+              page_table=page_table, slots=slots, starts=starts, weights=weights, stamps=stamps, token_stamps=token_stamps,
+              lens=lens, new_lens=new_lens, out=out)
+    dt = _dtype(q)
+    pages, kv, page, dim = _pool(name, keys, values, page_table, q.dtype)
+    a, out = _rotary_args(name, q, positions, frequencies, sections, interleaved, out)
+    tokens, streams = q.shape[0], page_table.shape[0]
+    _expect(q.shape[2] == dim, f"{name}: q has {q.shape[2]} elements a head, the cache {dim}")
+    _expect(k.shape == (tokens, kv, dim) and v.shape == (tokens, kv, dim),
+            f"{name}: k {tuple(k.shape)} and v {tuple(v.shape)} must be {(tokens, kv, dim)}")
+    a.k_token_stride, a.k_head_stride = _rows(name, "k", k, q.dtype)
+    a.v_token_stride, a.v_head_stride = _rows(name, "v", v, q.dtype)
+    _words(name, "slots", slots, (kv, tokens))
+    _words(name, "starts", starts, (streams + 1,))
+    _words(name, "weights", weights, (pages, kv, page), torch.float32)
+    _words(name, "stamps", stamps, (pages, kv, page))
+    _words(name, "token_stamps", token_stamps, (tokens,))
+    _words(name, "lens", lens, (streams,))
+    _words(name, "new_lens", new_lens, (streams,))
+    _expect(lens is None or new_lens is not None, f"{name}: lens without new_lens")
+    a.kv_heads, a.streams, a.num_pages, a.page_size, a.max_pages = kv, streams, pages, page, page_table.shape[1]
+    a.k, a.v, a.keys, a.values, a.page_table, a.slots = (t.data_ptr() for t in (k, v, keys, values, page_table, slots))
+    a.starts, a.weights, a.stamps, a.token_stamps, a.lens, a.new_lens = (
+        _ptr(t) for t in (starts, weights, stamps, token_stamps, lens, new_lens))
+    with torch.cuda.device(q.device):
+        _call("rotary_append", lib.dc_rotary, (ctypes.byref(a), dt, _stream()), tokens=tokens, q_heads=q.shape[1], kv_heads=kv,
+              dim=dim, axes=len(sections), esize=q.element_size(), with_weights=weights is not None, with_stamps=stamps is not None,
+              keep=(a, q, k, v, positions, frequencies, slots, starts, token_stamps, new_lens, out))
+    return out
+
+
+def paged_attention(q, keys, values, page_table, lens, *, starts=None, scale=None, causal_block=0, weights=None, decay=1.0,
+                    return_lse=False, out=None):
+    """Attention of new tokens ``q`` [T, q_heads, dim] over a paged cache that already holds them (see
+    :func:`rotary_append`); one token of a stream or a whole clip.  Returns ``out`` [T, q_heads, dim],
+    with ``return_lse`` also the log of every row's sum of exponentials, float32 [T, q_heads].
+
+    A token sees every slot in use of its stream, ``lens[b]`` of them; with ``causal_block = c`` the
+    new tokens are the last ``n`` slots in order, and token ``i`` sees slots below ``lens[b] - n +
+    (i // c + 1) * c`` (1: causal; the tokens of a frame: a frame sees itself and those before it).
+    A token that sees nothing gets zeros (and a log-sum of -inf); what is not visible has no influence,
+    NaN included; a stream that reads a page outside the pool gets NaN.  ``scale`` defaults to
+    ``dim ** -0.5``.  With ``weights`` [pages, kv_heads, page_size] float32 every slot in use also
+    receives ``weights = decay * weights + sum of its probabilities`` over the tokens and the query
+    heads that share its head; pages must then not be shared between streams."""
+    lib = _lib.load()
+    name = "paged_attention"
+    _expect(isinstance(q, torch.Tensor) and q.dim() == 3, f"{name}: q must be [tokens, heads, dim]")
+    _resident(name, q.device, q=q, keys=keys, values=values, page_table=page_table, lens=lens, starts=starts, weights=weights, out=out)
+    dt = _dtype(q)
+    pages, kv, page, dim = _pool(name, keys, values, page_table, q.dtype)
+    tokens, heads = q.shape[:2]
+    streams = page_table.shape[0]
+    a = _lib.AttentionArgs()
+    a.q_token_stride, a.q_head_stride = _rows(name, "q", q, dim=dim)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _expect(out.shape == q.shape, f"{name}: out {tuple(out.shape)} does not match q {tuple(q.shape)}")
+    a.out_token_stride, a.out_head_stride = _rows(name, "out", out, q.dtype)
+    _words(name, "lens", lens, (streams,))
+    _words(name, "starts", starts, (streams + 1,))
+    _words(name, "weights", weights, (pages, kv, page), torch.float32)
+    lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_lse else None
+    a.tokens, a.q_heads, a.kv_heads, a.dim = tokens, heads, kv, dim
+    a.streams, a.num_pages, a.page_size, a.max_pages = streams, pages, page, page_table.shape[1]
+    a.q, a.out, a.keys, a.values, a.page_table, a.lens = (t.data_ptr() for t in (q, out, keys, values, page_table, lens))
+    a.lse, a.starts, a.weights = _ptr(lse), _ptr(starts), _ptr(weights)
+    a.causal_block, a.decay = int(causal_block), float(decay)
+    a.scale = float(dim) ** -0.5 if scale is None else float(scale)
+    need = lib.dc_paged_attention_workspace(ctypes.byref(a), dt)
+    if need < 0:
+        _lib.check(int(need))
+    with torch.cuda.device(q.device):
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        a.workspace, a.workspace_bytes = _ptr(workspace), need
+        _call("paged_attention", lib.dc_paged_attention, (ctypes.byref(a), dt, _stream()), tokens=tokens, q_heads=heads, kv_heads=kv,
+              dim=dim, esize=q.element_size(), lens=lens, starts=starts, causal_block=int(causal_block),
+              with_weights=weights is not None, keep=(a, q, lse, out, workspace))
+    return (out, lse) if return_lse else out
+
+
+def cache_slots(weights, page_table, lens, tokens, budget, *, starts=None, stamps=None, keep_from=None):
+    """Where ``tokens`` new tokens go in a paged cache whose streams may use ``budget`` slots each: into
+    the slots of the tokens that have received the least attention, then behind the slots in use.
+    Returns ``(slots, new_lens)``, int32 [kv_heads, tokens] and [streams], for :func:`rotary_append`;
+    nothing is moved or changed.
+
+    Every kv head of a stream chooses for itself by ``weights`` [pages, kv_heads, page_size] (lowest
+    first, ties to the lowest slot, NaN last).  Tokens whose ``stamps`` are at least ``keep_from[b]``
+    (int32 [streams]) give way only after all others.  ``starts`` as in :func:`rotary_append`.  A
+    stream that already uses more than ``budget`` does not shrink; a token beyond it gets slot -1."""
+    lib = _lib.load()
+    name = "cache_slots"
+    _expect(isinstance(weights, torch.Tensor) and weights.dim() == 3 and 0 not in weights.shape, f"{name}: weights must be [pages, kv_heads, page_size]")
+    _resident(name, weights.device, weights=weights, page_table=page_table, lens=lens, starts=starts, stamps=stamps, keep_from=keep_from)
+    _words(name, "weights", weights, weights.shape, torch.float32)
+    _table(name, page_table)
+    pages, kv, page = weights.shape
+    streams, tokens, budget = page_table.shape[0], int(tokens), int(budget)
+    _expect(0 < tokens, f"{name}: tokens={tokens}")
+    _words(name, "lens", lens, (streams,))
+    _words(name, "starts", starts, (streams + 1,))
+    _words(name, "stamps", stamps, weights.shape)
+    _words(name, "keep_from", keep_from, (streams,))
+    _expect((stamps is None) == (keep_from is None), f"{name}: stamps and keep_from go together")
+    a = _lib.SlotsArgs()
+    a.streams, a.tokens, a.kv_heads, a.num_pages, a.page_size, a.max_pages, a.budget = streams, tokens, kv, pages, page, page_table.shape[1], budget
+    with torch.cuda.device(weights.device):
+        slots = torch.empty((kv, tokens), dtype=torch.int32, device=weights.device)
+        new_lens = torch.empty((streams,), dtype=torch.int32, device=weights.device)
+        a.weights, a.page_table, a.lens, a.slots, a.new_lens = (t.data_ptr() for t in (weights, page_table, lens, slots, new_lens))
+        a.starts, a.stamps, a.keep_from = _ptr(starts), _ptr(stamps), _ptr(keep_from)
+        _call("cache_slots", lib.dc_cache_slots, (ctypes.byref(a), _stream()), tokens=tokens, kv_heads=kv, lens=lens,
+              with_stamps=stamps is not None, keep=(a, starts, keep_from, slots, new_lens))
+    return slots, new_lens

@@ -482,6 +482,116 @@ int dc_mul_add(const void *input, const int32_t *mask, void *out, int32_t *mask_
                const void *scale, const void *bias, int32_t pixels, int32_t channels,
                int dtype, void *stream);
 
+/* ---- attention over the frames of a video stream ----
+ * No counterparts in the reference, whose layers look back one frame.  Every stream keeps the
+ * keys and values of earlier tokens (one token per position of a feature map) in PAGES of a pool:
+ *
+ *   keys, values  [num_pages][kv_heads][page_size][dim]   feature type, 16-byte aligned
+ *   weights       [num_pages][kv_heads][page_size]        fp32, attention received so far
+ *   stamps        [num_pages][kv_heads][page_size]        int32, when the token came (its frame)
+ *   page_table    [streams][max_pages] int32: slot s of stream b lies at place s % page_size of page
+ *                 page_table[b][s / page_size]; entries behind the slots in use are never read
+ *   lens          [streams] int32: slots in use.  All of it is device memory: nothing is read on
+ *                 the host, so a captured graph follows a stream from frame to frame.
+ *
+ * The new tokens of a call lie one stream after the other, T in all; starts [streams + 1] int32 says
+ * where each stream's begin (starts == NULL: T / streams each); tokens behind starts[streams] belong
+ * to no stream and what they index is left as it was.  The q_heads heads of a query share kv_heads
+ * heads of keys, q_heads / kv_heads consecutive ones each.  Strides are in elements; the innermost
+ * dimension is dense. */
+
+/* Operands of dc_rotary. */
+typedef struct dc_rotary_args {
+    int32_t tokens, q_heads, kv_heads, dim;
+    const void *q;                  /* [T][q_heads][dim] */
+    int64_t q_token_stride, q_head_stride;
+    void *out;                      /* rotated q; may be q itself */
+    int64_t out_token_stride, out_head_stride;
+    const int32_t *positions;       /* [T][axes] dense */
+    int32_t axes;                   /* 1 .. 4 */
+    int32_t sections[4];            /* rotated elements of each axis, even; the rest of a head is kept */
+    const double *frequencies;      /* [sum(sections) / 2] radians per position */
+    int32_t interleaved;            /* pairs (2i, 2i + 1), else (i, i + sum(sections) / 2) */
+    int32_t inverse;                /* turn backwards (the transposed rotation: its gradient) */
+    /* the cache part; keys == NULL: q alone is turned */
+    const void *k, *v;              /* [T][kv_heads][dim] */
+    int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    void *keys, *values;
+    float *weights;                 /* or NULL */
+    int32_t *stamps;                /* or NULL */
+    const int32_t *token_stamps;    /* [T]; NULL: the position on the first axis */
+    const int32_t *page_table;
+    const int32_t *slots;           /* [kv_heads][T]: where each token goes, distinct in a stream and head */
+    const int32_t *starts;          /* or NULL */
+    int32_t streams, num_pages, page_size, max_pages;
+    int32_t *lens;                  /* receives new_lens, or NULL */
+    const int32_t *new_lens;
+} dc_rotary_args;
+
+/* Rotary positions with 1 .. 4 axes (time, height, width, ..): pair p of a head, which belongs to
+ * axis a, turns by angle = positions[t][a] * frequencies[p]:
+ *   (x, y) -> (x cos - y sin, x sin + y cos),
+ * the angle and its reduction in 64 bits, sine, cosine and products in 32, one rounding at the end.
+ * With a cache the turned keys and the values go to their slots in the same launch, each slot's
+ * weight is set to 0, its stamp to the token's, and lens to new_lens.  A token whose slot is negative
+ * or lies in no page of the pool is not stored. */
+int dc_rotary(const dc_rotary_args *args, int dtype, void *stream);
+
+/* Operands of dc_paged_attention. */
+typedef struct dc_attention_args {
+    int32_t tokens, q_heads, kv_heads, dim; /* dim: multiple of 8 up to 256 */
+    const void *q;                  /* [T][q_heads][dim], 16-byte aligned rows */
+    int64_t q_token_stride, q_head_stride;
+    void *out;                      /* [T][q_heads][dim] */
+    int64_t out_token_stride, out_head_stride;
+    float *lse;                     /* [T][q_heads] log of each row's sum of exponentials, or NULL */
+    const void *keys, *values;
+    const int32_t *page_table, *lens, *starts;
+    int32_t streams, num_pages, page_size, max_pages;
+    int32_t causal_block;           /* 0: a token sees every slot in use */
+    float scale;
+    float *weights;                 /* or NULL */
+    float decay;
+    void *workspace;                /* dc_paged_attention_workspace bytes, 16-byte aligned */
+    int64_t workspace_bytes;
+} dc_attention_args;
+
+/* Attention of new tokens over a paged cache that already holds them:
+ *   out = sum_s p[s] values[s],  p = softmax over the visible slots s of scale * <q, keys[s]>.
+ * Token i of a stream's n sees slots [0, lens) or, with causal_block = c > 0 (the new tokens being
+ * the last n slots in order), slots below lens - n + (i / c + 1) * c: 1 is causal by tokens, the
+ * tokens of a frame make frames see themselves and the frames before them.  A token that sees
+ * nothing gets zeros and lse = -infinity.  Slots that are not visible never influence anything,
+ * whatever they hold.  A stream with a page outside the pool among the slots it reads gets NaN.
+ * With weights, every slot below lens receives, summed over the tokens and the heads that share it,
+ *   weights[s] = decay * weights[s] + sum p[s]          (decay 0: the old weight is not read);
+ * pages then belong to one stream each.  out must not overlap the operands.  Results do not depend
+ * on the order in which workgroups run. */
+int dc_paged_attention(const dc_attention_args *args, int dtype, void *stream);
+/* Bytes of workspace that the call needs (0: none; negative: a dc_status). */
+int64_t dc_paged_attention_workspace(const dc_attention_args *args, int dtype);
+
+/* Operands of dc_cache_slots. */
+typedef struct dc_slots_args {
+    const float *weights;
+    const int32_t *stamps;          /* or NULL: no token is protected */
+    const int32_t *keep_from;       /* [streams], with stamps */
+    const int32_t *page_table, *lens, *starts;
+    int32_t streams, tokens, kv_heads, num_pages, page_size, max_pages;
+    int32_t budget;                 /* slots a stream may use, at most max_pages * page_size */
+    int32_t *slots;                 /* [kv_heads][T] */
+    int32_t *new_lens;              /* [streams]; must not be lens */
+} dc_slots_args;
+
+/* Where the new tokens of every stream and kv head go: into the slots of the tokens that have
+ * received the least attention, then behind the slots in use.  With n = lens and c new tokens
+ * e = min(max(n + c - budget, 0), n, c) tokens give way: those not protected (stamp < keep_from)
+ * before those that are, the lowest weight first (-0 = +0, NaN above everything), ties to the lowest
+ * slot; a slot in no page of the pool gives way first.  slots lists them in ascending order, then
+ * n, n + 1, ..; a token without room below max(budget, n) gets -1.  new_lens = min(n + c - e,
+ * max(budget, n)).  No key or value moves, so a head's slots are in no order of time afterwards. */
+int dc_cache_slots(const dc_slots_args *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,274 @@
+"""Rotary positions into a paged cache, attention over it and the choice of slots for new tokens,
+against the 64-bit definition in frame_reference (bounds derived there)."""
+import math
+
+import pytest
+import torch
+
+import frame_reference as ref
+from util import DEV
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float16, torch.bfloat16, torch.float32]
+ids = lambda t: str(t)[6:] if isinstance(t, torch.dtype) else None  # noqa: E731
+
+
+def make_pool(gen, streams, slots, kv, page, dim, dtype, spare=3):
+    """Keys, values, weights, stamps and a page table whose pages are shuffled; what lies in no slot is NaN."""
+    per = max(1, -(-slots // page))
+    pages = streams * per + spare
+    table = torch.randperm(pages, generator=gen)[:streams * per].view(streams, per).to(torch.int32)
+    keys = torch.randn(pages, kv, page, dim, generator=gen).to(dtype)
+    values = torch.randn(pages, kv, page, dim, generator=gen).to(dtype)
+    weights = torch.rand(pages, kv, page, generator=gen)
+    stamps = torch.randint(0, 9, (pages, kv, page), generator=gen, dtype=torch.int32)
+    return keys, values, weights, stamps, table
+
+
+def poison_unused(keys, values, weights, table, lens, page):
+    """NaN wherever no stream has a slot in use."""
+    used = torch.zeros(keys.shape[0], page, dtype=torch.bool)
+    for b, n in enumerate(lens):
+        for s in range(n):
+            used[int(table[b, s // page]), s % page] = True
+    hole = ~used[:, None, :]
+    keys.masked_fill_(hole[..., None], math.nan)
+    values.masked_fill_(hole[..., None], math.nan)
+    weights.masked_fill_(hole, math.nan)
+
+
+def starts_of(counts):
+    s = [0]
+    for c in counts:
+        s.append(s[-1] + c)
+    return torch.tensor(s, dtype=torch.int32)
+
+
+# ---- rotary ----
+
+ROTARY = [  # tokens, heads, dim, sections
+    (1, 1, 8, (8,)), (3, 2, 64, (16, 24, 24)), (33, 5, 128, (32, 48, 48)), (7, 3, 40, (10, 6)), (5, 1, 30, (2, 4, 6, 8)),
+    (257, 4, 96, (0, 48, 48)), (19, 2, 72, (72,)), (2, 7, 256, (64, 64)), (65, 1, 17, (6,)),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("shape", ROTARY, ids=str)
+def test_rotary(lib, dtype, interleaved, shape):
+    from deltacnn_amd import hip_kernels as hk
+    tokens, heads, dim, sections = shape
+    gen = torch.Generator().manual_seed(41 + tokens)
+    x = torch.randn(tokens, heads, dim, generator=gen).to(dtype)
+    pos = torch.randint(-5000000, 5000000, (tokens, len(sections)), generator=gen, dtype=torch.int32)
+    freq = hk.rotary_frequencies(sections, device=DEV)
+    for inverse in (False, True):
+        want, tol = ref.rotary(x, pos, freq, sections, interleaved, inverse)
+        got = hk.rotary(x.to(DEV), pos.to(DEV), freq, sections, interleaved=interleaved, inverse=inverse)
+        ref.assert_within(got, want, tol, f"inverse={inverse}")
+    # a strided view (heads in the outer dimension), in place
+    buf = torch.full((heads + 1, tokens, dim + 3), 7.0, dtype=dtype, device=DEV)
+    view = buf[1:, :, :dim].transpose(0, 1)
+    view.copy_(x)
+    got = hk.rotary(view, pos.to(DEV), freq, sections, interleaved=interleaved, out=view)
+    want, tol = ref.rotary(x, pos, freq, sections, interleaved)
+    ref.assert_within(view, want, tol, "in place")
+    assert got.data_ptr() == view.data_ptr() and bool((buf[0] == 7).all()) and bool((buf[:, :, dim:] == 7).all())
+
+
+def test_rotary_back_and_forth_and_its_gradient(lib):
+    """inverse undoes the rotation, and is its transpose: <R x, y> = <x, R^-1 y>."""
+    from deltacnn_amd import hip_kernels as hk
+    gen = torch.Generator().manual_seed(5)
+    sections, tokens = (8, 12, 12), 50
+    x, y = (torch.randn(tokens, 3, 32, generator=gen).to(DEV) for _ in range(2))
+    pos = torch.randint(0, 2000, (tokens, 3), generator=gen, dtype=torch.int32).to(DEV)
+    freq = hk.rotary_frequencies(sections, device=DEV)
+    turned = hk.rotary(x, pos, freq, sections)
+    back = hk.rotary(turned, pos, freq, sections, inverse=True)
+    # two turns of the bound of frame_reference.rotary: 2 * (7 + 1) w (|a| + |b|), |a| + |b| < 12
+    assert float((back - x).abs().max()) < 16 * ref.W * 12
+    lhs = (turned.double() * y.double()).sum()
+    rhs = (x.double() * hk.rotary(y, pos, freq, sections, inverse=True).double()).sum()
+    bound = 16 * ref.W * 2 * float((x.abs() * y.abs()).sum() + x.abs().sum() * 6)
+    assert abs(float(lhs - rhs)) < bound
+
+
+# ---- rotary_append ----
+
+APPEND = [  # counts of new tokens, q_heads, kv_heads, dim, page, sections
+    ([1], 4, 2, 64, 16, (16, 24, 24)), ([5, 5], 3, 3, 32, 7, (32,)), ([3, 0, 9], 8, 1, 128, 64, (32, 48, 48)),
+    ([40, 1, 2, 17], 5, 5, 40, 30, (10, 6)), ([300], 2, 1, 96, 49, (48, 48)), ([70, 70, 70], 6, 2, 72, 1, (2, 2, 2)),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("shape", APPEND, ids=str)
+def test_rotary_append(lib, dtype, shape):
+    from deltacnn_amd import hip_kernels as hk
+    counts, heads, kv, dim, page, sections = shape
+    gen = torch.Generator().manual_seed(77 + sum(counts))
+    tokens, streams = sum(counts), len(counts)
+    behind = 3 if len(set(counts)) > 1 else 0  # tokens behind the last stream's
+    total = tokens + behind
+    slots_of = max(counts) + 11
+    keys, values, weights, stamps, table = make_pool(gen, streams, slots_of, kv, page, dim, dtype)
+    fused = torch.randn(total, (heads + 2 * kv) * dim, generator=gen).to(dtype)
+    q = fused[:, :heads * dim].view(total, heads, dim)
+    k = fused[:, heads * dim:(heads + kv) * dim].view(total, kv, dim)
+    v = fused[:, (heads + kv) * dim:].view(total, kv, dim)
+    pos = torch.randint(0, 100000, (total, len(sections)), generator=gen, dtype=torch.int32)
+    starts = starts_of(counts)
+    slots = torch.full((kv, total), -1, dtype=torch.int32)
+    for b, (first, count) in enumerate(ref.spans(starts, streams, tokens)):
+        for h in range(kv):
+            slots[h, first:first + count] = torch.randperm(slots_of, generator=gen)[:count].to(torch.int32)
+    if behind:
+        slots[:, tokens:] = 0
+    slots[0, 0] = -1                                       # a token that is not stored in head 0
+    if tokens > 2:
+        slots[kv - 1, 1] = table.shape[1] * page + 5       # ... and one beyond the stream's pages
+    lost = int(table[streams - 1, 0])
+    if streams > 1:
+        table[streams - 1, 0] = 10 ** 6                    # a page outside the pool
+    freq = hk.rotary_frequencies(sections)
+    new_lens = torch.arange(1, streams + 1, dtype=torch.int32)
+    want_q, q_tol = ref.rotary(q, pos, freq, sections, False)
+    want_k, k_tol = ref.rotary(k, pos, freq, sections, False)
+    wk, wv, ww, ws = keys.double(), values.clone(), weights.clone(), stamps.clone()
+    tol = torch.zeros_like(wk)
+    for b, (first, count) in enumerate(ref.spans(starts, streams, tokens)):
+        for t in range(first, first + count):
+            for h in range(kv):
+                s = int(slots[h, t])
+                if s < 0 or s >= table.shape[1] * page or not 0 <= int(table[b, s // page]) < keys.shape[0]:
+                    continue
+                pg, off = ref.place(table[b], s, page)
+                wk[pg, h, off], tol[pg, h, off], wv[pg, h, off] = want_k[t, h], k_tol[t, h], v[t, h]
+                ww[pg, h, off], ws[pg, h, off] = 0.0, pos[t, 0]
+    d = {n: t.to(DEV) for n, t in dict(fused=fused, pos=pos, freq=freq, keys=keys, values=values, weights=weights, stamps=stamps,
+                                       table=table, slots=slots, starts=starts, new=new_lens).items()}
+    f = d["fused"]
+    lens = torch.zeros(streams, dtype=torch.int32, device=DEV)
+    got = hk.rotary_append(f[:, :heads * dim].view(total, heads, dim), f[:, heads * dim:(heads + kv) * dim].view(total, kv, dim),
+                           f[:, (heads + kv) * dim:].view(total, kv, dim), d["pos"], d["freq"], sections, d["keys"], d["values"],
+                           d["table"], d["slots"], starts=d["starts"] if len(set(counts)) > 1 else None, weights=d["weights"],
+                           stamps=d["stamps"], lens=lens, new_lens=d["new"])
+    ref.assert_within(got, want_q, q_tol, "q")
+    ref.assert_within(d["keys"], wk, tol, "keys")
+    assert torch.equal(d["values"].cpu(), wv) and torch.equal(d["weights"].cpu(), ww) and torch.equal(d["stamps"].cpu(), ws)
+    assert lens.tolist() == new_lens.tolist()
+    assert lost >= 0 and torch.equal(f.cpu(), fused)  # the inputs are left alone
+    # stamps of the caller's own; no weights, no lens; q in place
+    own = torch.arange(total, dtype=torch.int32, device=DEV) + 1000
+    ws2 = ws.clone()
+    for b, (first, count) in enumerate(ref.spans(starts, streams, tokens)):
+        for t in range(first, first + count):
+            for h in range(kv):
+                s = int(slots[h, t])
+                if 0 <= s < table.shape[1] * page and 0 <= int(table[b, s // page]) < keys.shape[0]:
+                    pg, off = ref.place(table[b], s, page)
+                    ws2[pg, h, off] = 1000 + t
+    qv = f[:, :heads * dim].view(total, heads, dim)
+    hk.rotary_append(qv, f[:, heads * dim:(heads + kv) * dim].view(total, kv, dim), f[:, (heads + kv) * dim:].view(total, kv, dim),
+                     d["pos"], d["freq"], sections, d["keys"], d["values"], d["table"], d["slots"],
+                     starts=d["starts"] if len(set(counts)) > 1 else None, stamps=d["stamps"], token_stamps=own, out=qv)
+    ref.assert_within(qv, want_q, q_tol, "q in place")
+    assert torch.equal(d["stamps"].cpu(), ws2)
+
+
+# ---- paged_attention ----
+
+ATTEND = [  # counts, lens, q_heads, kv_heads, dim, page, causal_block
+    ([1], [1], 1, 1, 8, 1, 0),
+    ([1], [200], 5, 1, 64, 16, 0),
+    ([1, 1, 1], [77, 0, 300], 8, 2, 128, 64, 0),
+    ([1] * 9, [3, 64, 65, 63, 128, 1, 190, 5, 17], 4, 4, 40, 30, 0),
+    ([4], [67], 2, 1, 32, 7, 0),
+    ([49], [150], 4, 2, 64, 49, 0),
+    ([49], [150], 4, 2, 64, 49, 7),
+    ([33, 0, 70], [40, 20, 70], 3, 3, 96, 13, 1),
+    ([130], [130], 2, 2, 64, 64, 1),
+    ([130], [100], 2, 1, 64, 64, 1),           # more new tokens than slots: the first rows see nothing
+    ([20], [9], 1, 1, 16, 4, 6),
+    ([64, 64], [256, 256], 2, 2, 128, 64, 16),
+    ([1], [1500], 16, 1, 256, 100, 0),
+    ([90], [333], 1, 1, 256, 33, 30),
+    ([2, 1, 3], [500, 31, 129], 20, 4, 72, 77, 0),
+    ([300], [700], 2, 2, 128, 64, 0),
+    ([17], [1100], 8, 8, 64, 196, 1),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("shape", ATTEND, ids=str)
+def test_paged_attention(lib, dtype, shape):
+    from deltacnn_amd import hip_kernels as hk
+    counts, lens, heads, kv, dim, page, block = shape
+    gen = torch.Generator().manual_seed(1000 + sum(counts) + sum(lens))
+    tokens, streams = sum(counts), len(counts)
+    keys, values, weights, _, table = make_pool(gen, streams, max(max(lens), 1) + page, kv, page, dim, dtype)
+    poison_unused(keys, values, weights, table, lens, page)
+    q = (1.5 * torch.randn(tokens, heads, dim, generator=gen)).to(dtype)
+    ragged = len(set(counts)) > 1
+    starts = starts_of(counts)
+    for b, n in enumerate(lens):  # entries behind the slots in use are never read
+        table[b, -(-n // page):] = -12345
+    lens_t = torch.tensor(lens, dtype=torch.int32)
+    out, tol, lse, lse_tol, ww, w_tol = ref.attention(q, keys, values, table, lens_t, starts, None, block, weights, 0.75)
+    dev = [t.to(DEV) for t in (q, keys, values, table, lens_t)]
+    kw = dict(starts=starts.to(DEV) if ragged else None, causal_block=block)
+    got, got_lse = hk.paged_attention(*dev, return_lse=True, **kw)
+    ref.assert_within(got, out, tol, "out")
+    ref.assert_within(got_lse, lse, lse_tol, "lse")
+    w = weights.to(DEV)
+    again, again_lse = hk.paged_attention(*dev, weights=w, decay=0.75, return_lse=True, **kw)
+    ref.assert_within(again, out, tol, "out with weights")
+    ref.assert_within(again_lse, lse, lse_tol, "lse with weights")
+    ref.assert_within(w, ww, w_tol, "weights")
+    # decay 0 reads no old weight; the log-sum stays inside
+    w = torch.full_like(weights, math.nan).to(DEV)
+    again = hk.paged_attention(*dev, weights=w, decay=0.0, **kw)
+    want0, tol0 = ref.attention(q, keys, values, table, lens_t, starts, None, block, torch.full_like(weights, math.nan), 0.0)[4:]
+    ref.assert_within(again, out, tol, "out with weights, decay 0")
+    ref.assert_within(w, want0, tol0, "weights, decay 0")
+
+
+# ---- cache_slots ----
+
+SLOTS = [  # counts, lens, budget, kv_heads, page, protect
+    ([1], [1], 1, 1, 1, None), ([5], [20], 20, 2, 7, None), ([5], [20], 22, 2, 7, 6), ([5], [20], 64, 1, 64, 6),
+    ([3, 0, 7], [50, 9, 1], 50, 3, 16, 5), ([40], [40], 40, 2, 49, 3), ([9], [64], 64, 1, 64, 0),  # all protected
+    ([200], [1000], 1000, 2, 100, 8), ([64, 64], [2500, 2499], 2500, 1, 64, 7), ([30], [10], 20, 1, 30, None),
+    ([12, 12], [100, 3], 40, 1, 10, 4),       # one stream is over its budget already: it does not shrink
+]
+
+
+@pytest.mark.parametrize("kind", ["random", "ties", "odd"])
+@pytest.mark.parametrize("shape", SLOTS, ids=str)
+def test_cache_slots(lib, kind, shape):
+    from deltacnn_amd import hip_kernels as hk
+    counts, lens, budget, kv, page, protect = shape
+    gen = torch.Generator().manual_seed(9 + sum(counts))
+    streams = len(counts)
+    _, _, weights, stamps, table = make_pool(gen, streams, max(max(lens), budget), kv, page, 8, torch.float16)
+    if kind == "ties":
+        weights = torch.randint(0, 3, weights.shape, generator=gen).float()
+    if kind == "odd":
+        pick = torch.randint(0, 7, weights.shape, generator=gen)
+        special = torch.tensor([0.0, -0.0, math.nan, math.inf, -math.inf, 1e-42, -3.0])
+        weights = torch.where(torch.rand(weights.shape, generator=gen) < 0.6, special[pick], weights)
+        if streams > 1:
+            table[0, 0] = -1
+    starts = starts_of(counts)
+    lens_t = torch.tensor(lens, dtype=torch.int32)
+    keep = None if protect is None else torch.full((streams,), protect, dtype=torch.int32)
+    st = None if protect is None else stamps
+    total = sum(counts) + (2 if len(set(counts)) > 1 else 0)
+    want, new = ref.slots(weights, table, lens_t, total, budget, starts, st, keep)
+    on = lambda t: None if t is None else t.to(DEV)  # noqa: E731
+    got, got_new = hk.cache_slots(on(weights), on(table), on(lens_t), total, budget, starts=on(starts) if len(set(counts)) > 1 else None,
+                                  stamps=on(st), keep_from=on(keep))
+    n = sum(counts)
+    assert torch.equal(got.cpu()[:, :n], want[:, :n]) and torch.equal(got_new.cpu(), new)
