@@ -13,6 +13,7 @@ struct AttnPlan {
     PagePool pool;
     int32_t tokens, q_heads, kv_heads, dim, group, streams, causal_block;
     float scale, decay;
+    uint32_t flip;  // sign bits of a pair of 16-bit elements, or 0
     int64_t qt, qh, ot, oh;
 };
 
@@ -114,36 +115,665 @@ attention_weights_kernel(AttnPlan p, const T *__restrict__ q, const float *__res
     weights[row] = p.decay == 0.f ? received : fmaf(p.decay, weights[row], received);
 }
 
+typedef float float16_t __attribute__((ext_vector_type(16)));
+typedef float float2v_t __attribute__((ext_vector_type(2)));
+typedef half_t half2v_t __attribute__((ext_vector_type(2)));
+typedef bf16_t bf16x2_t __attribute__((ext_vector_type(2)));
+typedef short short4_t __attribute__((ext_vector_type(4)));
+#define DC_LDS(T) __attribute__((address_space(3))) T
+#define DC_GLOBAL(T) __attribute__((address_space(1))) T
+
+// 32 x 32 outputs, 16 reduction elements.  Operand A: lane (half, m) holds A[m][8 half + i]; operand B the
+// same of its columns; result: lane (half, n) holds rows 8 (r / 4) + 4 half + r % 4 of column n, r = 0 .. 15.
+__device__ __forceinline__ float16_t mfma32(half8_t a, half8_t b, float16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ float16_t mfma32(bf16x8_t a, bf16x8_t b, float16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+
+__device__ __forceinline__ uint32_t pack2(float a, float b, half_t) { return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2v_t{a, b}), half2v_t)); }
+__device__ __forceinline__ uint32_t pack2(float a, float b, bf16_t) { return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2v_t{a, b}), bf16x2_t)); }
+
+template <typename E>
+constexpr uint32_t EXP_BITS = 0x7c00u;
+template <>
+constexpr uint32_t EXP_BITS<bf16_t> = 0x7f80u;
+
+// The larger of the two halves' values, in both.
+__device__ __forceinline__ float max_halves(float x) {
+    const uint32_t u = __float_as_uint(x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_halves(float x) {
+    const uint32_t u = __float_as_uint(x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ const uint4 zero_chunk = {0, 0, 0, 0};
+
+// Where a workgroup's rows and slots are.  A ROW is one (token, head of the group) pair of a stream and
+// kv head: row r is token r / group, query head h * group + r % group, so the heads that share keys
+// share their tiles too.
+struct AttnGrid {
+    int32_t block_rows;     // rows of a workgroup
+    int32_t stream_blocks;  // row blocks of a stream (no starts)
+    int32_t flat;           // row blocks of all streams (an upper bound with starts)
+    int32_t splits;         // pieces of the slot axis
+    int32_t split_keys;     // slots of a piece
+    int32_t unit;           // consecutive row blocks that run on one XCD
+    FastDiv by_group, by_unit, by_flat, by_blocks, by_kv;
+    float *part;            // [splits][T * q_heads][dim] sums over a piece, [splits][T * q_heads][2] their maximum and normaliser behind
+};
+
+struct Work {
+    int b, h, split, rb, first, count;
+};
+
+// Row block f of all streams -> stream and block, a wavefront at a time over the streams.
+__device__ __forceinline__ bool find_block(const int32_t *starts, const AttnPlan &p, const AttnGrid &g, int f, Work &w) {
+    if (starts == nullptr) {
+        w.b = int(g.by_blocks.quot(f));
+        w.rb = f - w.b * g.stream_blocks;
+        w.count = p.tokens / p.streams;
+        w.first = w.b * w.count;
+    } else {
+        int base = 0;
+        bool hit = false;
+        for (int b0 = 0; b0 < p.streams && !hit; b0 += WAVE) {
+            const int b = b0 + lane_id();
+            int first = 0, count = 0;
+            if (b < p.streams) stream_tokens(starts, b, p.streams, p.tokens, first, count);
+            const int nb = int((int64_t(count) * p.group + g.block_rows - 1) / g.block_rows);
+            int sum = nb;
+#pragma unroll
+            for (int d = 1; d < WAVE; d <<= 1) {
+                const int o = __shfl_up(sum, d, WAVE);
+                if (lane_id() >= d) sum += o;
+            }
+            const bool mine = f >= base + sum - nb && f < base + sum;
+            const uint64_t who = ballot(mine);
+            if (who != 0) {
+                const int l = __ffsll((unsigned long long)who) - 1;
+                w.b = b0 + l;
+                w.rb = f - (base + __shfl(sum - nb, l, WAVE));
+                w.first = __shfl(first, l, WAVE);
+                w.count = __shfl(count, l, WAVE);
+                hit = true;
+            }
+            base += __shfl(sum, WAVE - 1, WAVE);
+        }
+        if (!hit) return false;
+        w.b = __builtin_amdgcn_readfirstlane(w.b), w.rb = __builtin_amdgcn_readfirstlane(w.rb);
+        w.first = __builtin_amdgcn_readfirstlane(w.first), w.count = __builtin_amdgcn_readfirstlane(w.count);
+    }
+    return true;
+}
+
+// Workgroups go to the 8 XCDs in turn, each with an L2 of its own: units of consecutive row blocks, which
+// read the same keys and values, stay on one.
+__device__ __forceinline__ bool find_work(const int32_t *starts, const AttnPlan &p, const AttnGrid &g, Work &w) {
+    const int x = blockIdx.x & 7, j = blockIdx.x >> 3;
+    const int u = int(g.by_unit.quot(j));
+    const int o = (x + 8 * u) * g.unit + (j - u * g.unit);
+    const int pair = int(g.by_flat.quot(o));
+    if (pair >= p.kv_heads * g.splits) return false;
+    w.split = int(g.by_kv.quot(pair));
+    w.h = pair - w.split * p.kv_heads;
+    if (!find_block(starts, p, g, o - pair * g.flat, w)) return false;
+    if (p.causal_block != 0) {  // the longest rows first
+        const int blocks = int((int64_t(w.count) * p.group + g.block_rows - 1) / g.block_rows);
+        w.rb = blocks - 1 - w.rb;
+    }
+    return true;
+}
+
+// BN slots of one head on their way into LDS, 16 bytes a lane and request, straight from memory.  Row r of
+// a tile is DP elements; its 16-byte chunk c lies at place c ^ swizzle(r), so that the reads below touch
+// every bank once (the lanes choose what they fetch, the places they fill are fixed).  What lies behind
+// `end` or in no page of the pool, and the elements from dim to DP, arrive as zeros.
+template <typename E, int DP, int BN, int LOADERS, bool ALIGNED>
+struct TileLoader {
+    static constexpr int CPR = DP / 8, RPI = WAVE / CPR, REQ = BN / RPI / LOADERS;
+    static_assert(REQ >= 1, "one request a wavefront at least");
+    int row0, kchunk[2], vchunk, dim;
+    bool bad = false;
+
+    static __device__ __forceinline__ int kswz(int row) { return row & 7; }
+    static __device__ __forceinline__ int vswz(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
+
+    __device__ __forceinline__ void init(int loader, int dim_) {
+        dim = dim_;
+        row0 = loader * REQ * RPI + lane_id() / CPR;
+    }
+    __device__ __forceinline__ void request(const AttnPlan &p, const int32_t *table, const E *keys, const E *values, int h, int k0, int end,
+                                            char *kt, char *vt, int loader) {
+        const int c = lane_id() % CPR;
+        if constexpr (ALIGNED) {
+            const int i = int(p.pool.by_page.quot(uint32_t(k0)));
+            const int page = __builtin_amdgcn_readfirstlane(table[i]);
+            const bool ok = uint32_t(page) < uint32_t(p.pool.num_pages);
+            bad = bad || !ok;
+            const int64_t base = ok ? ((int64_t(page) * p.kv_heads + h) * p.pool.page_size + (k0 - i * p.pool.page_size)) * dim : 0;
+            const int bytes = ok ? min(BN, end - k0) * dim * 2 : 0;
+            const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<E *>(keys) + base, 0, bytes, 0x00027000);
+            const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<E *>(values) + base, 0, bytes, 0x00027000);
+#pragma unroll
+            for (int j = 0; j < REQ; ++j) {
+                const int row = row0 + j * RPI, ck = c ^ kswz(row);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (DC_LDS(void) *)(kt + (loader * REQ + j) * 1024), 16,
+                                                         ck * 8 < dim ? (row * dim + ck * 8) * 2 : 0x40000000, 0, 0, 0);
+            }
+#pragma unroll
+            for (int j = 0; j < REQ; ++j) {
+                const int row = row0 + j * RPI, cv = c ^ vswz(row);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (DC_LDS(void) *)(vt + (loader * REQ + j) * 1024), 16,
+                                                         cv * 8 < dim ? (row * dim + cv * 8) * 2 : 0x40000000, 0, 0, 0);
+            }
+        } else {
+            const E *zero = reinterpret_cast<const E *>(&zero_chunk);
+            const E *kp[REQ], *vp[REQ];
+#pragma unroll
+            for (int j = 0; j < REQ; ++j) {
+                const int row = row0 + j * RPI, s = k0 + row;
+                int64_t at = -1;
+                if (s < end) {
+                    at = slot_row(p.pool, table, s, p.kv_heads, h);
+                    bad = bad || at < 0;
+                }
+                const int ck = c ^ kswz(row), cv = c ^ vswz(row);
+                kp[j] = at >= 0 && ck * 8 < dim ? keys + at * dim + ck * 8 : zero;
+                vp[j] = at >= 0 && cv * 8 < dim ? values + at * dim + cv * 8 : zero;
+            }
+#pragma unroll
+            for (int j = 0; j < REQ; ++j)
+                __builtin_amdgcn_global_load_lds((const DC_GLOBAL(void) *)kp[j], (DC_LDS(void) *)(kt + (loader * REQ + j) * 1024), 16, 0, 0);
+#pragma unroll
+            for (int j = 0; j < REQ; ++j)
+                __builtin_amdgcn_global_load_lds((const DC_GLOBAL(void) *)vp[j], (DC_LDS(void) *)(vt + (loader * REQ + j) * 1024), 16, 0, 0);
+        }
+    }
+};
+
+// The running state of 32 rows over the slots seen so far.  Scores are computed transposed, S^T = K Q^T,
+// so that a lane holds one row's scores for half of the slots: the maximum and the sum of a row are
+// sums over a lane's own registers, and the probabilities leave the first product in exactly the
+// places in which the second one, O^T += V^T P^T, wants them, if V's slots are taken in the order in
+// which a lane holds them (the order of a sum's terms is free).  V^T comes from LDS through the
+// transposing read.
+template <typename E, int DP, int BN>
+struct RowState {
+    typedef typename Elem16<E>::v8 v8;
+    static constexpr int BLK = BN / 32, STEPS = DP / 16, DB = DP / 32;
+    float16_t o[DB];
+    float m, l;
+    v8 q[STEPS];
+
+    __device__ __forceinline__ void init() {
+        m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+    }
+
+    // V^T fragment of 32 elements x 16 slots: slots 16 t + 8 e + 4 half + i of the tile in element 4 e + i
+    static __device__ __forceinline__ v8 vfrag(const char *vt, int t, int d, const int *voff) {
+        union {
+            short4_t h[2];
+            v8 v;
+        } f;
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            f.h[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DC_LDS(short4_t) *)(vt + voff[d] + (16 * t + 8 * e) * DP * 2));
+        return f.v;
+    }
+
+    // One tile: slots [k0, k0 + BN); this lane's row sees slots below `limit` (MASK: some of the tile's are not seen by some row)
+    template <bool MASK>
+    __device__ __forceinline__ void step(const char *kt, const char *vt, const int *koff, const int *voff, float scale, int k0, int limit) {
+        float16_t s[BLK];
+#pragma unroll
+        for (int b = 0; b < BLK; ++b) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[b][r] = 0.f;
+#pragma unroll
+            for (int t = 0; t < STEPS; ++t)
+                s[b] = mfma32(*reinterpret_cast<const v8 *>(kt + koff[t] + b * 32 * DP * 2), q[t], s[b]);
+        }
+        const int half = lane_id() >> 5;
+        if constexpr (MASK) {
+#pragma unroll
+            for (int b = 0; b < BLK; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (k0 + 32 * b + 8 * (r / 4) + 4 * half + r % 4 >= limit) s[b][r] = -INFINITY;
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int b = 0; b < BLK; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
+        top = max_halves(top) * scale;
+        // The reference of the exponentials follows the maximum only when that outgrows it by 2^8: any
+        // reference gives the same quotient, and a step without a new one leaves the sums alone.
+        if (ballot(top > m + 8.f) != 0) {
+            const float m2 = fmaxf(m, top), fade = m2 == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - m2);
+            m = m2;
+            l *= fade;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[d][r] *= fade;
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+        // probabilities: the sum in fp32, the product's operand rounded to the 16-bit type (half a step of
+        // it relative to each, the same as the values they multiply carry)
+        v8 pr[BLK][2];
+#pragma unroll
+        for (int b = 0; b < BLK; ++b)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                union {
+                    uint32_t u[4];
+                    v8 v;
+                } f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float a = __builtin_amdgcn_exp2f(fmaf(s[b][8 * t + 2 * i], scale, -ref));
+                    const float c = __builtin_amdgcn_exp2f(fmaf(s[b][8 * t + 2 * i + 1], scale, -ref));
+                    l += a;
+                    l += c;
+                    f.u[i] = pack2(a, c, E());
+                }
+                pr[b][t] = f.v;
+            }
+        if constexpr (MASK) {
+            // Slots that some rows see and others do not may hold infinities or NaN, and 0 * inf would carry
+            // them over: such elements leave the product and join the rows that see them one by one.
+            bool odd = false;
+#pragma unroll
+            for (int t = 0; t < BN / 16; ++t)
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    const v8 v = vfrag(vt, t, d, voff);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) odd = odd || (__builtin_bit_cast(uint16_t, E(v[i])) & EXP_BITS<E>) == EXP_BITS<E>;
+                }
+            if (ballot(odd) != 0) {
+#pragma unroll 1
+                for (int t = 0; t < BN / 16; ++t)
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) {
+                        v8 v = vfrag(vt, t, d, voff);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if ((__builtin_bit_cast(uint16_t, E(v[i])) & EXP_BITS<E>) == EXP_BITS<E>) v[i] = E(0.f);
+                        v8 pt = pr[0][0];
+#pragma unroll
+                        for (int k = 1; k < BN / 16; ++k) pt = k == t ? pr[k / 2][k % 2] : pt;
+                        o[d] = mfma32(v, pt, o[d]);
+                    }
+#pragma unroll 1
+                for (int k = 0; k < BN; ++k) {
+                    if (k0 + k >= limit) continue;
+                    const int swz = ((k & 3) << 1) | ((k >> 2) & 1);
+#pragma unroll
+                    for (int d = 0; d < DB; ++d)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const int e = 32 * d + 8 * (r / 4) + 4 * half + r % 4;
+                            const E v = *reinterpret_cast<const E *>(vt + k * DP * 2 + (((e / 8) ^ swz) * 16) + (e % 8) * 2);
+                            if ((__builtin_bit_cast(uint16_t, v) & EXP_BITS<E>) == EXP_BITS<E>) o[d][r] += float(v);
+                        }
+                }
+                return;
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < BLK; ++b)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int d = 0; d < DB; ++d) o[d] = mfma32(vfrag(vt, 2 * b + t, d, voff), pr[b][t], o[d]);
+    }
+};
+
+// Attention on the matrix cores, 16-bit types.  A wavefront owns 32 rows.
+//   KEYS == false: the workgroup's 4 wavefronts own different rows and share tiles of 64 slots.
+//   KEYS == true (few rows): they own the same rows and tiles of 32 slots in turn, without a
+//   barrier between them, and join their sums at the end.
+// Wavefronts of a workgroup; with wide heads the private tiles of 2 fill the LDS.
+constexpr int attn_waves(int dp, bool few) { return few && dp > 128 ? 2 : 4; }
+
+template <typename E, int DP, bool KEYS, bool ALIGNED>
+__global__ void __launch_bounds__(64 * attn_waves(DP, KEYS), KEYS || DP > 128 ? 1 : 2)
+attention_mfma_kernel(AttnPlan p, AttnGrid g, const E *__restrict__ q, E *__restrict__ out, float *__restrict__ lse,
+                      const E *__restrict__ keys, const E *__restrict__ values, const int32_t *__restrict__ lens,
+                      const int32_t *__restrict__ starts) {
+    constexpr int BN = KEYS ? 32 : 64, TILE = BN * DP * 2, NW = attn_waves(DP, KEYS);
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    typedef typename Elem16<E>::v8 v8;
+    Work w;
+    if (!find_work(starts, p, g, w)) return;
+    const int lane = lane_id(), wv = wave_id(), half = lane >> 5, col = lane & 31;
+    const int len = stream_len(p, lens, w.b);
+    const int rows = w.count * p.group;
+    const int r0 = w.rb * g.block_rows, row = r0 + (KEYS ? 0 : wv * 32) + col;
+    const int tok = int(g.by_group.quot(uint32_t(min(row, rows - 1))));
+    const int head = w.h * p.group + min(row, rows - 1) - tok * p.group;
+    const bool real = row < rows;
+    const int last_tok = int(g.by_group.quot(uint32_t(min(r0 + g.block_rows, rows) - 1)));
+    const int end_all = visible(len, w.count, last_tok, p.causal_block);  // slots that any row of the workgroup sees
+    const int kb = w.split * g.split_keys, ke = min(end_all, kb + g.split_keys);
+    if (kb >= end_all && w.split > 0) return;  // nothing: the joining launch knows
+    const int limit = real ? min(visible(len, w.count, tok, p.causal_block), ke) : 0;
+    // slots below `all` are seen by every row of this wavefront
+    const int wave_r0 = r0 + (KEYS ? 0 : wv * 32);
+    const int all = wave_r0 < rows ? min(visible(len, w.count, int(g.by_group.quot(uint32_t(wave_r0))), p.causal_block), ke) : 0;
+    const int wave_last = min(wave_r0 + 32, rows) - 1;
+    const int wave_end = wave_r0 < rows ? min(visible(len, w.count, int(g.by_group.quot(uint32_t(wave_last))), p.causal_block), ke) : 0;
+
+    RowState<E, DP, BN> st;
+    st.init();
+    const E *qr = q + int64_t(w.first + tok) * p.qt + head * p.qh;
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t) {
+        union {
+            uint4 u;
+            v8 v;
+        } f;
+        f.u = make_uint4(0, 0, 0, 0);
+        if (real && 16 * t + 8 * half < p.dim) f.u = *reinterpret_cast<const uint4 *>(qr + 16 * t + 8 * half);
+        f.u.x ^= p.flip, f.u.y ^= p.flip, f.u.z ^= p.flip, f.u.w ^= p.flip;
+        st.q[t] = f.v;
+    }
+    int koff[DP / 16], voff[DP / 32];
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t) koff[t] = col * DP * 2 + (((2 * t + half) ^ (col & 7)) << 4);
+    {
+        const int l16 = lane & 15, f = ((l16 >> 2) << 1) | half;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+            voff[d] = (4 * half + (l16 >> 2)) * DP * 2 + (((4 * d + 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1)) ^ f) << 4) + (l16 & 1) * 8;
+    }
+    const int32_t *table = p.pool.table + int64_t(w.b) * p.pool.max_pages;
+    TileLoader<E, DP, BN, KEYS ? 1 : NW, ALIGNED> load;
+    const int loader = KEYS ? 0 : wv;
+    load.init(loader, p.dim);
+    char *base = KEYS ? lds + wv * 4 * TILE : lds;  // [stage][K, V]
+    const int first = kb + (KEYS ? wv * BN : 0), stride = KEYS ? NW * BN : BN;
+    if (first < ke) load.request(p, table, keys, values, w.h, first, ke, base, base + TILE, loader);
+    int stage = 0;
+    for (int k0 = first; k0 < ke; k0 += stride, stage ^= 1) {
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this tile has arrived
+        if constexpr (KEYS) __builtin_amdgcn_wave_barrier();
+        else __syncthreads();                // .. everybody's part of it, and the other stage is free
+        char *kt = base + stage * 2 * TILE, *vt = kt + TILE;
+        char *nk = base + (stage ^ 1) * 2 * TILE;
+        if (k0 + stride < ke) load.request(p, table, keys, values, w.h, k0 + stride, ke, nk, nk + TILE, loader);
+        if (k0 + BN <= all) st.template step<false>(kt, vt, koff, voff, p.scale, k0, limit);
+        else if (k0 < wave_end) st.template step<true>(kt, vt, koff, voff, p.scale, k0, limit);
+    }
+
+    float l = sum_halves(st.l);
+    const bool bad = __syncthreads_or(load.bad) != 0;
+    const int64_t grow = int64_t(w.first + tok) * p.q_heads + head;  // this row among all
+    const int64_t all_rows = int64_t(p.tokens) * p.q_heads;
+    if constexpr (KEYS) {
+        // the four wavefronts' sums meet in LDS: [wavefront][row][DP + 4] and their (m, l)
+        constexpr int PITCH = DP + 4;
+        float *ml = reinterpret_cast<float *>(lds), *os = ml + NW * 32 * 2;
+        if (half == 0) ml[(wv * 32 + col) * 2] = st.m, ml[(wv * 32 + col) * 2 + 1] = l;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                *reinterpret_cast<float4_t *>(os + (wv * 32 + col) * PITCH + 32 * d + 8 * j + 4 * half) =
+                    float4_t{st.o[d][4 * j], st.o[d][4 * j + 1], st.o[d][4 * j + 2], st.o[d][4 * j + 3]};
+        __syncthreads();
+        const int here = min(32, rows - r0);
+        const int vecs = p.dim / 4;
+        for (int i = threadIdx.x; i < here * vecs; i += NW * WAVE) {
+            const int rr = i / vecs, c = (i - rr * vecs) * 4;
+            float mm = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < NW; ++k) mm = fmaxf(mm, ml[(k * 32 + rr) * 2]);
+            const float ref = mm == -INFINITY ? 0.f : mm;
+            float ll = 0.f;
+            float4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < NW; ++k) {
+                const float f = __builtin_amdgcn_exp2f(ml[(k * 32 + rr) * 2] - ref);
+                ll = fmaf(f, ml[(k * 32 + rr) * 2 + 1], ll);
+                const float4_t v = *reinterpret_cast<const float4_t *>(os + (k * 32 + rr) * PITCH + c);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[j] = fmaf(f, v[j], o[j]);
+            }
+            const int tk = int(g.by_group.quot(uint32_t(r0 + rr))), hd = w.h * p.group + r0 + rr - tk * p.group;
+            const int64_t gr = int64_t(w.first + tk) * p.q_heads + hd;
+            if (bad) ll = NAN;
+            if (g.splits > 1) {
+                *reinterpret_cast<float4_t *>(g.part + (w.split * all_rows + gr) * p.dim + c) = o;
+                if (c == 0) {
+                    float *x = g.part + g.splits * all_rows * p.dim + (w.split * all_rows + gr) * 2;
+                    x[0] = mm, x[1] = ll;
+                }
+            } else {
+                const float inv = ll == 0.f ? 0.f : 1.f / ll;
+                Vec<E, 4> v;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v.v[j] = E(o[j] * inv);
+                E *dst = out + int64_t(w.first + tk) * p.ot + hd * p.oh + c;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) dst[j] = v.v[j];
+                if (c == 0 && lse != nullptr) lse[gr] = ll == 0.f ? -INFINITY : (ref + __builtin_amdgcn_logf(ll)) * 0.693147180559945309f;
+            }
+        }
+    } else {
+        if (!real) return;
+        if (bad) l = NAN;
+        if (g.splits > 1) {
+            float *dst = g.part + (w.split * all_rows + grow) * p.dim;
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (32 * d + 8 * j + 4 * half < p.dim)
+                        *reinterpret_cast<float4_t *>(dst + 32 * d + 8 * j + 4 * half) =
+                            float4_t{st.o[d][4 * j], st.o[d][4 * j + 1], st.o[d][4 * j + 2], st.o[d][4 * j + 3]};
+            if (half == 0) {
+                float *x = g.part + g.splits * all_rows * p.dim + (w.split * all_rows + grow) * 2;
+                x[0] = st.m, x[1] = l;
+            }
+            return;
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        E *dst = out + int64_t(w.first + tok) * p.ot + head * p.oh;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (32 * d + 8 * j + 4 * half >= p.dim) continue;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) dst[32 * d + 8 * j + 4 * half + i] = E(st.o[d][4 * j + i] * inv);
+            }
+        if (half == 0 && lse != nullptr)
+            lse[grow] = l == 0.f ? -INFINITY : ((st.m == -INFINITY ? 0.f : st.m) + __builtin_amdgcn_logf(l)) * 0.693147180559945309f;
+    }
+}
+
+// Joins the pieces of the slot axis: one wavefront per row.
 template <typename T>
-hipError_t attention_t(const dc_attention_args &a, AttnPlan p, hipStream_t s) {
+__global__ void __launch_bounds__(256)
+attention_join_kernel(AttnPlan p, AttnGrid g, T *__restrict__ out, float *__restrict__ lse, const int32_t *__restrict__ lens,
+                      const int32_t *__restrict__ starts) {
+    const int64_t all_rows = int64_t(p.tokens) * p.q_heads, row = int64_t(blockIdx.x) * 4 + wave_id();
+    if (row >= all_rows) return;
+    const int t = int(row / p.q_heads), head = int(row - int64_t(t) * p.q_heads), lane = lane_id();
+    const int b = stream_of(starts, p.streams, p.tokens, t);
+    if (b < 0) return;
+    int first, count;
+    stream_tokens(starts, b, p.streams, p.tokens, first, count);
+    const int n = visible(stream_len(p, lens, b), count, t - first, p.causal_block);
+    const int pieces = min(g.splits, max(1, (n + g.split_keys - 1) / g.split_keys));
+    const float *ml = g.part + g.splits * all_rows * p.dim;
+    float top = -INFINITY;
+    for (int s = 0; s < pieces; ++s) top = fmaxf(top, ml[(s * all_rows + row) * 2]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < pieces; ++s) {
+        const float f = __builtin_amdgcn_exp2f(ml[(s * all_rows + row) * 2] - ref);
+        l = fmaf(f, ml[(s * all_rows + row) * 2 + 1], l);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            if (c * WAVE + lane < p.dim) o[c] = fmaf(f, g.part[(s * all_rows + row) * p.dim + c * WAVE + lane], o[c]);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+        if (c * WAVE + lane < p.dim) out[t * p.ot + head * p.oh + c * WAVE + lane] = T(o[c] * inv);
+    if (lane == 0 && lse != nullptr) lse[row] = l == 0.f ? -INFINITY : (ref + __builtin_amdgcn_logf(l)) * 0.693147180559945309f;
+}
+
+// How the rows and the slots are divided.
+AttnGrid plan_grid(const AttnPlan &p, bool ragged, bool few, int bm) {
+    AttnGrid g = {};
+    g.block_rows = bm;
+    const int64_t rows = int64_t(p.tokens) * p.group;
+    g.stream_blocks = int(ceil_div64(rows / p.streams, bm));
+    g.flat = ragged ? int(rows / bm) + p.streams : g.stream_blocks * p.streams;
+    const int64_t cap = int64_t(p.pool.max_pages) * p.pool.page_size;
+    const int64_t base = int64_t(g.flat) * p.kv_heads;
+    // pieces of the slot axis until about two workgroups a compute unit are there, none below 8 tiles
+    const int64_t want = few ? 512 : 768, least = few ? 256 : 512;
+    int64_t splits = base >= want ? 1 : ceil_div64(want, base);
+    int64_t keys = max(least, ceil_div64(ceil_div64(cap, splits), 128) * 128);
+    splits = ceil_div64(cap, keys);
+    g.splits = int(splits);
+    g.split_keys = int(keys);
+    const int64_t total = base * splits;
+    g.unit = 1;
+    while (g.unit < 16 && g.unit * 2 <= g.flat && total >= 8 * 2 * g.unit * 2) g.unit *= 2;
+    g.by_group = FastDiv(uint32_t(p.group));
+    g.by_unit = FastDiv(uint32_t(g.unit));
+    g.by_flat = FastDiv(uint32_t(g.flat));
+    g.by_blocks = FastDiv(uint32_t(max(1, g.stream_blocks)));
+    g.by_kv = FastDiv(uint32_t(p.kv_heads));
+    return g;
+}
+
+bool few_rows(const AttnPlan &p) { return int64_t(p.tokens) * p.group <= int64_t(32) * p.streams; }
+
+int64_t part_bytes(const AttnPlan &p, const AttnGrid &g) {
+    return g.splits > 1 ? int64_t(g.splits) * p.tokens * p.q_heads * (p.dim + 2) * 4 : 0;
+}
+
+template <typename E, int DP, bool KEYS, bool ALIGNED>
+hipError_t attention_go(const dc_attention_args &a, const AttnPlan &p, const AttnGrid &g, float *lse, hipStream_t s) {
+    constexpr int BN = KEYS ? 32 : 64, NW = attn_waves(DP, KEYS);
+    const size_t tiles = size_t(KEYS ? NW : 1) * 4 * BN * DP * 2;
+    const size_t join = KEYS ? size_t(NW) * 32 * (2 + DP + 4) * 4 : 0;
+    const size_t lds = max(tiles, join);
+    auto kernel = attention_mfma_kernel<E, DP, KEYS, ALIGNED>;
+    static thread_local uint64_t raised = 0;  // devices whose limit this instantiation has raised
+    int dev = 0;
+    hipError_t err = hipGetDevice(&dev);
+    if (err != hipSuccess) return err;
+    if (dev >= 64 || !(raised >> dev & 1)) {
+        err = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, int(lds));
+        if (err != hipSuccess) return err;
+        if (dev < 64) raised |= 1ull << dev;
+    }
+    const int64_t total = int64_t(g.flat) * p.kv_heads * g.splits;
+    const int64_t blocks = ceil_div64(total, 8 * g.unit) * 8 * g.unit;
+    if (blocks > (1 << 30)) return hipErrorInvalidConfiguration;
+    note_kernel("attention_mfma_kernel");
+    kernel<<<dim3(uint32_t(blocks)), NW * WAVE, lds, s>>>(p, g, (const E *)a.q, (E *)a.out, lse, (const E *)a.keys, (const E *)a.values, a.lens, a.starts);
+    return hipGetLastError();
+}
+
+template <typename E, int DP>
+hipError_t attention_dp(const dc_attention_args &a, const AttnPlan &p, const AttnGrid &g, bool few, float *lse, hipStream_t s) {
+    const bool aligned = p.pool.page_size % (few ? 32 : 64) == 0;
+    if (few) return aligned ? attention_go<E, DP, true, true>(a, p, g, lse, s) : attention_go<E, DP, true, false>(a, p, g, lse, s);
+    return aligned ? attention_go<E, DP, false, true>(a, p, g, lse, s) : attention_go<E, DP, false, false>(a, p, g, lse, s);
+}
+
+template <typename T>
+hipError_t weights_go(const dc_attention_args &a, const AttnPlan &p, const float *lse, hipStream_t s) {
+    note_kernel("attention_weights_kernel");
+    const int most = int(ceil_div64(int64_t(a.max_pages) * a.page_size, WAVE));
+    attention_weights_kernel<T><<<dim3(most, p.kv_heads, p.streams), 64, 0, s>>>(p, (const T *)a.q, lse, (const T *)a.keys,
+                                                                                a.weights, a.lens, a.starts);
+    return hipGetLastError();
+}
+
+AttnPlan make_plan(const dc_attention_args &a) {
+    AttnPlan p = {};
+    p.pool = {a.page_table, a.num_pages, a.page_size, a.max_pages, FastDiv(uint32_t(a.page_size))};
+    p.tokens = a.tokens, p.q_heads = a.q_heads, p.kv_heads = a.kv_heads, p.dim = a.dim, p.group = a.q_heads / a.kv_heads;
+    p.streams = a.streams, p.causal_block = a.causal_block, p.decay = a.decay;
+    p.scale = a.scale;
+    p.qt = a.q_token_stride, p.qh = a.q_head_stride, p.ot = a.out_token_stride, p.oh = a.out_head_stride;
+    return p;
+}
+
+// Layout of the workspace: partial sums, then the log-sums.
+struct Room {
+    int64_t part, lse;
+};
+Room room(const dc_attention_args &a, int dtype) {
+    const AttnPlan p = make_plan(a);
+    Room r = {0, 0};
+    if (dtype != DC_F32) {
+        const bool few = few_rows(p);
+        r.part = part_bytes(p, plan_grid(p, a.starts != nullptr, few, few ? 32 : 128));
+    }
+    if (a.weights != nullptr && a.lse == nullptr) r.lse = int64_t(a.tokens) * a.q_heads * 4;
+    return r;
+}
+
+template <typename E>
+hipError_t attention_16(const dc_attention_args &a, AttnPlan p, hipStream_t s) {
+    const Room r = room(a, DC_F16);
+    float *lse = a.lse != nullptr || a.weights == nullptr ? a.lse : (float *)((char *)a.workspace + r.part);
+    const bool few = few_rows(p);
+    AttnGrid g = plan_grid(p, a.starts != nullptr, few, few ? 32 : 128);
+    g.part = (float *)a.workspace;
+    AttnPlan m = p;
+    // exponentials are powers of two; a negative scale turns q's signs instead, so that the largest score has the largest product
+    m.flip = p.scale < 0.f ? 0x80008000u : 0u;
+    m.scale = fabsf(p.scale) * 1.44269504088896341f;
+    hipError_t e = p.dim <= 64 ? attention_dp<E, 64>(a, m, g, few, lse, s) : p.dim <= 128 ? attention_dp<E, 128>(a, m, g, few, lse, s)
+                                                                                 : attention_dp<E, 256>(a, m, g, few, lse, s);
+    if (e == hipSuccess && g.splits > 1) {
+        note_kernel("attention_join_kernel");
+        attention_join_kernel<E><<<ceil_div(p.tokens * p.q_heads, 4), 256, 0, s>>>(m, g, (E *)a.out, lse, a.lens, a.starts);
+        e = hipGetLastError();
+    }
+    return e == hipSuccess && a.weights != nullptr ? weights_go<E>(a, p, lse, s) : e;
+}
+
+hipError_t attention_32(const dc_attention_args &a, const AttnPlan &p, hipStream_t s) {
     float *lse = a.lse != nullptr || a.weights == nullptr ? a.lse : (float *)a.workspace;
     note_kernel("paged_attention_kernel");
-    paged_attention_kernel<T><<<dim3(p.tokens, p.q_heads), 64, 0, s>>>(p, (const T *)a.q, (T *)a.out, lse, (const T *)a.keys,
-                                                                      (const T *)a.values, a.lens, a.starts);
-    if (a.weights != nullptr) {
-        note_kernel("attention_weights_kernel");
-        const int most = int(ceil_div64(int64_t(a.max_pages) * a.page_size, WAVE));
-        attention_weights_kernel<T><<<dim3(most, p.kv_heads, p.streams), 64, 0, s>>>(p, (const T *)a.q, lse, (const T *)a.keys,
-                                                                                    a.weights, a.lens, a.starts);
-    }
-    return hipGetLastError();
+    paged_attention_kernel<float><<<dim3(p.tokens, p.q_heads), 64, 0, s>>>(p, (const float *)a.q, (float *)a.out, lse, (const float *)a.keys,
+                                                                          (const float *)a.values, a.lens, a.starts);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess && a.weights != nullptr ? weights_go<float>(a, p, lse, s) : e;
 }
 
 }  // namespace
 
-int64_t paged_attention_workspace(const dc_attention_args &a, int) {
-    return a.weights != nullptr && a.lse == nullptr ? int64_t(a.tokens) * a.q_heads * 4 : 0;
+int64_t paged_attention_workspace(const dc_attention_args &a, int dtype) {
+    const Room r = room(a, dtype);
+    return r.part + r.lse;
 }
 
 hipError_t launch_paged_attention(const dc_attention_args &a, int dtype, hipStream_t s) {
-    AttnPlan p = {};
-    p.pool = {a.page_table, a.num_pages, a.page_size, a.max_pages, FastDiv(uint32_t(a.page_size))};
-    p.tokens = a.tokens, p.q_heads = a.q_heads, p.kv_heads = a.kv_heads, p.dim = a.dim, p.group = a.q_heads / a.kv_heads;
-    p.streams = a.streams, p.causal_block = a.causal_block, p.scale = a.scale, p.decay = a.decay;
-    p.qt = a.q_token_stride, p.qh = a.q_head_stride, p.ot = a.out_token_stride, p.oh = a.out_head_stride;
-    if (dtype == DC_F32) return attention_t<float>(a, p, s);
-    if (dtype == DC_BF16) return attention_t<bf16_t>(a, p, s);
-    return attention_t<half_t>(a, p, s);
+    const AttnPlan p = make_plan(a);
+    if (dtype == DC_F32) return attention_32(a, p, s);
+    if (dtype == DC_BF16) return attention_16<bf16_t>(a, p, s);
+    return attention_16<half_t>(a, p, s);
 }
 
 }  // namespace dc
