@@ -13,7 +13,7 @@ struct AttnPlan {
     PagePool pool;
     int32_t tokens, q_heads, kv_heads, dim, group, streams, causal_block;
     float scale, decay;
-    uint32_t flip;  // sign bits of a pair of 16-bit elements, or 0
+    uint32_t flip;  // sign bits of the elements in 32 bits, or 0
     int64_t qt, qh, ot, oh;
 };
 
@@ -26,93 +26,6 @@ __device__ __forceinline__ int visible(int len, int count, int i, int block) {
 
 __device__ __forceinline__ int stream_len(const AttnPlan &p, const int32_t *lens, int b) {
     return int(min(int64_t(max(lens[b], 0)), int64_t(p.pool.max_pages) * p.pool.page_size));
-}
-
-// One wavefront per token and query head; a lane scores one slot and sums four elements of the output.
-template <typename T>
-__global__ void __launch_bounds__(64)
-paged_attention_kernel(AttnPlan p, const T *__restrict__ q, T *__restrict__ out, float *__restrict__ lse,
-                       const T *__restrict__ keys, const T *__restrict__ values, const int32_t *__restrict__ lens,
-                       const int32_t *__restrict__ starts) {
-    __shared__ float prob[WAVE];
-    __shared__ int64_t row_of[WAVE];
-    const int t = blockIdx.x, head = blockIdx.y, h = head / p.group, lane = lane_id();
-    const int b = stream_of(starts, p.streams, p.tokens, t);
-    if (b < 0) return;
-    int first, count;
-    stream_tokens(starts, b, p.streams, p.tokens, first, count);
-    const int n = visible(stream_len(p, lens, b), count, t - first, p.causal_block);
-    const int32_t *table = p.pool.table + int64_t(b) * p.pool.max_pages;
-    const T *qr = q + t * p.qt + head * p.qh;
-    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    bool bad = false;
-    for (int s0 = 0; s0 < n; s0 += WAVE) {
-        const int s = s0 + lane;
-        int64_t row = -1;
-        float score = -INFINITY;
-        if (s < n) {
-            row = slot_row(p.pool, table, s, p.kv_heads, h);
-            bad = bad || row < 0;
-            if (row >= 0) {
-                float sum = 0.f;
-                for (int d = 0; d < p.dim; ++d) sum = fmaf(float(qr[d]), float(keys[row * p.dim + d]), sum);
-                score = sum * p.scale;
-            }
-        }
-        float top = score;
-#pragma unroll
-        for (int d = 32; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, WAVE));
-        const float m2 = fmaxf(m, top), ref = m2 == -INFINITY ? 0.f : m2;
-        const float pr = row < 0 ? 0.f : expf(score - ref), fade = expf(m - ref);
-        m = m2;
-        l = l * fade + pr;
-        prob[lane] = pr;
-        row_of[lane] = row;
-        __syncthreads();
-#pragma unroll
-        for (int c = 0; c < 4; ++c) o[c] *= fade;
-        for (int j = 0; j < min(WAVE, n - s0); ++j) {
-            if (row_of[j] < 0) continue;
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                if (c * WAVE + lane < p.dim) o[c] = fmaf(prob[j], float(values[row_of[j] * p.dim + c * WAVE + lane]), o[c]);
-        }
-        __syncthreads();
-    }
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) l += __shfl_xor(l, d, WAVE);
-    bad = ballot(bad) != 0;
-    const float inv = bad ? NAN : l > 0.f || l != l ? 1.f / l : 0.f;
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-        if (c * WAVE + lane < p.dim) out[t * p.ot + head * p.oh + c * WAVE + lane] = T(o[c] * inv);
-    if (lane == 0 && lse != nullptr) lse[int64_t(t) * p.q_heads + head] = bad ? NAN : l == 0.f ? -INFINITY : m + logf(l);
-}
-
-// One thread per slot and kv head: the sum of its probabilities over the rows that share the head.
-template <typename T>
-__global__ void __launch_bounds__(64)
-attention_weights_kernel(AttnPlan p, const T *__restrict__ q, const float *__restrict__ lse, const T *__restrict__ keys,
-                         float *__restrict__ weights, const int32_t *__restrict__ lens, const int32_t *__restrict__ starts) {
-    const int b = blockIdx.z, h = blockIdx.y, len = stream_len(p, lens, b);
-    const int s = blockIdx.x * WAVE + threadIdx.x;
-    if (s >= len) return;
-    int first, count;
-    stream_tokens(starts, b, p.streams, p.tokens, first, count);
-    const int64_t row = slot_row(p.pool, p.pool.table + int64_t(b) * p.pool.max_pages, s, p.kv_heads, h);
-    if (row < 0) return;
-    float received = 0.f;
-    for (int i = 0; i < count; ++i) {
-        if (s >= visible(len, count, i, p.causal_block)) continue;
-        for (int g = 0; g < p.group; ++g) {
-            const T *qr = q + (first + i) * p.qt + (h * p.group + g) * p.qh;
-            float sum = 0.f;
-            for (int d = 0; d < p.dim; ++d) sum = fmaf(float(qr[d]), float(keys[row * p.dim + d]), sum);
-            const float z = lse[int64_t(first + i) * p.q_heads + h * p.group + g];
-            if (z != -INFINITY) received += expf(sum * p.scale - z);
-        }
-    }
-    weights[row] = p.decay == 0.f ? received : fmaf(p.decay, weights[row], received);
 }
 
 typedef float float16_t __attribute__((ext_vector_type(16)));
@@ -131,10 +44,30 @@ __device__ __forceinline__ float16_t mfma32(bf16x8_t a, bf16x8_t b, float16_t c)
 __device__ __forceinline__ uint32_t pack2(float a, float b, half_t) { return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2v_t{a, b}), half2v_t)); }
 __device__ __forceinline__ uint32_t pack2(float a, float b, bf16_t) { return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2v_t{a, b}), bf16x2_t)); }
 
+// A 16-byte operand chunk of each type and what it does in a product: one instruction over 2 x 8 elements
+// for the 16-bit types, four over 2 x 1 in fp32 (element i of both halves' chunks: the order of a
+// sum's terms is free as long as both operands keep it).
 template <typename E>
-constexpr uint32_t EXP_BITS = 0x7c00u;
+struct Chunk {
+    static constexpr int N = 8;
+    typedef typename Elem16<E>::v8 v;
+    static __device__ __forceinline__ float16_t mma(v a, v b, float16_t c) { return mfma32(a, b, c); }
+};
 template <>
-constexpr uint32_t EXP_BITS<bf16_t> = 0x7f80u;
+struct Chunk<float> {
+    static constexpr int N = 4;
+    typedef float4_t v;
+    static __device__ __forceinline__ float16_t mma(v a, v b, float16_t c) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
+        return c;
+    }
+};
+
+// Infinity or NaN?
+__device__ __forceinline__ bool odd_value(half_t x) { return (__builtin_bit_cast(uint16_t, x) & 0x7c00u) == 0x7c00u; }
+__device__ __forceinline__ bool odd_value(bf16_t x) { return (__builtin_bit_cast(uint16_t, x) & 0x7f80u) == 0x7f80u; }
+__device__ __forceinline__ bool odd_value(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
 
 // The larger of the two halves' values, in both.
 __device__ __forceinline__ float max_halves(float x) {
@@ -202,8 +135,6 @@ __device__ __forceinline__ bool find_block(const int32_t *starts, const AttnPlan
             base += __shfl(sum, WAVE - 1, WAVE);
         }
         if (!hit) return false;
-        w.b = __builtin_amdgcn_readfirstlane(w.b), w.rb = __builtin_amdgcn_readfirstlane(w.rb);
-        w.first = __builtin_amdgcn_readfirstlane(w.first), w.count = __builtin_amdgcn_readfirstlane(w.count);
     }
     return true;
 }
@@ -223,6 +154,9 @@ __device__ __forceinline__ bool find_work(const int32_t *starts, const AttnPlan 
         const int blocks = int((int64_t(w.count) * p.group + g.block_rows - 1) / g.block_rows);
         w.rb = blocks - 1 - w.rb;
     }
+    w.b = __builtin_amdgcn_readfirstlane(w.b), w.rb = __builtin_amdgcn_readfirstlane(w.rb), w.h = __builtin_amdgcn_readfirstlane(w.h);
+    w.split = __builtin_amdgcn_readfirstlane(w.split);
+    w.first = __builtin_amdgcn_readfirstlane(w.first), w.count = __builtin_amdgcn_readfirstlane(w.count);
     return true;
 }
 
@@ -232,13 +166,13 @@ __device__ __forceinline__ bool find_work(const int32_t *starts, const AttnPlan 
 // `end` or in no page of the pool, and the elements from dim to DP, arrive as zeros.
 template <typename E, int DP, int BN, int LOADERS, bool ALIGNED>
 struct TileLoader {
-    static constexpr int CPR = DP / 8, RPI = WAVE / CPR, REQ = BN / RPI / LOADERS;
+    static constexpr int N = Chunk<E>::N, CPR = DP / N, RPI = WAVE / CPR, REQ = BN / RPI / LOADERS;
     static_assert(REQ >= 1, "one request a wavefront at least");
-    int row0, kchunk[2], vchunk, dim;
+    int row0, dim;
     bool bad = false;
 
     static __device__ __forceinline__ int kswz(int row) { return row & 7; }
-    static __device__ __forceinline__ int vswz(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
+    static __device__ __forceinline__ int vswz(int row) { return sizeof(E) == 2 ? ((row & 3) << 1) | ((row >> 2) & 1) : 0; }
 
     __device__ __forceinline__ void init(int loader, int dim_) {
         dim = dim_;
@@ -252,21 +186,23 @@ struct TileLoader {
             const int page = __builtin_amdgcn_readfirstlane(table[i]);
             const bool ok = uint32_t(page) < uint32_t(p.pool.num_pages);
             bad = bad || !ok;
-            const int64_t base = ok ? ((int64_t(page) * p.kv_heads + h) * p.pool.page_size + (k0 - i * p.pool.page_size)) * dim : 0;
-            const int bytes = ok ? min(BN, end - k0) * dim * 2 : 0;
-            const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<E *>(keys) + base, 0, bytes, 0x00027000);
-            const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<E *>(values) + base, 0, bytes, 0x00027000);
+            const uint64_t base = ok ? uint64_t(((int64_t(page) * p.kv_heads + h) * p.pool.page_size + (k0 - i * p.pool.page_size)) * dim) : 0;
+            const uint64_t at = uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(uint32_t(base)))) |
+                                uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(uint32_t(base >> 32)))) << 32;
+            const int bytes = __builtin_amdgcn_readfirstlane(ok ? min(BN, end - k0) * dim * int(sizeof(E)) : 0);
+            const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<E *>(keys) + at, 0, bytes, 0x00027000);
+            const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<E *>(values) + at, 0, bytes, 0x00027000);
 #pragma unroll
             for (int j = 0; j < REQ; ++j) {
                 const int row = row0 + j * RPI, ck = c ^ kswz(row);
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (DC_LDS(void) *)(kt + (loader * REQ + j) * 1024), 16,
-                                                         ck * 8 < dim ? (row * dim + ck * 8) * 2 : 0x40000000, 0, 0, 0);
+                                                         ck * N < dim ? (row * dim + ck * N) * int(sizeof(E)) : 0x40000000, 0, 0, 0);
             }
 #pragma unroll
             for (int j = 0; j < REQ; ++j) {
                 const int row = row0 + j * RPI, cv = c ^ vswz(row);
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (DC_LDS(void) *)(vt + (loader * REQ + j) * 1024), 16,
-                                                         cv * 8 < dim ? (row * dim + cv * 8) * 2 : 0x40000000, 0, 0, 0);
+                                                         cv * N < dim ? (row * dim + cv * N) * int(sizeof(E)) : 0x40000000, 0, 0, 0);
             }
         } else {
             const E *zero = reinterpret_cast<const E *>(&zero_chunk);
@@ -280,8 +216,8 @@ struct TileLoader {
                     bad = bad || at < 0;
                 }
                 const int ck = c ^ kswz(row), cv = c ^ vswz(row);
-                kp[j] = at >= 0 && ck * 8 < dim ? keys + at * dim + ck * 8 : zero;
-                vp[j] = at >= 0 && cv * 8 < dim ? values + at * dim + cv * 8 : zero;
+                kp[j] = at >= 0 && ck * N < dim ? keys + at * dim + ck * N : zero;
+                vp[j] = at >= 0 && cv * N < dim ? values + at * dim + cv * N : zero;
             }
 #pragma unroll
             for (int j = 0; j < REQ; ++j)
@@ -301,11 +237,13 @@ struct TileLoader {
 // transposing read.
 template <typename E, int DP, int BN>
 struct RowState {
-    typedef typename Elem16<E>::v8 v8;
-    static constexpr int BLK = BN / 32, STEPS = DP / 16, DB = DP / 32;
+    typedef typename Chunk<E>::v chunk;
+    static constexpr int ROW = DP * int(sizeof(E)), BLK = BN / 32, STEPS = DP / (2 * Chunk<E>::N), DB = DP / 32;
+    static constexpr int VOFF = sizeof(E) == 2 ? DB : 1;
     float16_t o[DB];
     float m, l;
-    v8 q[STEPS];
+    chunk q[STEPS];
+    int koff[STEPS], voff[VOFF];  // this lane's places in a tile of keys / values
 
     __device__ __forceinline__ void init() {
         m = -INFINITY, l = 0.f;
@@ -313,23 +251,80 @@ struct RowState {
         for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+        const int lane = lane_id(), half = lane >> 5, col = lane & 31;
+#pragma unroll
+        for (int t = 0; t < STEPS; ++t) koff[t] = col * ROW + (((2 * t + half) ^ (col & 7)) << 4);
+        if constexpr (sizeof(E) == 2) {
+            const int l16 = lane & 15, f = ((l16 >> 2) << 1) | half;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+                voff[d] = (4 * half + (l16 >> 2)) * ROW + (((4 * d + 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1)) ^ f) << 4) + (l16 & 1) * 8;
+        } else {
+            voff[0] = 4 * half * ROW + col * 4;
+        }
     }
 
-    // V^T fragment of 32 elements x 16 slots: slots 16 t + 8 e + 4 half + i of the tile in element 4 e + i
-    static __device__ __forceinline__ v8 vfrag(const char *vt, int t, int d, const int *voff) {
+    // 16-bit: V^T fragment of 32 elements x 16 slots: slot 16 t + 8 e + 4 half + i of the tile in element 4 e + i
+    __device__ __forceinline__ chunk vfrag(const char *vt, int t, int d) const {
         union {
             short4_t h[2];
-            v8 v;
+            chunk v;
         } f;
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-            f.h[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DC_LDS(short4_t) *)(vt + voff[d] + (16 * t + 8 * e) * DP * 2));
+            f.h[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DC_LDS(short4_t) *)(vt + voff[d] + (16 * t + 8 * e) * ROW));
         return f.v;
     }
+    // fp32: element 32 d + col of slot 32 b + 8 (r / 4) + 4 half + r % 4
+    __device__ __forceinline__ float vword(const char *vt, int b, int r, int d) const {
+        return *reinterpret_cast<const float *>(vt + voff[0] + (32 * b + 8 * (r / 4) + r % 4) * ROW + 128 * d);
+    }
 
-    // One tile: slots [k0, k0 + BN); this lane's row sees slots below `limit` (MASK: some of the tile's are not seen by some row)
+    // Slots that some rows see and others do not may hold infinities or NaN, and 0 * inf would carry them
+    // over: such elements leave the product and join the rows that see them one by one.
+    __device__ __forceinline__ bool any_odd(const char *vt) const {
+        bool odd = false;
+        if constexpr (sizeof(E) == 2) {
+#pragma unroll
+            for (int t = 0; t < BN / 16; ++t)
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    const chunk v = vfrag(vt, t, d);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) odd = odd || odd_value(E(v[i]));
+                }
+        } else {
+#pragma unroll
+            for (int b = 0; b < BLK; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) odd = odd || odd_value(vword(vt, b, r, d));
+        }
+        return ballot(odd) != 0;
+    }
+    __device__ __forceinline__ void add_odd(const char *vt, int k0, int limit) {
+        const int half = lane_id() >> 5;
+#pragma unroll 1
+        for (int k = 0; k < BN; ++k) {
+            if (k0 + k >= limit) continue;
+            const int swz = TileLoader<E, DP, BN, 1, true>::vswz(k);
+            const char *row = vt + k * ROW;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    constexpr int N = Chunk<E>::N;
+                    const int e = 32 * d + 8 * (r / 4) + 4 * half + r % 4;
+                    const E v = *reinterpret_cast<const E *>(row + (((e / N) ^ swz) * 16) + (e % N) * int(sizeof(E)));
+                    if (odd_value(v)) o[d][r] += float(v);
+                }
+        }
+    }
+
+    // One tile: slots [k0, k0 + BN); this lane's row sees slots below `limit` (MASK: some row does not see some of the tile's)
     template <bool MASK>
-    __device__ __forceinline__ void step(const char *kt, const char *vt, const int *koff, const int *voff, float scale, int k0, int limit) {
+    __device__ __forceinline__ void step(const char *kt, const char *vt, float scale, int k0, int limit) {
         float16_t s[BLK];
 #pragma unroll
         for (int b = 0; b < BLK; ++b) {
@@ -337,7 +332,7 @@ struct RowState {
             for (int r = 0; r < 16; ++r) s[b][r] = 0.f;
 #pragma unroll
             for (int t = 0; t < STEPS; ++t)
-                s[b] = mfma32(*reinterpret_cast<const v8 *>(kt + koff[t] + b * 32 * DP * 2), q[t], s[b]);
+                s[b] = Chunk<E>::mma(*reinterpret_cast<const chunk *>(kt + koff[t] + b * 32 * ROW), q[t], s[b]);
         }
         const int half = lane_id() >> 5;
         if constexpr (MASK) {
@@ -365,93 +360,100 @@ struct RowState {
                 for (int r = 0; r < 16; ++r) o[d][r] *= fade;
         }
         const float ref = m == -INFINITY ? 0.f : m;
-        // probabilities: the sum in fp32, the product's operand rounded to the 16-bit type (half a step of
-        // it relative to each, the same as the values they multiply carry)
-        v8 pr[BLK][2];
 #pragma unroll
         for (int b = 0; b < BLK; ++b)
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                union {
-                    uint32_t u[4];
-                    v8 v;
-                } f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float a = __builtin_amdgcn_exp2f(fmaf(s[b][8 * t + 2 * i], scale, -ref));
-                    const float c = __builtin_amdgcn_exp2f(fmaf(s[b][8 * t + 2 * i + 1], scale, -ref));
-                    l += a;
-                    l += c;
-                    f.u[i] = pack2(a, c, E());
-                }
-                pr[b][t] = f.v;
+            for (int r = 0; r < 16; ++r) {
+                s[b][r] = __builtin_amdgcn_exp2f(fmaf(s[b][r], scale, -ref));
+                l += s[b][r];
             }
-        if constexpr (MASK) {
-            // Slots that some rows see and others do not may hold infinities or NaN, and 0 * inf would carry
-            // them over: such elements leave the product and join the rows that see them one by one.
-            bool odd = false;
+        bool odd = false;
+        if constexpr (MASK) odd = any_odd(vt);
+        if constexpr (sizeof(E) == 2) {
+            // the sum above is of the probabilities in fp32; the product's operand is rounded to the 16-bit type
+            // (half a step of it relative to each, as much as the values that it multiplies carry)
+            chunk pr[BLK][2];
 #pragma unroll
-            for (int t = 0; t < BN / 16; ++t)
+            for (int b = 0; b < BLK; ++b)
 #pragma unroll
-                for (int d = 0; d < DB; ++d) {
-                    const v8 v = vfrag(vt, t, d, voff);
+                for (int t = 0; t < 2; ++t) {
+                    union {
+                        uint32_t u[4];
+                        chunk v;
+                    } f;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) odd = odd || (__builtin_bit_cast(uint16_t, E(v[i])) & EXP_BITS<E>) == EXP_BITS<E>;
+                    for (int i = 0; i < 4; ++i) f.u[i] = pack2(s[b][8 * t + 2 * i], s[b][8 * t + 2 * i + 1], E());
+                    pr[b][t] = f.v;
                 }
-            if (ballot(odd) != 0) {
-#pragma unroll 1
-                for (int t = 0; t < BN / 16; ++t)
+            if (MASK && odd) {
 #pragma unroll
-                    for (int d = 0; d < DB; ++d) {
-                        v8 v = vfrag(vt, t, d, voff);
+                for (int b = 0; b < BLK; ++b)
 #pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            if ((__builtin_bit_cast(uint16_t, E(v[i])) & EXP_BITS<E>) == EXP_BITS<E>) v[i] = E(0.f);
-                        v8 pt = pr[0][0];
+                    for (int t = 0; t < 2; ++t)
 #pragma unroll
-                        for (int k = 1; k < BN / 16; ++k) pt = k == t ? pr[k / 2][k % 2] : pt;
-                        o[d] = mfma32(v, pt, o[d]);
-                    }
-#pragma unroll 1
-                for (int k = 0; k < BN; ++k) {
-                    if (k0 + k >= limit) continue;
-                    const int swz = ((k & 3) << 1) | ((k >> 2) & 1);
+                        for (int d = 0; d < DB; ++d) {
+                            chunk v = vfrag(vt, 2 * b + t, d);
 #pragma unroll
-                    for (int d = 0; d < DB; ++d)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const int e = 32 * d + 8 * (r / 4) + 4 * half + r % 4;
-                            const E v = *reinterpret_cast<const E *>(vt + k * DP * 2 + (((e / 8) ^ swz) * 16) + (e % 8) * 2);
-                            if ((__builtin_bit_cast(uint16_t, v) & EXP_BITS<E>) == EXP_BITS<E>) o[d][r] += float(v);
+                            for (int i = 0; i < 8; ++i)
+                                if (odd_value(E(v[i]))) v[i] = E(0.f);
+                            o[d] = Chunk<E>::mma(v, pr[b][t], o[d]);
                         }
-                }
+                add_odd(vt, k0, limit);
                 return;
             }
+#pragma unroll
+            for (int b = 0; b < BLK; ++b)
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) o[d] = Chunk<E>::mma(vfrag(vt, 2 * b + t, d), pr[b][t], o[d]);
+        } else {
+            if (MASK && odd) {
+#pragma unroll
+                for (int b = 0; b < BLK; ++b)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+#pragma unroll
+                        for (int d = 0; d < DB; ++d) {
+                            const float v = vword(vt, b, r, d);
+                            o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(odd_value(v) ? 0.f : v, s[b][r], o[d], 0, 0, 0);
+                        }
+                add_odd(vt, k0, limit);
+                return;
+            }
+#pragma unroll
+            for (int b = 0; b < BLK; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vword(vt, b, r, d), s[b][r], o[d], 0, 0, 0);
         }
-#pragma unroll
-        for (int b = 0; b < BLK; ++b)
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int d = 0; d < DB; ++d) o[d] = mfma32(vfrag(vt, 2 * b + t, d, voff), pr[b][t], o[d]);
     }
 };
 
-// Attention on the matrix cores, 16-bit types.  A wavefront owns 32 rows.
-//   KEYS == false: the workgroup's 4 wavefronts own different rows and share tiles of 64 slots.
-//   KEYS == true (few rows): they own the same rows and tiles of 32 slots in turn, without a
-//   barrier between them, and join their sums at the end.
-// Wavefronts of a workgroup; with wide heads the private tiles of 2 fill the LDS.
-constexpr int attn_waves(int dp, bool few) { return few && dp > 128 ? 2 : 4; }
+// Slots of a tile and wavefronts of a workgroup (KEYS: every wavefront has two stages of tiles of its own).
+template <typename E, int DP, bool KEYS>
+struct Shape {
+    static constexpr int ROW = DP * int(sizeof(E)), BN = KEYS || sizeof(E) == 4 ? 32 : 64, TILE = BN * ROW;
+    static constexpr int NW = !KEYS ? 4 : ROW <= 256 ? 4 : ROW <= 512 ? 2 : 1;
+    static constexpr int TILES = 4 * TILE * (KEYS ? NW : 1), JOIN = KEYS ? NW * 32 * (DP + 6) * 4 : 0;
+    static constexpr int LDS = TILES > JOIN ? TILES : JOIN;
+    static constexpr int GROUPS = LDS <= 80 << 10 && ROW <= 256 ? 2 : 1;  // workgroups a compute unit is to hold
+};
 
+// Attention on the matrix cores.  A wavefront owns 32 rows.
+//   KEYS == false: the workgroup's 4 wavefronts own different rows and share tiles of 64 slots (fp32: 32).
+//   KEYS == true (few rows): they own the same rows and tiles of 32 slots each in turn, without a
+//   barrier between them, and join their sums at the end.
 template <typename E, int DP, bool KEYS, bool ALIGNED>
-__global__ void __launch_bounds__(64 * attn_waves(DP, KEYS), KEYS || DP > 128 ? 1 : 2)
+__global__ void __launch_bounds__((WAVE * Shape<E, DP, KEYS>::NW), (Shape<E, DP, KEYS>::GROUPS))
 attention_mfma_kernel(AttnPlan p, AttnGrid g, const E *__restrict__ q, E *__restrict__ out, float *__restrict__ lse,
                       const E *__restrict__ keys, const E *__restrict__ values, const int32_t *__restrict__ lens,
                       const int32_t *__restrict__ starts) {
-    constexpr int BN = KEYS ? 32 : 64, TILE = BN * DP * 2, NW = attn_waves(DP, KEYS);
+    typedef Shape<E, DP, KEYS> S;
+    typedef typename Chunk<E>::v chunk;
+    constexpr int BN = S::BN, TILE = S::TILE, NW = S::NW, N = Chunk<E>::N;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    typedef typename Elem16<E>::v8 v8;
     Work w;
     if (!find_work(starts, p, g, w)) return;
     const int lane = lane_id(), wv = wave_id(), half = lane >> 5, col = lane & 31;
@@ -476,24 +478,12 @@ attention_mfma_kernel(AttnPlan p, AttnGrid g, const E *__restrict__ q, E *__rest
     st.init();
     const E *qr = q + int64_t(w.first + tok) * p.qt + head * p.qh;
 #pragma unroll
-    for (int t = 0; t < DP / 16; ++t) {
-        union {
-            uint4 u;
-            v8 v;
-        } f;
-        f.u = make_uint4(0, 0, 0, 0);
-        if (real && 16 * t + 8 * half < p.dim) f.u = *reinterpret_cast<const uint4 *>(qr + 16 * t + 8 * half);
-        f.u.x ^= p.flip, f.u.y ^= p.flip, f.u.z ^= p.flip, f.u.w ^= p.flip;
-        st.q[t] = f.v;
-    }
-    int koff[DP / 16], voff[DP / 32];
-#pragma unroll
-    for (int t = 0; t < DP / 16; ++t) koff[t] = col * DP * 2 + (((2 * t + half) ^ (col & 7)) << 4);
-    {
-        const int l16 = lane & 15, f = ((l16 >> 2) << 1) | half;
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d)
-            voff[d] = (4 * half + (l16 >> 2)) * DP * 2 + (((4 * d + 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1)) ^ f) << 4) + (l16 & 1) * 8;
+    for (int t = 0; t < RowState<E, DP, BN>::STEPS; ++t) {
+        uint4 u = make_uint4(0, 0, 0, 0);
+        const int e = (2 * t + half) * N;
+        if (real && e < p.dim) u = *reinterpret_cast<const uint4 *>(qr + e);
+        u.x ^= p.flip, u.y ^= p.flip, u.z ^= p.flip, u.w ^= p.flip;
+        st.q[t] = __builtin_bit_cast(chunk, u);
     }
     const int32_t *table = p.pool.table + int64_t(w.b) * p.pool.max_pages;
     TileLoader<E, DP, BN, KEYS ? 1 : NW, ALIGNED> load;
@@ -510,8 +500,8 @@ attention_mfma_kernel(AttnPlan p, AttnGrid g, const E *__restrict__ q, E *__rest
         char *kt = base + stage * 2 * TILE, *vt = kt + TILE;
         char *nk = base + (stage ^ 1) * 2 * TILE;
         if (k0 + stride < ke) load.request(p, table, keys, values, w.h, k0 + stride, ke, nk, nk + TILE, loader);
-        if (k0 + BN <= all) st.template step<false>(kt, vt, koff, voff, p.scale, k0, limit);
-        else if (k0 < wave_end) st.template step<true>(kt, vt, koff, voff, p.scale, k0, limit);
+        if (k0 + BN <= all) st.template step<false>(kt, vt, p.scale, k0, limit);
+        else if (k0 < wave_end) st.template step<true>(kt, vt, p.scale, k0, limit);
     }
 
     float l = sum_halves(st.l);
@@ -601,6 +591,129 @@ attention_mfma_kernel(AttnPlan p, AttnGrid g, const E *__restrict__ q, E *__rest
     }
 }
 
+// The attention that slots receive, once every row's log-sum is known.  A wavefront keeps the keys of
+// 32 NB slots in registers as the first operand and walks over all rows of its stream and head, tiles
+// of 64 at a time through LDS; a lane's scores are those of one row, so its sums over the rows stay
+// in place until the end, where the lanes of a half are added up in a fixed order.
+template <typename E, int DP, int NB>
+__global__ void __launch_bounds__(256, DP * sizeof(E) <= 256 ? 2 : 1)
+attention_weights_kernel(AttnPlan p, FastDiv by_group, const E *__restrict__ q, const float *__restrict__ lse,
+                         const E *__restrict__ keys, float *__restrict__ weights, const int32_t *__restrict__ lens,
+                         const int32_t *__restrict__ starts) {
+    typedef typename Chunk<E>::v chunk;
+    constexpr int N = Chunk<E>::N, ROW = DP * int(sizeof(E)), STEPS = DP / (2 * N), BM = DP * sizeof(E) <= 512 ? 64 : 32, TILE = BM * ROW;
+    constexpr int CPR = DP / N, RPI = WAVE / CPR, REQ = BM / RPI / 4;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int b = blockIdx.z, h = blockIdx.y, len = stream_len(p, lens, b);
+    const int lane = lane_id(), wv = wave_id(), half = lane >> 5, col = lane & 31;
+    const int s_block = blockIdx.x * (4 * 32 * NB), s0 = s_block + wv * 32 * NB;
+    if (s_block >= len) return;
+    int first, count;
+    stream_tokens(starts, b, p.streams, p.tokens, first, count);
+    const int32_t *table = p.pool.table + int64_t(b) * p.pool.max_pages;
+    chunk k[NB][STEPS];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+        const int s = s0 + 32 * i + col;
+        const int64_t row = s < len ? slot_row(p.pool, table, s, p.kv_heads, h) : -1;
+#pragma unroll
+        for (int t = 0; t < STEPS; ++t) {
+            const int e = (2 * t + half) * N;
+            uint4 u = make_uint4(0, 0, 0, 0);
+            if (row >= 0 && e < p.dim) u = *reinterpret_cast<const uint4 *>(keys + row * p.dim + e);
+            k[i][t] = __builtin_bit_cast(chunk, u);
+        }
+    }
+    // the first token that sees this workgroup's first slot
+    int begin = 0;
+    if (p.causal_block != 0) {
+        const int past = s_block - (len - count);
+        begin = past > 0 ? past / p.causal_block * p.causal_block : 0;
+    }
+    const int rows = count * p.group, r_first = min(begin * p.group, rows) / BM * BM;
+    const E *zero = reinterpret_cast<const E *>(&zero_chunk);
+    auto request = [&](int r0, char *to) {
+#pragma unroll
+        for (int j = 0; j < REQ; ++j) {
+            const int rr = (wv * REQ + j) * RPI + lane / CPR, r = r0 + rr, e = ((lane % CPR) ^ (rr & 7)) * N;
+            const int tok = int(by_group.quot(uint32_t(min(r, rows - 1))));
+            const E *src = r < rows && e < p.dim ? q + int64_t(first + tok) * p.qt + (h * p.group + r - tok * p.group) * p.qh + e : zero;
+            __builtin_amdgcn_global_load_lds((const DC_GLOBAL(void) *)src, (DC_LDS(void) *)(to + (wv * REQ + j) * 1024), 16, 0, 0);
+        }
+    };
+    const float scale = p.flip != 0 ? -p.scale : p.scale;
+    float16_t acc[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
+    if (r_first < rows) request(r_first, lds);
+    int stage = 0;
+    for (int r0 = r_first; r0 < rows; r0 += BM, stage ^= 1) {
+        // this lane's rows: minus their log-sum in powers of two (no row, or one that sees nothing: -inf), and what they see
+        float less[BM / 32];
+        int limit[BM / 32];
+#pragma unroll
+        for (int i = 0; i < BM / 32; ++i) {
+            const int r = r0 + 32 * i + col, tok = int(by_group.quot(uint32_t(min(r, rows - 1))));
+            less[i] = -INFINITY, limit[i] = 0;
+            if (r < rows) {
+                const float z = lse[int64_t(first + tok) * p.q_heads + h * p.group + r - tok * p.group];
+                less[i] = z == -INFINITY ? -INFINITY : z * -1.44269504088896341f;
+                limit[i] = visible(len, count, tok, p.causal_block);
+            }
+        }
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this tile has arrived
+        __syncthreads();
+        const char *qt = lds + stage * TILE;
+        if (r0 + BM < rows) request(r0 + BM, lds + (stage ^ 1) * TILE);
+        const bool whole = s0 + 32 * NB <= visible(len, count, int(by_group.quot(uint32_t(r0))), p.causal_block);
+#pragma unroll
+        for (int j = 0; j < BM / 32; ++j) {
+            float16_t s[NB];
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[i][r] = 0.f;
+#pragma unroll
+            for (int t = 0; t < STEPS; ++t) {
+                const chunk qf = *reinterpret_cast<const chunk *>(qt + (32 * j + col) * ROW + (((2 * t + half) ^ (col & 7)) << 4));
+#pragma unroll
+                for (int i = 0; i < NB; ++i) s[i] = Chunk<E>::mma(k[i][t], qf, s[i]);
+            }
+            if (whole) {
+#pragma unroll
+                for (int i = 0; i < NB; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) acc[i][r] += __builtin_amdgcn_exp2f(fmaf(s[i][r], scale, less[j]));
+            } else {
+#pragma unroll
+                for (int i = 0; i < NB; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const float e = __builtin_amdgcn_exp2f(fmaf(s[i][r], scale, less[j]));
+                        acc[i][r] += s0 + 32 * i + 8 * (r / 4) + 4 * half + r % 4 < limit[j] ? e : 0.f;
+                    }
+            }
+        }
+    }
+    // sums over the 32 lanes of a half; lane `col` keeps sum number `col`
+    float mine = 0.f;
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            float x = acc[i][r];
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) x += __shfl_xor(x, d, WAVE);
+            if (col == 16 * i + r) mine = x;
+        }
+    const int i = col >> 4, r = col & 15, s = s0 + 32 * i + 8 * (r / 4) + 4 * half + r % 4;
+    if (i >= NB || s >= len) return;
+    const int64_t row = slot_row(p.pool, table, s, p.kv_heads, h);
+    if (row >= 0) weights[row] = p.decay == 0.f ? mine : fmaf(p.decay, weights[row], mine);
+}
+
 // Joins the pieces of the slot axis: one wavefront per row.
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -667,44 +780,60 @@ int64_t part_bytes(const AttnPlan &p, const AttnGrid &g) {
     return g.splits > 1 ? int64_t(g.splits) * p.tokens * p.q_heads * (p.dim + 2) * 4 : 0;
 }
 
-template <typename E, int DP, bool KEYS, bool ALIGNED>
-hipError_t attention_go(const dc_attention_args &a, const AttnPlan &p, const AttnGrid &g, float *lse, hipStream_t s) {
-    constexpr int BN = KEYS ? 32 : 64, NW = attn_waves(DP, KEYS);
-    const size_t tiles = size_t(KEYS ? NW : 1) * 4 * BN * DP * 2;
-    const size_t join = KEYS ? size_t(NW) * 32 * (2 + DP + 4) * 4 : 0;
-    const size_t lds = max(tiles, join);
-    auto kernel = attention_mfma_kernel<E, DP, KEYS, ALIGNED>;
-    static thread_local uint64_t raised = 0;  // devices whose limit this instantiation has raised
+// Raises a kernel's limit of dynamic LDS, once per device.
+hipError_t raise_lds(const void *kernel, int bytes, uint64_t &raised) {
     int dev = 0;
     hipError_t err = hipGetDevice(&dev);
+    if (err != hipSuccess || (dev < 64 && (raised >> dev & 1))) return err;
+    err = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (err == hipSuccess && dev < 64) raised |= 1ull << dev;
+    return err;
+}
+
+template <typename E, int DP, bool KEYS, bool ALIGNED>
+hipError_t attention_go(const dc_attention_args &a, const AttnPlan &p, const AttnGrid &g, float *lse, hipStream_t s) {
+    typedef Shape<E, DP, KEYS> S;
+    auto kernel = attention_mfma_kernel<E, DP, KEYS, ALIGNED>;
+    static thread_local uint64_t raised = 0;
+    const hipError_t err = raise_lds((const void *)kernel, S::LDS, raised);
     if (err != hipSuccess) return err;
-    if (dev >= 64 || !(raised >> dev & 1)) {
-        err = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, int(lds));
-        if (err != hipSuccess) return err;
-        if (dev < 64) raised |= 1ull << dev;
-    }
     const int64_t total = int64_t(g.flat) * p.kv_heads * g.splits;
     const int64_t blocks = ceil_div64(total, 8 * g.unit) * 8 * g.unit;
     if (blocks > (1 << 30)) return hipErrorInvalidConfiguration;
     note_kernel("attention_mfma_kernel");
-    kernel<<<dim3(uint32_t(blocks)), NW * WAVE, lds, s>>>(p, g, (const E *)a.q, (E *)a.out, lse, (const E *)a.keys, (const E *)a.values, a.lens, a.starts);
+    kernel<<<dim3(uint32_t(blocks)), S::NW * WAVE, S::LDS, s>>>(p, g, (const E *)a.q, (E *)a.out, lse, (const E *)a.keys, (const E *)a.values,
+                                                               a.lens, a.starts);
+    return hipGetLastError();
+}
+
+template <typename E, int DP, int NB>
+hipError_t weights_go(const dc_attention_args &a, const AttnPlan &p, const AttnGrid &g, const float *lse, hipStream_t s) {
+    auto kernel = attention_weights_kernel<E, DP, NB>;
+    constexpr int BM = DP * sizeof(E) <= 512 ? 64 : 32, LDS = 2 * BM * DP * int(sizeof(E));
+    static thread_local uint64_t raised = 0;
+    const hipError_t err = raise_lds((const void *)kernel, LDS, raised);
+    if (err != hipSuccess) return err;
+    const int64_t blocks = ceil_div64(int64_t(a.max_pages) * a.page_size, 128 * NB);
+    note_kernel("attention_weights_kernel");
+    kernel<<<dim3(uint32_t(blocks), p.kv_heads, p.streams), 256, LDS, s>>>(p, g.by_group, (const E *)a.q, lse, (const E *)a.keys, a.weights,
+                                                                           a.lens, a.starts);
     return hipGetLastError();
 }
 
 template <typename E, int DP>
 hipError_t attention_dp(const dc_attention_args &a, const AttnPlan &p, const AttnGrid &g, bool few, float *lse, hipStream_t s) {
-    const bool aligned = p.pool.page_size % (few ? 32 : 64) == 0;
-    if (few) return aligned ? attention_go<E, DP, true, true>(a, p, g, lse, s) : attention_go<E, DP, true, false>(a, p, g, lse, s);
-    return aligned ? attention_go<E, DP, false, true>(a, p, g, lse, s) : attention_go<E, DP, false, false>(a, p, g, lse, s);
-}
-
-template <typename T>
-hipError_t weights_go(const dc_attention_args &a, const AttnPlan &p, const float *lse, hipStream_t s) {
-    note_kernel("attention_weights_kernel");
-    const int most = int(ceil_div64(int64_t(a.max_pages) * a.page_size, WAVE));
-    attention_weights_kernel<T><<<dim3(most, p.kv_heads, p.streams), 64, 0, s>>>(p, (const T *)a.q, lse, (const T *)a.keys,
-                                                                                a.weights, a.lens, a.starts);
-    return hipGetLastError();
+    const bool aligned = p.pool.page_size % (few ? Shape<E, DP, true>::BN : Shape<E, DP, false>::BN) == 0;
+    hipError_t e = few ? aligned ? attention_go<E, DP, true, true>(a, p, g, lse, s) : attention_go<E, DP, true, false>(a, p, g, lse, s)
+                       : aligned ? attention_go<E, DP, false, true>(a, p, g, lse, s) : attention_go<E, DP, false, false>(a, p, g, lse, s);
+    if (e == hipSuccess && g.splits > 1) {
+        note_kernel("attention_join_kernel");
+        attention_join_kernel<E><<<ceil_div(p.tokens * p.q_heads, 4), 256, 0, s>>>(p, g, (E *)a.out, lse, a.lens, a.starts);
+        e = hipGetLastError();
+    }
+    if (e != hipSuccess || a.weights == nullptr) return e;
+    // 64 slots a wavefront where that leaves a workgroup and more for every compute unit
+    const bool wide = ceil_div64(int64_t(a.max_pages) * a.page_size, 256) * p.kv_heads * p.streams >= 512;
+    return wide ? weights_go<E, DP, 2>(a, p, g, lse, s) : weights_go<E, DP, 1>(a, p, g, lse, s);
 }
 
 AttnPlan make_plan(const dc_attention_args &a) {
@@ -721,59 +850,43 @@ AttnPlan make_plan(const dc_attention_args &a) {
 struct Room {
     int64_t part, lse;
 };
-Room room(const dc_attention_args &a, int dtype) {
+Room room(const dc_attention_args &a) {
     const AttnPlan p = make_plan(a);
     Room r = {0, 0};
-    if (dtype != DC_F32) {
-        const bool few = few_rows(p);
-        r.part = part_bytes(p, plan_grid(p, a.starts != nullptr, few, few ? 32 : 128));
-    }
+    const bool few = few_rows(p);
+    r.part = part_bytes(p, plan_grid(p, a.starts != nullptr, few, few ? 32 : 128));
     if (a.weights != nullptr && a.lse == nullptr) r.lse = int64_t(a.tokens) * a.q_heads * 4;
     return r;
 }
 
 template <typename E>
-hipError_t attention_16(const dc_attention_args &a, AttnPlan p, hipStream_t s) {
-    const Room r = room(a, DC_F16);
+hipError_t attention_t(const dc_attention_args &a, AttnPlan p, hipStream_t s) {
+    const Room r = room(a);
     float *lse = a.lse != nullptr || a.weights == nullptr ? a.lse : (float *)((char *)a.workspace + r.part);
     const bool few = few_rows(p);
     AttnGrid g = plan_grid(p, a.starts != nullptr, few, few ? 32 : 128);
     g.part = (float *)a.workspace;
-    AttnPlan m = p;
-    // exponentials are powers of two; a negative scale turns q's signs instead, so that the largest score has the largest product
-    m.flip = p.scale < 0.f ? 0x80008000u : 0u;
-    m.scale = fabsf(p.scale) * 1.44269504088896341f;
-    hipError_t e = p.dim <= 64 ? attention_dp<E, 64>(a, m, g, few, lse, s) : p.dim <= 128 ? attention_dp<E, 128>(a, m, g, few, lse, s)
-                                                                                 : attention_dp<E, 256>(a, m, g, few, lse, s);
-    if (e == hipSuccess && g.splits > 1) {
-        note_kernel("attention_join_kernel");
-        attention_join_kernel<E><<<ceil_div(p.tokens * p.q_heads, 4), 256, 0, s>>>(m, g, (E *)a.out, lse, a.lens, a.starts);
-        e = hipGetLastError();
-    }
-    return e == hipSuccess && a.weights != nullptr ? weights_go<E>(a, p, lse, s) : e;
-}
-
-hipError_t attention_32(const dc_attention_args &a, const AttnPlan &p, hipStream_t s) {
-    float *lse = a.lse != nullptr || a.weights == nullptr ? a.lse : (float *)a.workspace;
-    note_kernel("paged_attention_kernel");
-    paged_attention_kernel<float><<<dim3(p.tokens, p.q_heads), 64, 0, s>>>(p, (const float *)a.q, (float *)a.out, lse, (const float *)a.keys,
-                                                                          (const float *)a.values, a.lens, a.starts);
-    const hipError_t e = hipGetLastError();
-    return e == hipSuccess && a.weights != nullptr ? weights_go<float>(a, p, lse, s) : e;
+    // exponentials are powers of two; with a negative scale q changes its signs instead, so that the largest
+    // product has the largest score
+    p.flip = p.scale < 0.f ? sizeof(E) == 2 ? 0x80008000u : 0x80000000u : 0u;
+    // (a scale of zero: as good as zero, but -inf times it stays -inf)
+    p.scale = fmaxf(fabsf(p.scale) * 1.44269504088896341f, 1.2e-38f);
+    return p.dim <= 64 ? attention_dp<E, 64>(a, p, g, few, lse, s) : p.dim <= 128 ? attention_dp<E, 128>(a, p, g, few, lse, s)
+                                                                                 : attention_dp<E, 256>(a, p, g, few, lse, s);
 }
 
 }  // namespace
 
-int64_t paged_attention_workspace(const dc_attention_args &a, int dtype) {
-    const Room r = room(a, dtype);
+int64_t paged_attention_workspace(const dc_attention_args &a) {
+    const Room r = room(a);
     return r.part + r.lse;
 }
 
 hipError_t launch_paged_attention(const dc_attention_args &a, int dtype, hipStream_t s) {
     const AttnPlan p = make_plan(a);
-    if (dtype == DC_F32) return attention_32(a, p, s);
-    if (dtype == DC_BF16) return attention_16<bf16_t>(a, p, s);
-    return attention_16<half_t>(a, p, s);
+    if (dtype == DC_F32) return attention_t<float>(a, p, s);
+    if (dtype == DC_BF16) return attention_t<bf16_t>(a, p, s);
+    return attention_t<half_t>(a, p, s);
 }
 
 }  // namespace dc

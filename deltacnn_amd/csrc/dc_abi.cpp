@@ -1066,7 +1066,7 @@ int dc_rotary(const dc_rotary_args *a, int dtype, void *stream) {
 
 int64_t dc_paged_attention_workspace(const dc_attention_args *a, int dtype) {
     int rc = check_attention(a, dtype);
-    return rc != DC_OK ? rc : dc::paged_attention_workspace(*a, dtype);
+    return rc != DC_OK ? rc : dc::paged_attention_workspace(*a);
 }
 
 int dc_paged_attention(const dc_attention_args *a, int dtype, void *stream) {
@@ -1093,7 +1093,7 @@ int dc_paged_attention(const dc_attention_args *a, int dtype, void *stream) {
     const size_t pool = size_t(a->num_pages) * a->kv_heads * a->page_size * a->dim * esize(dtype);
     if (out.meets(q) || out.meets(Span(a->keys, pool)) || out.meets(Span(a->values, pool)))
         return fail(DC_ERR_UNSUPPORTED, "%s: out overlaps an operand", fn);
-    const int64_t need = dc::paged_attention_workspace(*a, dtype);
+    const int64_t need = dc::paged_attention_workspace(*a);
     if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need))
         return fail(DC_ERR_NULL, "%s: needs %lld bytes of workspace", fn, (long long)need);
     if (need > 0) DC_REQUIRE_ALIGNED("dc_paged_attention", a->workspace, 16);

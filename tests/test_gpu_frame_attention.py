@@ -235,6 +235,94 @@ def test_paged_attention(lib, dtype, shape):
     ref.assert_within(w, want0, tol0, "weights, decay 0")
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 3.0])
+@pytest.mark.parametrize("tokens", [2, 70])
+def test_paged_attention_scales(lib, dtype, scale, tokens):
+    """Negative, zero and large scales, causal and not, rows of a wider buffer as q and out."""
+    from deltacnn_amd import hip_kernels as hk
+    gen = torch.Generator().manual_seed(31 + tokens)
+    heads, kv, dim, page, lens = 4, 2, 48, 32, [100, 75]
+    keys, values, weights, _, table = make_pool(gen, 2, 128, kv, page, dim, dtype)
+    wide = torch.randn(2 * tokens, heads * dim + 16, generator=gen).to(dtype)
+    q = wide[:, :heads * dim].view(2 * tokens, heads, dim)
+    lens_t = torch.tensor(lens, dtype=torch.int32)
+    for block in (0, 1):
+        out, tol, lse, lse_tol, ww, w_tol = ref.attention(q, keys, values, table, lens_t, None, scale, block, weights, 1.0)
+        buf = torch.full((2 * tokens, heads * dim + 24), 5.0, dtype=dtype, device=DEV)
+        w = weights.to(DEV)
+        wd = wide.to(DEV)
+        got = hk.paged_attention(wd[:, :heads * dim].view(2 * tokens, heads, dim), keys.to(DEV), values.to(DEV), table.to(DEV),
+                                 lens_t.to(DEV), scale=scale, causal_block=block, weights=w,
+                                 out=buf[:, 8:8 + heads * dim].view(2 * tokens, heads, dim))
+        ref.assert_within(got, out, tol, "out")
+        ref.assert_within(w, ww, w_tol, "weights")
+        assert bool((buf[:, :8] == 5).all()) and bool((buf[:, 8 + heads * dim:] == 5).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("tokens", [3, 150])
+def test_paged_attention_masked_infinities(lib, dtype, tokens):
+    """Infinities and NaN in keys and values that a row does not see leave it alone; rows that see
+    them get what the definition says."""
+    from deltacnn_amd import hip_kernels as hk
+    gen = torch.Generator().manual_seed(12)
+    dim, page, past = 64, 32, 20
+    n = past + tokens
+    keys, values, weights, _, table = make_pool(gen, 1, n, 1, page, dim, dtype)
+    bad = n - max(1, tokens // 2)  # seen by the later rows alone
+    pg, off = ref.place(table[0], bad, page)
+    values[pg, 0, off, 3], values[pg, 0, off, 40], values[pg, 0, off, 41] = math.nan, math.inf, -math.inf
+    q = torch.randn(tokens, 1, dim, generator=gen).to(dtype)
+    lens_t = torch.tensor([n], dtype=torch.int32)
+    out, tol, lse, lse_tol, _, _ = ref.attention(q, keys, values, table, lens_t, None, None, 1)
+    got = hk.paged_attention(q.to(DEV), keys.to(DEV), values.to(DEV), table.to(DEV), lens_t.to(DEV), causal_block=1)
+    assert bool(out[:, 0, 3].isnan().any()) and not bool(out[:, 0, 3].isnan().all()) and bool((out[:, 0, 40] == math.inf).any())
+    tol = torch.where(out.isfinite(), tol, 0.0)
+    ref.assert_within(got, out, tol, "values")
+    keys[pg, 0, off, 5] = math.nan  # a key: the rows that see it are NaN, the others are not
+    out, tol, lse, lse_tol, _, _ = ref.attention(q, keys, torch.nan_to_num(values, 0, 0, 0), table, lens_t, None, None, 1)
+    w = torch.zeros_like(weights).to(DEV)
+    got, got_lse = hk.paged_attention(q.to(DEV), keys.to(DEV), torch.nan_to_num(values, 0, 0, 0).to(DEV), table.to(DEV), lens_t.to(DEV),
+                                      causal_block=1, weights=w, return_lse=True)
+    seen = torch.arange(tokens) + past >= bad
+    assert torch.equal(got.isnan().all(2).all(1).cpu(), seen) and torch.equal(got.isnan().any(2).any(1).cpu(), seen)
+    ref.assert_within(got[~seen.to(DEV)], out[~seen], tol[~seen], "rows that do not see the key")
+    ref.assert_within(got_lse, lse, torch.where(lse.isfinite(), lse_tol, 0.0), "lse")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("tokens,page", [(2, 32), (2, 20), (80, 64), (80, 20)])
+def test_paged_attention_lost_page_and_rows_behind(lib, dtype, tokens, page):
+    """A page outside the pool makes its own stream NaN and no other; rows behind the last stream stay."""
+    from deltacnn_amd import hip_kernels as hk
+    gen = torch.Generator().manual_seed(3)
+    dim, lens = 32, [90, 130, 41]
+    keys, values, weights, _, table = make_pool(gen, 3, 140, 1, page, dim, dtype)
+    table[1, 1] = keys.shape[0] if page > 20 else -1
+    counts = [tokens, tokens, tokens - 1]
+    starts = starts_of(counts)
+    total = sum(counts) + 4
+    q = torch.randn(total, 2, dim, generator=gen).to(dtype)
+    lens_t = torch.tensor(lens, dtype=torch.int32)
+    safe = table.clone()
+    safe[1] = safe[0]
+    out, tol, lse, _, _, _ = ref.attention(q[:sum(counts)], keys, values, safe, lens_t, starts, None, 0)
+    buf = torch.full((total, 2, dim), 9.0, dtype=dtype, device=DEV)
+    w = weights.to(DEV)
+    got = hk.paged_attention(q.to(DEV), keys.to(DEV), values.to(DEV), table.to(DEV), lens_t.to(DEV), starts=starts.to(DEV), out=buf, weights=w)
+    second = slice(counts[0], 2 * tokens)
+    assert bool(got[second].isnan().all()) and bool((got[sum(counts):] == 9).all())
+    for part in (slice(0, tokens), slice(2 * tokens, sum(counts))):
+        ref.assert_within(got[part], out[part], tol[part], "other streams")
+    touched = torch.zeros(keys.shape[0], dtype=torch.bool)
+    for b in (0, 1, 2):
+        for i in range(-(-lens[b] // page)):
+            if 0 <= int(table[b, i]) < keys.shape[0]:
+                touched[int(table[b, i])] = True
+    assert torch.equal(w.cpu()[~touched], weights[~touched])
+
+
 # ---- cache_slots ----
 
 SLOTS = [  # counts, lens, budget, kv_heads, page, protect
