@@ -118,7 +118,8 @@ class SlotsArgs(ctypes.Structure):
         ("weights", c_void_p), ("stamps", c_void_p), ("keep_from", c_void_p),
         ("page_table", c_void_p), ("lens", c_void_p), ("starts", c_void_p),
         ("streams", c_int32), ("tokens", c_int32), ("kv_heads", c_int32), ("num_pages", c_int32),
-        ("page_size", c_int32), ("max_pages", c_int32), ("budget", c_int32), ("slots", c_void_p), ("new_lens", c_void_p)]
+        ("page_size", c_int32), ("max_pages", c_int32), ("budget", c_int32), ("slots", c_void_p), ("new_lens", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_int64)]
 
 
 CONV_GROUP_MAX = 8
@@ -159,6 +160,7 @@ _SIGNATURES = {
     "dc_paged_attention": (c_int, [POINTER(AttentionArgs), c_int, _P]),
     "dc_paged_attention_workspace": (c_int64, [POINTER(AttentionArgs), c_int]),
     "dc_cache_slots": (c_int, [POINTER(SlotsArgs), _P]),
+    "dc_cache_slots_workspace": (c_int64, [POINTER(SlotsArgs)]),
 }
 
 _lib = None

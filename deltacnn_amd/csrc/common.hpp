@@ -433,6 +433,7 @@ hipError_t launch_rotary(const dc_rotary_args &a, int dtype, hipStream_t s);
 hipError_t launch_paged_attention(const dc_attention_args &a, int dtype, hipStream_t s);
 int64_t paged_attention_workspace(const dc_attention_args &a);
 hipError_t launch_cache_slots(const dc_slots_args &a, hipStream_t s);
+int64_t cache_slots_workspace(const dc_slots_args &a);
 
 // Fused depthwise -> projection (-> expansion) block.  block_unsupported names the reason a
 // shape is outside the kernel's range (nullptr: supported as far as the shape check goes);

@@ -1010,6 +1010,17 @@ int check_attention(const dc_attention_args *a, int dtype) {
     return DC_OK;
 }
 
+int check_slots(const dc_slots_args *a) {
+    const char *fn = "dc_cache_slots";
+    if (a == nullptr) return fail(DC_ERR_NULL, "%s: args is NULL", fn);
+    int rc = check_heads(fn, a->tokens, 1, a->kv_heads, 1);
+    if (rc != DC_OK) return rc;
+    if ((rc = check_pool(fn, a->streams, a->num_pages, a->page_size, a->max_pages, a->tokens, a->page_table, a->starts)) != DC_OK) return rc;
+    if (a->budget <= 0 || a->budget > (int64_t)a->max_pages * a->page_size)
+        return fail(DC_ERR_SHAPE, "%s: budget=%d is not 1 .. %lld, the slots of a stream", fn, a->budget, (long long)a->max_pages * a->page_size);
+    return DC_OK;
+}
+
 }  // namespace
 
 int dc_rotary(const dc_rotary_args *a, int dtype, void *stream) {
@@ -1100,15 +1111,16 @@ int dc_paged_attention(const dc_attention_args *a, int dtype, void *stream) {
     return finish(dc::launch_paged_attention(*a, dtype, (hipStream_t)stream), fn);
 }
 
+int64_t dc_cache_slots_workspace(const dc_slots_args *a) {
+    int rc = check_slots(a);
+    return rc != DC_OK ? rc : dc::cache_slots_workspace(*a);
+}
+
 int dc_cache_slots(const dc_slots_args *a, void *stream) {
     dc::kernel_log_reset();
     const char *fn = "dc_cache_slots";
-    if (a == nullptr) return fail(DC_ERR_NULL, "%s: args is NULL", fn);
-    int rc = check_heads(fn, a->tokens, 1, a->kv_heads, 1);
+    int rc = check_slots(a);
     if (rc != DC_OK) return rc;
-    if ((rc = check_pool(fn, a->streams, a->num_pages, a->page_size, a->max_pages, a->tokens, a->page_table, a->starts)) != DC_OK) return rc;
-    if (a->budget <= 0 || a->budget > (int64_t)a->max_pages * a->page_size)
-        return fail(DC_ERR_SHAPE, "%s: budget=%d is not 1 .. %lld, the slots of a stream", fn, a->budget, (long long)a->max_pages * a->page_size);
     DC_REQUIRE_PTR("dc_cache_slots", a->weights);
     DC_REQUIRE_PTR("dc_cache_slots", a->lens);
     DC_REQUIRE_PTR("dc_cache_slots", a->slots);
@@ -1122,6 +1134,10 @@ int dc_cache_slots(const dc_slots_args *a, void *stream) {
     DC_REQUIRE_ALIGNED("dc_cache_slots", a->new_lens, 4);
     if (Span(a->lens, size_t(a->streams) * 4).meets(Span(a->new_lens, size_t(a->streams) * 4)))
         return fail(DC_ERR_UNSUPPORTED, "%s: new_lens overlaps lens", fn);
+    const int64_t need = dc::cache_slots_workspace(*a);
+    if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need))
+        return fail(DC_ERR_NULL, "%s: needs %lld bytes of workspace", fn, (long long)need);
+    if (need > 0) DC_REQUIRE_ALIGNED("dc_cache_slots", a->workspace, 16);
     return finish(dc::launch_cache_slots(*a, (hipStream_t)stream), fn);
 }
 

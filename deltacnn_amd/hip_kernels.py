@@ -948,6 +948,11 @@ def cache_slots(weights, page_table, lens, tokens, budget, *, starts=None, stamp
         new_lens = torch.empty((streams,), dtype=torch.int32, device=weights.device)
         a.weights, a.page_table, a.lens, a.slots, a.new_lens = (t.data_ptr() for t in (weights, page_table, lens, slots, new_lens))
         a.starts, a.stamps, a.keep_from = _ptr(starts), _ptr(stamps), _ptr(keep_from)
+        need = lib.dc_cache_slots_workspace(ctypes.byref(a))
+        if need < 0:
+            _lib.check(int(need))
+        workspace = torch.empty(need, dtype=torch.uint8, device=weights.device) if need else None
+        a.workspace, a.workspace_bytes = _ptr(workspace), need
         _call("cache_slots", lib.dc_cache_slots, (ctypes.byref(a), _stream()), tokens=tokens, kv_heads=kv, lens=lens,
-              with_stamps=stamps is not None, keep=(a, starts, keep_from, slots, new_lens))
+              with_stamps=stamps is not None, keep=(a, starts, keep_from, slots, new_lens, workspace))
     return slots, new_lens

@@ -581,6 +581,8 @@ typedef struct dc_slots_args {
     int32_t budget;                 /* slots a stream may use, at most max_pages * page_size */
     int32_t *slots;                 /* [kv_heads][T] */
     int32_t *new_lens;              /* [streams]; must not be lens */
+    void *workspace;                /* dc_cache_slots_workspace bytes, 16-byte aligned */
+    int64_t workspace_bytes;
 } dc_slots_args;
 
 /* Where the new tokens of every stream and kv head go: into the slots of the tokens that have
@@ -591,6 +593,8 @@ typedef struct dc_slots_args {
  * n, n + 1, ..; a token without room below max(budget, n) gets -1.  new_lens = min(n + c - e,
  * max(budget, n)).  No key or value moves, so a head's slots are in no order of time afterwards. */
 int dc_cache_slots(const dc_slots_args *args, void *stream);
+/* Bytes of workspace that the call needs (0: none; negative: a dc_status). */
+int64_t dc_cache_slots_workspace(const dc_slots_args *args);
 
 #ifdef __cplusplus
 }

@@ -330,6 +330,8 @@ SLOTS = [  # counts, lens, budget, kv_heads, page, protect
     ([3, 0, 7], [50, 9, 1], 50, 3, 16, 5), ([40], [40], 40, 2, 49, 3), ([9], [64], 64, 1, 64, 0),  # all protected
     ([200], [1000], 1000, 2, 100, 8), ([64, 64], [2500, 2499], 2500, 1, 64, 7), ([30], [10], 20, 1, 30, None),
     ([12, 12], [100, 3], 40, 1, 10, 4),       # one stream is over its budget already: it does not shrink
+    ([700], [9000], 9000, 1, 64, 7), ([50], [20000], 20000, 1, 128, 8),    # several slots a thread
+    ([3000, 10], [40000, 33000], 40000, 1, 64, 6), ([2100], [70000], 70000, 2, 100, 1),  # cut into pieces
 ]
 
 
