@@ -723,83 +723,117 @@ def sparse_concatenate(a, b, out=None):
 
 
 # ---- attention over the frames of a video stream (include/deltacnn_hip.h) ----
+# One token of one stream takes the device a few microseconds, so the checks below are ordered for
+# the call that passes them: cheap tests first, messages only once something is wrong.
 
-def _expect(ok, message):
-    if not ok:
-        raise _lib.DeltaCNNError(-2, message)
+def _refuse(message, code=-2):
+    raise _lib.DeltaCNNError(code, message)
 
 
-def _resident(name, device, **tensors):
-    """Every operand lives on the device of the call, and nothing asks for a gradient."""
-    for what, t in tensors.items():
+def _same_device(name, what, tensors) -> int:
+    """Index of the device that every operand lives on; nothing may ask for a gradient."""
+    grad = torch.is_grad_enabled()
+    try:
+        device = tensors[0].get_device()
+        ok = device >= 0
+        for t in tensors:
+            if t is not None and (t.get_device() != device or (grad and t.requires_grad)):
+                ok = False
+    except AttributeError:
+        ok = False
+    if ok:
+        return device
+    for w, t in zip(what, tensors):
         if t is None:
             continue
         if not isinstance(t, torch.Tensor) or not t.is_cuda:
-            raise _lib.DeltaCNNError(-4, f"{name}: {what} must be a tensor on the GPU")
-        _expect(t.device == device, f"{name}: {what} lives on {t.device}, the call on {device}")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise _lib.DeltaCNNError(-3, f"{name}: {what} asks for a gradient (the operator has none: call it under torch.no_grad())")
+            _refuse(f"{name}: {w} must be a tensor on the GPU", -4)
+        if t.device != tensors[0].device:
+            _refuse(f"{name}: {w} lives on {t.device}, {what[0]} on {tensors[0].device}")
+        if t.requires_grad and grad:
+            _refuse(f"{name}: {w} asks for a gradient (the operator has none: call it under torch.no_grad())", -3)
+    raise AssertionError("unreachable")
 
 
 def _words(name, what, t, shape, dtype=torch.int32):
-    if t is not None:
-        _expect(t.dtype == dtype and tuple(t.shape) == tuple(shape) and t.is_contiguous(),
-                f"{name}: {what} must be a dense {str(dtype)[6:]} tensor {tuple(shape)}, got {str(t.dtype)[6:]} {tuple(t.shape)}")
+    """A dense tensor of this type and shape."""
+    if t is not None and not (t.dtype is dtype and t.shape == shape and t.is_contiguous()):
+        _refuse(f"{name}: {what} must be a dense {str(dtype)[6:]} tensor {tuple(shape)}, got {str(t.dtype)[6:]} {tuple(t.shape)}")
 
 
-def _rows(name, what, t, dtype=None, dim=None):
-    """Strides of [tokens][heads][dim] rows whose elements are dense; a dimension of one element may
-    have any stride in torch, and gets the dense one here."""
-    _expect(t.dim() == 3 and 0 not in t.shape, f"{name}: {what} must be [tokens, heads, dim], got {tuple(t.shape)}")
-    _expect(dtype is None or t.dtype == dtype, f"{name}: {what} is {str(t.dtype)[6:]}, expected {str(dtype)[6:]}")
-    _expect(dim is None or t.shape[2] == dim, f"{name}: {what} has {t.shape[2]} elements a head, expected {dim}")
-    tokens, heads, d = t.shape
-    _expect(t.stride(2) == 1 or d == 1, f"{name}: the elements of a head of {what} must be dense")
-    head = t.stride(1) if heads > 1 else d
-    return (t.stride(0) if tokens > 1 else max(heads * head, d)), head
+def _rows(name, what, t, shape, dtype):
+    """(token, head) strides of [tokens, heads, dim] rows whose elements are dense; a dimension of one
+    element may have any stride in torch, and gets the dense one here."""
+    if t.shape != shape or t.dtype is not dtype:
+        _refuse(f"{name}: {what} is {str(t.dtype)[6:]} {tuple(t.shape)}, expected {str(dtype)[6:]} {tuple(shape)}")
+    ts, hs, ds = t.stride()
+    tokens, heads, dim = shape
+    if ds != 1 and dim != 1:
+        _refuse(f"{name}: the elements of a head of {what} must be dense")
+    if heads == 1:
+        hs = dim
+    return (ts if tokens > 1 else heads * hs), hs
+
+
+def _queries(name, q):
+    if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.numel() == 0:
+        _refuse(f"{name}: the first operand must be a [tokens, heads, dim] tensor with elements")
+    return q.shape
 
 
 def _pool(name, keys, values, page_table, dtype):
-    _expect(keys.dim() == 4 and keys.is_contiguous() and 0 not in keys.shape,
-            f"{name}: keys must be a dense [pages, kv_heads, page_size, dim] tensor, got {tuple(keys.shape)}")
-    _expect(values.shape == keys.shape and values.is_contiguous(), f"{name}: values {tuple(values.shape)} do not match keys {tuple(keys.shape)}")
-    _expect(keys.dtype == dtype and values.dtype == dtype, f"{name}: the cache holds {str(keys.dtype)[6:]}, the call has {str(dtype)[6:]}")
-    _table(name, page_table)
-    return keys.shape
+    """Sizes of a paged cache: (pages, kv_heads, page_size, dim), (streams, pages of a stream)."""
+    shape = keys.shape
+    if len(shape) != 4 or 0 in shape or not keys.is_contiguous():
+        _refuse(f"{name}: keys must be a dense [pages, kv_heads, page_size, dim] tensor, got {tuple(shape)}")
+    if values.shape != shape or not values.is_contiguous():
+        _refuse(f"{name}: values {tuple(values.shape)} do not match keys {tuple(shape)}")
+    if keys.dtype is not dtype or values.dtype is not dtype:
+        _refuse(f"{name}: the cache holds {str(keys.dtype)[6:]} and {str(values.dtype)[6:]}, the call has {str(dtype)[6:]}")
+    return shape, _table(name, page_table)
 
 
 def _table(name, page_table):
-    _expect(page_table.dim() == 2 and 0 not in page_table.shape and page_table.dtype == torch.int32 and page_table.is_contiguous(),
-            f"{name}: page_table must be a dense int32 [streams, pages of a stream] tensor")
+    shape = page_table.shape
+    if len(shape) != 2 or 0 in shape or page_table.dtype is not torch.int32 or not page_table.is_contiguous():
+        _refuse(f"{name}: page_table must be a dense int32 [streams, pages of a stream] tensor")
+    return shape
+
+
+def _launch(op, fn, device, args, meta):
+    """``fn(*args, stream)`` on the operands' device and its current stream; ``meta()`` is for tracers."""
+    if torch.cuda.current_device() != device:
+        with torch.cuda.device(device):
+            return _launch(op, fn, device, args, meta)
+    args += (torch._C._cuda_getCurrentRawStream(device),)
+    if _TRACER is None:
+        rc = fn(*args)
+        if rc != 0:
+            _lib.check(rc)
+    else:
+        _call(op, fn, args, **meta())
 
 
 def rotary_frequencies(sections: Sequence[int], base: float = 10000.0, device=None) -> torch.Tensor:
     """Angular frequencies of :func:`rotary` and :func:`rotary_append`: a ladder of its own for each
     axis, ``base ** (-2 i / n)`` for pair ``i`` of the ``n`` rotated elements of that axis, as the
     float64 tensor the operators take (a far position times a rounded frequency is a wrong angle)."""
-    _expect(len(sections) > 0 and all(int(n) >= 0 and int(n) % 2 == 0 for n in sections), f"rotary_frequencies: sections {tuple(sections)} must be even")
+    if len(sections) == 0 or any(int(n) < 0 or int(n) % 2 for n in sections):
+        _refuse(f"rotary_frequencies: sections {tuple(sections)} must be even")
     rows = [float(base) ** (-torch.arange(0, int(n), 2, dtype=torch.float64) / int(n)) for n in sections if int(n) > 0]
     return torch.cat(rows).to(device) if rows else torch.empty(0, dtype=torch.float64, device=device)
 
 
-def _rotary_args(name, q, positions, frequencies, sections, interleaved, out):
-    sections = [int(n) for n in sections]
-    _expect(1 <= len(sections) <= 4, f"{name}: 1 .. 4 axes, got sections {tuple(sections)}")
-    a = _lib.RotaryArgs()
-    a.tokens, a.q_heads, a.dim = q.shape[0], q.shape[1], q.shape[2]
-    a.q_token_stride, a.q_head_stride = _rows(name, "q", q)
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _expect(out.shape == q.shape, f"{name}: out {tuple(out.shape)} does not match q {tuple(q.shape)}")
-    a.out_token_stride, a.out_head_stride = _rows(name, "out", out, q.dtype)
-    _words(name, "positions", positions, (q.shape[0], len(sections)))
+_SECTIONS = ctypes.c_int32 * 4
+
+
+def _sections(name, sections, tokens, positions, frequencies):
+    axes = len(sections)
+    if not 1 <= axes <= 4:
+        _refuse(f"{name}: 1 .. 4 axes, got sections {tuple(sections)}")
+    _words(name, "positions", positions, (tokens, axes))
     _words(name, "frequencies", frequencies, (sum(sections) // 2,), torch.float64)
-    a.q, a.out, a.positions, a.frequencies = q.data_ptr(), out.data_ptr(), positions.data_ptr(), frequencies.data_ptr()
-    a.axes = len(sections)
-    for i, n in enumerate(sections):
-        a.sections[i] = n
-    a.interleaved = int(bool(interleaved))
-    return a, out
+    return axes, _SECTIONS(*sections)
 
 
 def rotary(x, positions, frequencies, sections, *, interleaved=False, inverse=False, out=None):
@@ -810,14 +844,19 @@ def rotary(x, positions, frequencies, sections, *, interleaved=False, inverse=Fa
     ``positions`` is int32 [tokens, axes], ``frequencies`` float64 (:func:`rotary_frequencies`).
     ``inverse`` turns back, which is also how a gradient passes through.  ``out`` may be ``x``."""
     lib = _lib.load()
-    _expect(isinstance(x, torch.Tensor) and x.dim() == 3, "rotary: x must be [tokens, heads, dim]")
-    _resident("rotary", x.device, x=x, positions=positions, frequencies=frequencies, out=out)
-    dt = _dtype(x)
-    a, out = _rotary_args("rotary", x, positions, frequencies, sections, interleaved, out)
-    a.inverse = int(bool(inverse))
-    with torch.cuda.device(x.device):
-        _call("rotary", lib.dc_rotary, (ctypes.byref(a), dt, _stream()), tokens=x.shape[0], q_heads=x.shape[1], kv_heads=0,
-              dim=x.shape[2], axes=len(sections), esize=x.element_size(), keep=(a, x, positions, frequencies, out))
+    shape = _queries("rotary", x)
+    device = _same_device("rotary", ("x", "positions", "frequencies", "out"), (x, positions, frequencies, out))
+    dt, dtype = _dtype(x), x.dtype
+    tokens, heads, dim = shape
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=x.device)
+    axes, sec = _sections("rotary", sections, tokens, positions, frequencies)
+    xs, xh = _rows("rotary", "x", x, shape, dtype)
+    os_, oh = _rows("rotary", "out", out, shape, dtype)
+    a = _lib.RotaryArgs(tokens, heads, 0, dim, x.data_ptr(), xs, xh, out.data_ptr(), os_, oh, positions.data_ptr(), axes, sec,
+                        frequencies.data_ptr(), bool(interleaved), bool(inverse))
+    _launch("rotary", lib.dc_rotary, device, (ctypes.byref(a), dt), lambda: dict(
+        tokens=tokens, q_heads=heads, kv_heads=0, dim=dim, axes=axes, esize=x.element_size(), keep=(a, x, positions, frequencies, out)))
     return out
 
 
@@ -835,19 +874,24 @@ def rotary_append(q, k, v, positions, frequencies, sections, keys, values, page_
     A token whose slot is negative, or lies in a page outside the pool, is not stored."""
     lib = _lib.load()
     name = "rotary_append"
-    _expect(isinstance(q, torch.Tensor) and q.dim() == 3, f"{name}: q must be [tokens, heads, dim]")
-    _resident(name, q.device, q=q, k=k, v=v, positions=positions, frequencies=frequencies, keys=keys, values=values,
-              page_table=page_table, slots=slots, starts=starts, weights=weights, stamps=stamps, token_stamps=token_stamps,
-              lens=lens, new_lens=new_lens, out=out)
-    dt = _dtype(q)
-    pages, kv, page, dim = _pool(name, keys, values, page_table, q.dtype)
-    a, out = _rotary_args(name, q, positions, frequencies, sections, interleaved, out)
-    tokens, streams = q.shape[0], page_table.shape[0]
-    _expect(q.shape[2] == dim, f"{name}: q has {q.shape[2]} elements a head, the cache {dim}")
-    _expect(k.shape == (tokens, kv, dim) and v.shape == (tokens, kv, dim),
-            f"{name}: k {tuple(k.shape)} and v {tuple(v.shape)} must be {(tokens, kv, dim)}")
-    a.k_token_stride, a.k_head_stride = _rows(name, "k", k, q.dtype)
-    a.v_token_stride, a.v_head_stride = _rows(name, "v", v, q.dtype)
+    shape = _queries(name, q)
+    device = _same_device(name, ("q", "k", "v", "positions", "frequencies", "keys", "values", "page_table", "slots", "starts",
+                                 "weights", "stamps", "token_stamps", "lens", "new_lens", "out"),
+                          (q, k, v, positions, frequencies, keys, values, page_table, slots, starts, weights, stamps,
+                           token_stamps, lens, new_lens, out))
+    dt, dtype = _dtype(q), q.dtype
+    tokens, heads, dim = shape
+    pool, (streams, most) = _pool(name, keys, values, page_table, dtype)
+    pages, kv, page, cached_dim = pool
+    if dim != cached_dim:
+        _refuse(f"{name}: q has {dim} elements a head, the cache {cached_dim}")
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=q.device)
+    axes, sec = _sections(name, sections, tokens, positions, frequencies)
+    qs, qh = _rows(name, "q", q, shape, dtype)
+    os_, oh = _rows(name, "out", out, shape, dtype)
+    ks, kh = _rows(name, "k", k, (tokens, kv, dim), dtype)
+    vs, vh = _rows(name, "v", v, (tokens, kv, dim), dtype)
     _words(name, "slots", slots, (kv, tokens))
     _words(name, "starts", starts, (streams + 1,))
     _words(name, "weights", weights, (pages, kv, page), torch.float32)
@@ -855,15 +899,15 @@ def rotary_append(q, k, v, positions, frequencies, sections, keys, values, page_
     _words(name, "token_stamps", token_stamps, (tokens,))
     _words(name, "lens", lens, (streams,))
     _words(name, "new_lens", new_lens, (streams,))
-    _expect(lens is None or new_lens is not None, f"{name}: lens without new_lens")
-    a.kv_heads, a.streams, a.num_pages, a.page_size, a.max_pages = kv, streams, pages, page, page_table.shape[1]
-    a.k, a.v, a.keys, a.values, a.page_table, a.slots = (t.data_ptr() for t in (k, v, keys, values, page_table, slots))
-    a.starts, a.weights, a.stamps, a.token_stamps, a.lens, a.new_lens = (
-        _ptr(t) for t in (starts, weights, stamps, token_stamps, lens, new_lens))
-    with torch.cuda.device(q.device):
-        _call("rotary_append", lib.dc_rotary, (ctypes.byref(a), dt, _stream()), tokens=tokens, q_heads=q.shape[1], kv_heads=kv,
-              dim=dim, axes=len(sections), esize=q.element_size(), with_weights=weights is not None, with_stamps=stamps is not None,
-              keep=(a, q, k, v, positions, frequencies, slots, starts, token_stamps, new_lens, out))
+    if lens is not None and new_lens is None:
+        _refuse(f"{name}: lens without new_lens")
+    a = _lib.RotaryArgs(tokens, heads, kv, dim, q.data_ptr(), qs, qh, out.data_ptr(), os_, oh, positions.data_ptr(), axes, sec,
+                        frequencies.data_ptr(), bool(interleaved), 0, k.data_ptr(), v.data_ptr(), ks, kh, vs, vh, keys.data_ptr(),
+                        values.data_ptr(), _ptr(weights), _ptr(stamps), _ptr(token_stamps), page_table.data_ptr(), slots.data_ptr(),
+                        _ptr(starts), streams, pages, page, most, _ptr(lens), _ptr(new_lens))
+    _launch(name, lib.dc_rotary, device, (ctypes.byref(a), dt), lambda: dict(
+        tokens=tokens, q_heads=heads, kv_heads=kv, dim=dim, axes=axes, esize=q.element_size(), with_weights=weights is not None,
+        with_stamps=stamps is not None, keep=(a, q, k, v, positions, frequencies, slots, starts, token_stamps, new_lens, out)))
     return out
 
 
@@ -883,37 +927,37 @@ def paged_attention(q, keys, values, page_table, lens, *, starts=None, scale=Non
     heads that share its head; pages must then not be shared between streams."""
     lib = _lib.load()
     name = "paged_attention"
-    _expect(isinstance(q, torch.Tensor) and q.dim() == 3, f"{name}: q must be [tokens, heads, dim]")
-    _resident(name, q.device, q=q, keys=keys, values=values, page_table=page_table, lens=lens, starts=starts, weights=weights, out=out)
-    dt = _dtype(q)
-    pages, kv, page, dim = _pool(name, keys, values, page_table, q.dtype)
-    tokens, heads = q.shape[:2]
-    streams = page_table.shape[0]
-    a = _lib.AttentionArgs()
-    a.q_token_stride, a.q_head_stride = _rows(name, "q", q, dim=dim)
+    shape = _queries(name, q)
+    device = _same_device(name, ("q", "keys", "values", "page_table", "lens", "starts", "weights", "out"),
+                          (q, keys, values, page_table, lens, starts, weights, out))
+    dt, dtype = _dtype(q), q.dtype
+    tokens, heads, dim = shape
+    pool, (streams, most) = _pool(name, keys, values, page_table, dtype)
+    pages, kv, page, cached_dim = pool
+    if dim != cached_dim:
+        _refuse(f"{name}: q has {dim} elements a head, the cache {cached_dim}")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _expect(out.shape == q.shape, f"{name}: out {tuple(out.shape)} does not match q {tuple(q.shape)}")
-    a.out_token_stride, a.out_head_stride = _rows(name, "out", out, q.dtype)
+        out = torch.empty(shape, dtype=dtype, device=q.device)
+    qs, qh = _rows(name, "q", q, shape, dtype)
+    os_, oh = _rows(name, "out", out, shape, dtype)
     _words(name, "lens", lens, (streams,))
     _words(name, "starts", starts, (streams + 1,))
     _words(name, "weights", weights, (pages, kv, page), torch.float32)
     lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_lse else None
-    a.tokens, a.q_heads, a.kv_heads, a.dim = tokens, heads, kv, dim
-    a.streams, a.num_pages, a.page_size, a.max_pages = streams, pages, page, page_table.shape[1]
-    a.q, a.out, a.keys, a.values, a.page_table, a.lens = (t.data_ptr() for t in (q, out, keys, values, page_table, lens))
-    a.lse, a.starts, a.weights = _ptr(lse), _ptr(starts), _ptr(weights)
-    a.causal_block, a.decay = int(causal_block), float(decay)
-    a.scale = float(dim) ** -0.5 if scale is None else float(scale)
-    need = lib.dc_paged_attention_workspace(ctypes.byref(a), dt)
-    if need < 0:
-        _lib.check(int(need))
-    with torch.cuda.device(q.device):
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        a.workspace, a.workspace_bytes = _ptr(workspace), need
-        _call("paged_attention", lib.dc_paged_attention, (ctypes.byref(a), dt, _stream()), tokens=tokens, q_heads=heads, kv_heads=kv,
-              dim=dim, esize=q.element_size(), lens=lens, starts=starts, causal_block=int(causal_block),
-              with_weights=weights is not None, keep=(a, q, lse, out, workspace))
+    a = _lib.AttentionArgs(tokens, heads, kv, dim, q.data_ptr(), qs, qh, out.data_ptr(), os_, oh, _ptr(lse), keys.data_ptr(),
+                           values.data_ptr(), page_table.data_ptr(), lens.data_ptr(), _ptr(starts), streams, pages, page, most,
+                           int(causal_block), dim ** -0.5 if scale is None else float(scale), _ptr(weights), float(decay))
+    ref = ctypes.byref(a)
+    need = lib.dc_paged_attention_workspace(ref, dt)
+    workspace = None
+    if need:
+        if need < 0:
+            _lib.check(int(need))
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), need
+    _launch(name, lib.dc_paged_attention, device, (ref, dt), lambda: dict(
+        tokens=tokens, q_heads=heads, kv_heads=kv, dim=dim, esize=q.element_size(), lens=lens, starts=starts,
+        causal_block=int(causal_block), with_weights=weights is not None, keep=(a, q, lse, out, workspace)))
     return (out, lse) if return_lse else out
 
 
@@ -929,30 +973,36 @@ def cache_slots(weights, page_table, lens, tokens, budget, *, starts=None, stamp
     stream that already uses more than ``budget`` does not shrink; a token beyond it gets slot -1."""
     lib = _lib.load()
     name = "cache_slots"
-    _expect(isinstance(weights, torch.Tensor) and weights.dim() == 3 and 0 not in weights.shape, f"{name}: weights must be [pages, kv_heads, page_size]")
-    _resident(name, weights.device, weights=weights, page_table=page_table, lens=lens, starts=starts, stamps=stamps, keep_from=keep_from)
-    _words(name, "weights", weights, weights.shape, torch.float32)
-    _table(name, page_table)
-    pages, kv, page = weights.shape
-    streams, tokens, budget = page_table.shape[0], int(tokens), int(budget)
-    _expect(0 < tokens, f"{name}: tokens={tokens}")
+    device = _same_device(name, ("weights", "page_table", "lens", "starts", "stamps", "keep_from"),
+                          (weights, page_table, lens, starts, stamps, keep_from))
+    shape = weights.shape
+    if len(shape) != 3 or 0 in shape:
+        _refuse(f"{name}: weights must be [pages, kv_heads, page_size], got {tuple(shape)}")
+    _words(name, "weights", weights, shape, torch.float32)
+    streams, most = _table(name, page_table)
+    pages, kv, page = shape
+    tokens, budget = int(tokens), int(budget)
+    if tokens <= 0:
+        _refuse(f"{name}: tokens={tokens}")
     _words(name, "lens", lens, (streams,))
     _words(name, "starts", starts, (streams + 1,))
-    _words(name, "stamps", stamps, weights.shape)
+    _words(name, "stamps", stamps, shape)
     _words(name, "keep_from", keep_from, (streams,))
-    _expect((stamps is None) == (keep_from is None), f"{name}: stamps and keep_from go together")
-    a = _lib.SlotsArgs()
-    a.streams, a.tokens, a.kv_heads, a.num_pages, a.page_size, a.max_pages, a.budget = streams, tokens, kv, pages, page, page_table.shape[1], budget
-    with torch.cuda.device(weights.device):
-        slots = torch.empty((kv, tokens), dtype=torch.int32, device=weights.device)
-        new_lens = torch.empty((streams,), dtype=torch.int32, device=weights.device)
-        a.weights, a.page_table, a.lens, a.slots, a.new_lens = (t.data_ptr() for t in (weights, page_table, lens, slots, new_lens))
-        a.starts, a.stamps, a.keep_from = _ptr(starts), _ptr(stamps), _ptr(keep_from)
-        need = lib.dc_cache_slots_workspace(ctypes.byref(a))
+    if (stamps is None) != (keep_from is None):
+        _refuse(f"{name}: stamps and keep_from go together")
+    slots = torch.empty((kv, tokens), dtype=torch.int32, device=weights.device)
+    new_lens = torch.empty((streams,), dtype=torch.int32, device=weights.device)
+    a = _lib.SlotsArgs(weights.data_ptr(), _ptr(stamps), _ptr(keep_from), page_table.data_ptr(), lens.data_ptr(), _ptr(starts),
+                       streams, tokens, kv, pages, page, most, budget, slots.data_ptr(), new_lens.data_ptr())
+    ref = ctypes.byref(a)
+    need = lib.dc_cache_slots_workspace(ref)
+    workspace = None
+    if need:
         if need < 0:
             _lib.check(int(need))
-        workspace = torch.empty(need, dtype=torch.uint8, device=weights.device) if need else None
-        a.workspace, a.workspace_bytes = _ptr(workspace), need
-        _call("cache_slots", lib.dc_cache_slots, (ctypes.byref(a), _stream()), tokens=tokens, kv_heads=kv, lens=lens,
-              with_stamps=stamps is not None, keep=(a, starts, keep_from, slots, new_lens, workspace))
+        workspace = torch.empty(need, dtype=torch.uint8, device=weights.device)
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), need
+    _launch(name, lib.dc_cache_slots, device, (ref,), lambda: dict(
+        tokens=tokens, kv_heads=kv, lens=lens, esize=4, with_stamps=stamps is not None,
+        keep=(a, starts, keep_from, slots, new_lens, workspace)))
     return slots, new_lens
