@@ -27,6 +27,8 @@ __device__ __forceinline__ int visible(int len, int count, int i, int block) {
 __device__ __forceinline__ int stream_len(const AttnPlan &p, const int32_t *lens, int b) {
     return int(min(int64_t(max(lens[b], 0)), int64_t(p.pool.max_pages) * p.pool.page_size));
 }
+// A value that is the same in all lanes, as a scalar.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 typedef float float16_t __attribute__((ext_vector_type(16)));
 typedef float float2v_t __attribute__((ext_vector_type(2)));
@@ -34,7 +36,6 @@ typedef half_t half2v_t __attribute__((ext_vector_type(2)));
 typedef bf16_t bf16x2_t __attribute__((ext_vector_type(2)));
 typedef short short4_t __attribute__((ext_vector_type(4)));
 #define DC_LDS(T) __attribute__((address_space(3))) T
-#define DC_GLOBAL(T) __attribute__((address_space(1))) T
 
 // 32 x 32 outputs, 16 reduction elements.  Operand A: lane (half, m) holds A[m][8 half + i]; operand B the
 // same of its columns; result: lane (half, n) holds rows 8 (r / 4) + 4 half + r % 4 of column n, r = 0 .. 15.
@@ -51,12 +52,13 @@ template <typename E>
 struct Chunk {
     static constexpr int N = 8;
     typedef typename Elem16<E>::v8 v;
+    typedef typename Elem16<E>::v4 v4;
     static __device__ __forceinline__ float16_t mma(v a, v b, float16_t c) { return mfma32(a, b, c); }
 };
 template <>
 struct Chunk<float> {
     static constexpr int N = 4;
-    typedef float4_t v;
+    typedef float4_t v, v4;
     static __device__ __forceinline__ float16_t mma(v a, v b, float16_t c) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
@@ -160,53 +162,102 @@ __device__ __forceinline__ bool find_work(const int32_t *starts, const AttnPlan 
     return true;
 }
 
-// BN slots of one head on their way into LDS, 16 bytes a lane and request, straight from memory.  Row r of
-// a tile is DP elements; its 16-byte chunk c lies at place c ^ swizzle(r), so that the reads below touch
-// every bank once (the lanes choose what they fetch, the places they fill are fixed).  What lies behind
-// `end` or in no page of the pool, and the elements from dim to DP, arrive as zeros.
+// 16 bytes a lane from memory straight into LDS: lane l's go to `to` + 16 l.  Written as assembly because
+// the compiler, which knows such a request of its own making for a write to LDS, waits for all of them in
+// front of every transposing read (it cannot tell the two stages apart): that wait cost a third of the
+// kernel's time.  There is no output register; arrived() below is the wait, in front of every barrier or read
+// that needs the data.
+__device__ __forceinline__ uint32_t lds_place(const char *to) { return uint32_t(__builtin_amdgcn_readfirstlane(uint32_t(uintptr_t((DC_LDS(const char) *)to)))); }
+template <typename V>
+__device__ __forceinline__ V lds_read(uint32_t at) {
+    return *(DC_LDS(const V) *)(uintptr_t)at;
+}
+__device__ __forceinline__ void fetch_bounded(u32x4_t resource, uint32_t offset, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(offset), "s"(resource), "s"(to) : "memory");
+}
+__device__ __forceinline__ void fetch(const void *from, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "memory");
+}
+__device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// Where 16-byte chunk c of row r of a tile lies: at place c ^ swizzle(r) of the row.  The LDS serves 256 bytes a
+// cycle from 64 banks: of keys 16 rows' chunks side by side, of values 32 lanes of the transposing read,
+// 64 bytes of each of four consecutive rows.  Both hit every bank once this way.  fp32 values are read as
+// words along a row.
+template <typename E, int DP>
+__device__ __forceinline__ int key_swizzle(int row) {
+    return DP * int(sizeof(E)) >= 256 ? row & 15 : row >> 1 & 7;
+}
+template <typename E, int DP>
+__device__ __forceinline__ int value_swizzle(int row) {
+    return sizeof(E) == 4 ? 0 : DP >= 128 ? (row & 3) << 2 : (row & 2) << 1;
+}
+
+// BN slots of one head on their way into LDS.  The lanes choose what they fetch, the places they fill are
+// fixed.  What lies behind `end` or in no page of the pool, and the elements from dim to DP, arrive as
+// zeros: from the bound of the buffer resource where a tile lies in one page (ALIGNED), else from a
+// chunk of zeros.
 template <typename E, int DP, int BN, int LOADERS, bool ALIGNED>
 struct TileLoader {
     static constexpr int N = Chunk<E>::N, CPR = DP / N, RPI = WAVE / CPR, REQ = BN / RPI / LOADERS;
     static_assert(REQ >= 1, "one request a wavefront at least");
-    int row0, dim;
+    const int32_t *table;
+    const E *keys, *values;  // ALIGNED: from this head's first row of a page
+    int dim, h, page_size, num_pages;
     bool bad = false;
+    // ALIGNED: bytes of a lane from the tile's first element; page and place in it of the tile to be requested next
+    uint32_t koffset[REQ], voffset[REQ], page_bytes, row_bytes;
+    int index, inside, page;
 
-    static __device__ __forceinline__ int kswz(int row) { return row & 7; }
-    static __device__ __forceinline__ int vswz(int row) { return sizeof(E) == 2 ? ((row & 3) << 1) | ((row >> 2) & 1) : 0; }
-
-    __device__ __forceinline__ void init(int loader, int dim_) {
-        dim = dim_;
-        row0 = loader * REQ * RPI + lane_id() / CPR;
-    }
-    __device__ __forceinline__ void request(const AttnPlan &p, const int32_t *table, const E *keys, const E *values, int h, int k0, int end,
-                                            char *kt, char *vt, int loader) {
-        const int c = lane_id() % CPR;
+    __device__ __forceinline__ void init(const AttnPlan &p, const int32_t *table_, const E *k, const E *v, int h_, int loader, int k0) {
+        table = table_, dim = p.dim, h = h_, page_size = p.pool.page_size, num_pages = p.pool.num_pages;
+        const int64_t head = ALIGNED ? int64_t(h) * page_size * dim : 0;
+        keys = k + head, values = v + head;
         if constexpr (ALIGNED) {
-            const int i = int(p.pool.by_page.quot(uint32_t(k0)));
-            const int page = __builtin_amdgcn_readfirstlane(table[i]);
-            const bool ok = uint32_t(page) < uint32_t(p.pool.num_pages);
+            row_bytes = uint32_t(dim) * sizeof(E);
+            page_bytes = uint32_t(p.kv_heads) * page_size * row_bytes;
+            index = uniform(p.pool.by_page.quot(uint32_t(k0)));
+            inside = uniform(k0 - index * page_size);
+            page = 0;
+            const int c = lane_id() % CPR, row0 = loader * REQ * RPI + lane_id() / CPR;
+#pragma unroll
+            for (int j = 0; j < REQ; ++j) {
+                const int row = row0 + j * RPI, ck = c ^ key_swizzle<E, DP>(row), cv = c ^ value_swizzle<E, DP>(row);
+                koffset[j] = ck * N < dim ? uint32_t(row * dim + ck * N) * sizeof(E) : 0x40000000u;
+                voffset[j] = cv * N < dim ? uint32_t(row * dim + cv * N) * sizeof(E) : 0x40000000u;
+            }
+        }
+    }
+    // The page of the next tile, a step ahead of its request.
+    __device__ __forceinline__ void look() {
+        if constexpr (ALIGNED) page = table[index];
+    }
+    __device__ __forceinline__ void advance(int by) {
+        if constexpr (ALIGNED) {
+            inside += by;
+            while (inside >= page_size) inside -= page_size, ++index;
+        }
+    }
+    // Slots [k0, end) of the tile into LDS places kt, vt (of this wavefront's first row)
+    __device__ __forceinline__ void request(const AttnPlan &p, int loader, int k0, int end, uint32_t kt, uint32_t vt) {
+        if constexpr (ALIGNED) {
+            const uint32_t pg = uint32_t(uniform(page));
+            const bool ok = pg < uint32_t(num_pages);
             bad = bad || !ok;
-            const uint64_t base = ok ? uint64_t(((int64_t(page) * p.kv_heads + h) * p.pool.page_size + (k0 - i * p.pool.page_size)) * dim) : 0;
-            const uint64_t at = uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(uint32_t(base)))) |
-                                uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(uint32_t(base >> 32)))) << 32;
-            const int bytes = __builtin_amdgcn_readfirstlane(ok ? min(BN, end - k0) * dim * int(sizeof(E)) : 0);
-            const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<E *>(keys) + at, 0, bytes, 0x00027000);
-            const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<E *>(values) + at, 0, bytes, 0x00027000);
+            const uint64_t at = ok ? uint64_t(pg) * page_bytes + uint32_t(inside) * row_bytes : 0;
+            const uint64_t ka = uint64_t(uintptr_t(keys)) + at, va = uint64_t(uintptr_t(values)) + at;
+            u32x4_t rk, rv;
+            rk[0] = uniform(uint32_t(ka)), rk[1] = uniform(uint32_t(ka >> 32) & 0xffffu);
+            rv[0] = uniform(uint32_t(va)), rv[1] = uniform(uint32_t(va >> 32) & 0xffffu);
+            rk[2] = rv[2] = uniform(ok ? min(BN, end - k0) * row_bytes : 0u), rk[3] = rv[3] = 0x00027000u;
 #pragma unroll
-            for (int j = 0; j < REQ; ++j) {
-                const int row = row0 + j * RPI, ck = c ^ kswz(row);
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (DC_LDS(void) *)(kt + (loader * REQ + j) * 1024), 16,
-                                                         ck * N < dim ? (row * dim + ck * N) * int(sizeof(E)) : 0x40000000, 0, 0, 0);
-            }
+            for (int j = 0; j < REQ; ++j) fetch_bounded(rk, koffset[j], kt + j * 1024);
 #pragma unroll
-            for (int j = 0; j < REQ; ++j) {
-                const int row = row0 + j * RPI, cv = c ^ vswz(row);
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (DC_LDS(void) *)(vt + (loader * REQ + j) * 1024), 16,
-                                                         cv * N < dim ? (row * dim + cv * N) * int(sizeof(E)) : 0x40000000, 0, 0, 0);
-            }
+            for (int j = 0; j < REQ; ++j) fetch_bounded(rv, voffset[j], vt + j * 1024);
         } else {
             const E *zero = reinterpret_cast<const E *>(&zero_chunk);
             const E *kp[REQ], *vp[REQ];
+            const int c = lane_id() % CPR, row0 = loader * REQ * RPI + lane_id() / CPR;
 #pragma unroll
             for (int j = 0; j < REQ; ++j) {
                 const int row = row0 + j * RPI, s = k0 + row;
@@ -215,16 +266,14 @@ struct TileLoader {
                     at = slot_row(p.pool, table, s, p.kv_heads, h);
                     bad = bad || at < 0;
                 }
-                const int ck = c ^ kswz(row), cv = c ^ vswz(row);
+                const int ck = c ^ key_swizzle<E, DP>(row), cv = c ^ value_swizzle<E, DP>(row);
                 kp[j] = at >= 0 && ck * N < dim ? keys + at * dim + ck * N : zero;
                 vp[j] = at >= 0 && cv * N < dim ? values + at * dim + cv * N : zero;
             }
 #pragma unroll
-            for (int j = 0; j < REQ; ++j)
-                __builtin_amdgcn_global_load_lds((const DC_GLOBAL(void) *)kp[j], (DC_LDS(void) *)(kt + (loader * REQ + j) * 1024), 16, 0, 0);
+            for (int j = 0; j < REQ; ++j) fetch(kp[j], kt + j * 1024);
 #pragma unroll
-            for (int j = 0; j < REQ; ++j)
-                __builtin_amdgcn_global_load_lds((const DC_GLOBAL(void) *)vp[j], (DC_LDS(void) *)(vt + (loader * REQ + j) * 1024), 16, 0, 0);
+            for (int j = 0; j < REQ; ++j) fetch(vp[j], vt + j * 1024);
         }
     }
 };
@@ -239,11 +288,10 @@ template <typename E, int DP, int BN>
 struct RowState {
     typedef typename Chunk<E>::v chunk;
     static constexpr int ROW = DP * int(sizeof(E)), BLK = BN / 32, STEPS = DP / (2 * Chunk<E>::N), DB = DP / 32;
-    static constexpr int VOFF = sizeof(E) == 2 ? DB : 1;
     float16_t o[DB];
     float m, l;
     chunk q[STEPS];
-    int koff[STEPS], voff[VOFF];  // this lane's places in a tile of keys / values
+    int koff, voff;  // this lane's places in a tile of keys / values
 
     __device__ __forceinline__ void init() {
         m = -INFINITY, l = 0.f;
@@ -251,38 +299,37 @@ struct RowState {
         for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
-        const int lane = lane_id(), half = lane >> 5, col = lane & 31;
-#pragma unroll
-        for (int t = 0; t < STEPS; ++t) koff[t] = col * ROW + (((2 * t + half) ^ (col & 7)) << 4);
-        if constexpr (sizeof(E) == 2) {
-            const int l16 = lane & 15, f = ((l16 >> 2) << 1) | half;
-#pragma unroll
-            for (int d = 0; d < DB; ++d)
-                voff[d] = (4 * half + (l16 >> 2)) * ROW + (((4 * d + 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1)) ^ f) << 4) + (l16 & 1) * 8;
-        } else {
-            voff[0] = 4 * half * ROW + col * 4;
-        }
+        const int lane = lane_id(), half = lane >> 5, col = lane & 31, l16 = lane & 15;
+        koff = col * ROW + ((half ^ key_swizzle<E, DP>(col)) << 4);
+        if constexpr (sizeof(E) == 2)
+            voff = (4 * half + (l16 >> 2)) * ROW + (((2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1)) ^ value_swizzle<E, DP>(l16 >> 2)) << 4) + (l16 & 1) * 8;
+        else
+            voff = 4 * half * ROW + col * 4;
     }
 
+    // Operand t of the keys: chunk 2 t + half of row 32 b + col, at a place that differs from that of t = 0 in
+    // the bits of t alone (rows, tiles and stages are whole multiples of their range)
+    __device__ __forceinline__ chunk kfrag(uint32_t kt, int b, int t) const { return lds_read<chunk>(((kt + koff) ^ (t << 5)) + b * 32 * ROW); }
     // 16-bit: V^T fragment of 32 elements x 16 slots: slot 16 t + 8 e + 4 half + i of the tile in element 4 e + i
-    __device__ __forceinline__ chunk vfrag(const char *vt, int t, int d) const {
+    __device__ __forceinline__ chunk vfrag(uint32_t vt, int t, int d) const {
         union {
             short4_t h[2];
             chunk v;
         } f;
+        const uint32_t at = (vt + voff) ^ (d << 6);
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-            f.h[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DC_LDS(short4_t) *)(vt + voff[d] + (16 * t + 8 * e) * ROW));
+            f.h[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DC_LDS(short4_t) *)(uintptr_t)(at + (16 * t + 8 * e) * ROW));
         return f.v;
     }
     // fp32: element 32 d + col of slot 32 b + 8 (r / 4) + 4 half + r % 4
-    __device__ __forceinline__ float vword(const char *vt, int b, int r, int d) const {
-        return *reinterpret_cast<const float *>(vt + voff[0] + (32 * b + 8 * (r / 4) + r % 4) * ROW + 128 * d);
+    __device__ __forceinline__ float vword(uint32_t vt, int b, int r, int d) const {
+        return lds_read<float>(vt + voff + (32 * b + 8 * (r / 4) + r % 4) * ROW + 128 * d);
     }
 
     // Slots that some rows see and others do not may hold infinities or NaN, and 0 * inf would carry them
     // over: such elements leave the product and join the rows that see them one by one.
-    __device__ __forceinline__ bool any_odd(const char *vt) const {
+    __device__ __forceinline__ bool any_odd(uint32_t vt) const {
         bool odd = false;
         if constexpr (sizeof(E) == 2) {
 #pragma unroll
@@ -303,37 +350,55 @@ struct RowState {
         }
         return ballot(odd) != 0;
     }
-    __device__ __forceinline__ void add_odd(const char *vt, int k0, int limit) {
+    __device__ __forceinline__ void add_odd(uint32_t vt, int k0, int limit) {
+        constexpr int N = Chunk<E>::N;
         const int half = lane_id() >> 5;
 #pragma unroll 1
         for (int k = 0; k < BN; ++k) {
             if (k0 + k >= limit) continue;
-            const int swz = TileLoader<E, DP, BN, 1, true>::vswz(k);
-            const char *row = vt + k * ROW;
+            const int swz = value_swizzle<E, DP>(k) << 4;
+            const uint32_t row = vt + k * ROW;
 #pragma unroll
             for (int d = 0; d < DB; ++d)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    constexpr int N = Chunk<E>::N;
-                    const int e = 32 * d + 8 * (r / 4) + 4 * half + r % 4;
-                    const E v = *reinterpret_cast<const E *>(row + (((e / N) ^ swz) * 16) + (e % N) * int(sizeof(E)));
-                    if (odd_value(v)) o[d][r] += float(v);
+                for (int j = 0; j < 4; ++j) {
+                    const int e = 32 * d + 8 * j + 4 * half;  // four elements side by side in one chunk
+                    const typename Chunk<E>::v4 v = lds_read<typename Chunk<E>::v4>(row + (((e / N) << 4) ^ swz) + (e % N) * int(sizeof(E)));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (odd_value(E(v[i]))) o[d][4 * j + i] += float(E(v[i]));
                 }
         }
     }
 
     // One tile: slots [k0, k0 + BN); this lane's row sees slots below `limit` (MASK: some row does not see some of the tile's)
     template <bool MASK>
-    __device__ __forceinline__ void step(const char *kt, const char *vt, float scale, int k0, int limit) {
+    __device__ __forceinline__ void step(uint32_t kt, uint32_t vt, float scale, int k0, int limit) {
+        // LDS answers after some hundred cycles, three products' time: a block's operands are requested in one
+        // go, those of the next block before the products of this one, and the first values before the
+        // exponentials (left to itself the compiler asks for two operands at a time and waits for each)
         float16_t s[BLK];
+        chunk kf[2][STEPS];
+#pragma unroll
+        for (int t = 0; t < STEPS; ++t) kf[0][t] = kfrag(kt, 0, t);
 #pragma unroll
         for (int b = 0; b < BLK; ++b) {
+            if (b + 1 < BLK) {
+#pragma unroll
+                for (int t = 0; t < STEPS; ++t) kf[(b + 1) & 1][t] = kfrag(kt, b + 1, t);
+            }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[b][r] = 0.f;
 #pragma unroll
-            for (int t = 0; t < STEPS; ++t)
-                s[b] = Chunk<E>::mma(*reinterpret_cast<const chunk *>(kt + koff[t] + b * 32 * ROW), q[t], s[b]);
+            for (int t = 0; t < STEPS; ++t) s[b] = Chunk<E>::mma(kf[b & 1][t], q[t], s[b]);
         }
+        chunk vf[2][sizeof(E) == 2 ? DB : 1];
+        if constexpr (sizeof(E) == 2) {
+#pragma unroll
+            for (int d = 0; d < DB; ++d) vf[0][d] = vfrag(vt, 0, d);
+        }
+        __builtin_amdgcn_sched_barrier(0);
         const int half = lane_id() >> 5;
         if constexpr (MASK) {
 #pragma unroll
@@ -360,13 +425,15 @@ struct RowState {
                 for (int r = 0; r < 16; ++r) o[d][r] *= fade;
         }
         const float ref = m == -INFINITY ? 0.f : m;
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int b = 0; b < BLK; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 s[b][r] = __builtin_amdgcn_exp2f(fmaf(s[b][r], scale, -ref));
-                l += s[b][r];
+                part[r & 3] += s[b][r];
             }
+        l += (part[0] + part[1]) + (part[2] + part[3]);
         bool odd = false;
         if constexpr (MASK) odd = any_odd(vt);
         if constexpr (sizeof(E) == 2) {
@@ -402,11 +469,15 @@ struct RowState {
                 return;
             }
 #pragma unroll
-            for (int b = 0; b < BLK; ++b)
+            for (int t = 0; t < BN / 16; ++t) {
+                if (t + 1 < BN / 16) {
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
+                    for (int d = 0; d < DB; ++d) vf[(t + 1) & 1][d] = vfrag(vt, t + 1, d);
+                }
 #pragma unroll
-                    for (int d = 0; d < DB; ++d) o[d] = Chunk<E>::mma(vfrag(vt, 2 * b + t, d), pr[b][t], o[d]);
+                for (int d = 0; d < DB; ++d) o[d] = Chunk<E>::mma(vf[t & 1][d], pr[t / 2][t % 2], o[d]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         } else {
             if (MASK && odd) {
 #pragma unroll
@@ -453,26 +524,25 @@ attention_mfma_kernel(AttnPlan p, AttnGrid g, const E *__restrict__ q, E *__rest
     typedef Shape<E, DP, KEYS> S;
     typedef typename Chunk<E>::v chunk;
     constexpr int BN = S::BN, TILE = S::TILE, NW = S::NW, N = Chunk<E>::N;
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+    extern __shared__ __attribute__((aligned(1024))) char lds[];  // whole rows of any tile: see kfrag()
     Work w;
     if (!find_work(starts, p, g, w)) return;
     const int lane = lane_id(), wv = wave_id(), half = lane >> 5, col = lane & 31;
-    const int len = stream_len(p, lens, w.b);
+    const int len = uniform(stream_len(p, lens, w.b));
     const int rows = w.count * p.group;
     const int r0 = w.rb * g.block_rows, row = r0 + (KEYS ? 0 : wv * 32) + col;
     const int tok = int(g.by_group.quot(uint32_t(min(row, rows - 1))));
     const int head = w.h * p.group + min(row, rows - 1) - tok * p.group;
     const bool real = row < rows;
     const int last_tok = int(g.by_group.quot(uint32_t(min(r0 + g.block_rows, rows) - 1)));
-    const int end_all = visible(len, w.count, last_tok, p.causal_block);  // slots that any row of the workgroup sees
+    const int end_all = uniform(visible(len, w.count, last_tok, p.causal_block));  // slots that any row of the workgroup sees
     const int kb = w.split * g.split_keys, ke = min(end_all, kb + g.split_keys);
     if (kb >= end_all && w.split > 0) return;  // nothing: the joining launch knows
     const int limit = real ? min(visible(len, w.count, tok, p.causal_block), ke) : 0;
-    // slots below `all` are seen by every row of this wavefront
-    const int wave_r0 = r0 + (KEYS ? 0 : wv * 32);
-    const int all = wave_r0 < rows ? min(visible(len, w.count, int(g.by_group.quot(uint32_t(wave_r0))), p.causal_block), ke) : 0;
-    const int wave_last = min(wave_r0 + 32, rows) - 1;
-    const int wave_end = wave_r0 < rows ? min(visible(len, w.count, int(g.by_group.quot(uint32_t(wave_last))), p.causal_block), ke) : 0;
+    // slots below `all` are seen by every row of the workgroup, those from wave_end by none of this wavefront's
+    const int all = uniform(min(visible(len, w.count, int(g.by_group.quot(uint32_t(r0))), p.causal_block), ke));
+    const int wave_r0 = r0 + (KEYS ? 0 : wv * 32), wave_last = min(wave_r0 + 32, rows) - 1;
+    const int wave_end = uniform(wave_r0 < rows ? min(visible(len, w.count, int(g.by_group.quot(uint32_t(wave_last))), p.causal_block), ke) : 0);
 
     RowState<E, DP, BN> st;
     st.init();
@@ -486,22 +556,38 @@ attention_mfma_kernel(AttnPlan p, AttnGrid g, const E *__restrict__ q, E *__rest
         st.q[t] = __builtin_bit_cast(chunk, u);
     }
     const int32_t *table = p.pool.table + int64_t(w.b) * p.pool.max_pages;
-    TileLoader<E, DP, BN, KEYS ? 1 : NW, ALIGNED> load;
-    const int loader = KEYS ? 0 : wv;
-    load.init(loader, p.dim);
-    char *base = KEYS ? lds + wv * 4 * TILE : lds;  // [stage][K, V]
-    const int first = kb + (KEYS ? wv * BN : 0), stride = KEYS ? NW * BN : BN;
-    if (first < ke) load.request(p, table, keys, values, w.h, first, ke, base, base + TILE, loader);
-    int stage = 0;
-    for (int k0 = first; k0 < ke; k0 += stride, stage ^= 1) {
-        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this tile has arrived
-        if constexpr (KEYS) __builtin_amdgcn_wave_barrier();
-        else __syncthreads();                // .. everybody's part of it, and the other stage is free
-        char *kt = base + stage * 2 * TILE, *vt = kt + TILE;
-        char *nk = base + (stage ^ 1) * 2 * TILE;
-        if (k0 + stride < ke) load.request(p, table, keys, values, w.h, k0 + stride, ke, nk, nk + TILE, loader);
-        if (k0 + BN <= all) st.template step<false>(kt, vt, p.scale, k0, limit);
-        else if (k0 < wave_end) st.template step<true>(kt, vt, p.scale, k0, limit);
+    typedef TileLoader<E, DP, BN, KEYS ? 1 : NW, ALIGNED> Loader;
+    Loader load;
+    const int loader = KEYS ? 0 : wv, first = kb + (KEYS ? wv * BN : 0), stride = KEYS ? NW * BN : BN;
+    load.init(p, table, keys, values, w.h, loader, first);
+    const uint32_t place = lds_place(lds) + (KEYS ? wv * 4 * TILE : 0), mine = place + loader * Loader::REQ * 1024;  // [stage][K, V]
+    if (first < ke) {
+        load.look();
+        load.request(p, loader, first, ke, mine, mine + TILE);
+        load.advance(stride);
+        if (first + stride < ke) load.look();
+    }
+    uint32_t stage = 0;
+    int k0 = first;
+    // the next tile's requests and the page of the one behind it, once this tile is there
+    auto turn = [&]() {
+        arrived();                             // this tile, of this wavefront's requests
+        if constexpr (!KEYS) __syncthreads();  // .. of everybody's, and the other stage is free
+        if (k0 + stride < ke) {
+            const uint32_t to = mine + (stage ^ 2 * TILE);
+            load.request(p, loader, k0 + stride, ke, to, to + TILE);
+            load.advance(stride);
+            if (k0 + 2 * stride < ke) load.look();
+        }
+    };
+    // tiles that every row of the workgroup sees as a whole, then the rest
+    for (; k0 + BN <= all; k0 += stride, stage ^= 2 * TILE) {
+        turn();
+        st.template step<false>(place + stage, place + stage + TILE, p.scale, k0, limit);
+    }
+    for (; k0 < ke; k0 += stride, stage ^= 2 * TILE) {
+        turn();
+        if (k0 < wave_end) st.template step<true>(place + stage, place + stage + TILE, p.scale, k0, limit);
     }
 
     float l = sum_halves(st.l);
@@ -603,8 +689,8 @@ attention_weights_kernel(AttnPlan p, FastDiv by_group, const E *__restrict__ q, 
     typedef typename Chunk<E>::v chunk;
     constexpr int N = Chunk<E>::N, ROW = DP * int(sizeof(E)), STEPS = DP / (2 * N), BM = DP * sizeof(E) <= 512 ? 64 : 32, TILE = BM * ROW;
     constexpr int CPR = DP / N, RPI = WAVE / CPR, REQ = BM / RPI / 4;
-    extern __shared__ __attribute__((aligned(16))) char lds[];
-    const int b = blockIdx.z, h = blockIdx.y, len = stream_len(p, lens, b);
+    extern __shared__ __attribute__((aligned(1024))) char lds[];  // whole rows of any tile: see kfrag()
+    const int b = blockIdx.z, h = blockIdx.y, len = uniform(stream_len(p, lens, b));
     const int lane = lane_id(), wv = wave_id(), half = lane >> 5, col = lane & 31;
     const int s_block = blockIdx.x * (4 * 32 * NB), s0 = s_block + wv * 32 * NB;
     if (s_block >= len) return;
@@ -635,10 +721,10 @@ attention_weights_kernel(AttnPlan p, FastDiv by_group, const E *__restrict__ q, 
     auto request = [&](int r0, char *to) {
 #pragma unroll
         for (int j = 0; j < REQ; ++j) {
-            const int rr = (wv * REQ + j) * RPI + lane / CPR, r = r0 + rr, e = ((lane % CPR) ^ (rr & 7)) * N;
+            const int rr = (wv * REQ + j) * RPI + lane / CPR, r = r0 + rr, e = ((lane % CPR) ^ key_swizzle<E, DP>(rr)) * N;
             const int tok = int(by_group.quot(uint32_t(min(r, rows - 1))));
             const E *src = r < rows && e < p.dim ? q + int64_t(first + tok) * p.qt + (h * p.group + r - tok * p.group) * p.qh + e : zero;
-            __builtin_amdgcn_global_load_lds((const DC_GLOBAL(void) *)src, (DC_LDS(void) *)(to + (wv * REQ + j) * 1024), 16, 0, 0);
+            fetch(src, lds_place(to) + (wv * REQ + j) * 1024);
         }
     };
     const float scale = p.flip != 0 ? -p.scale : p.scale;
@@ -663,9 +749,9 @@ attention_weights_kernel(AttnPlan p, FastDiv by_group, const E *__restrict__ q, 
                 limit[i] = visible(len, count, tok, p.causal_block);
             }
         }
-        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this tile has arrived
+        arrived();
         __syncthreads();
-        const char *qt = lds + stage * TILE;
+        const uint32_t qt = lds_place(lds) + stage * TILE;
         if (r0 + BM < rows) request(r0 + BM, lds + (stage ^ 1) * TILE);
         const bool whole = s0 + 32 * NB <= visible(len, count, int(by_group.quot(uint32_t(r0))), p.causal_block);
 #pragma unroll
@@ -677,7 +763,7 @@ attention_weights_kernel(AttnPlan p, FastDiv by_group, const E *__restrict__ q, 
                 for (int r = 0; r < 16; ++r) s[i][r] = 0.f;
 #pragma unroll
             for (int t = 0; t < STEPS; ++t) {
-                const chunk qf = *reinterpret_cast<const chunk *>(qt + (32 * j + col) * ROW + (((2 * t + half) ^ (col & 7)) << 4));
+                const chunk qf = lds_read<chunk>(((qt + col * ROW + ((half ^ key_swizzle<E, DP>(col)) << 4)) ^ (t << 5)) + 32 * j * ROW);
 #pragma unroll
                 for (int i = 0; i < NB; ++i) s[i] = Chunk<E>::mma(k[i][t], qf, s[i]);
             }
@@ -822,7 +908,9 @@ hipError_t weights_go(const dc_attention_args &a, const AttnPlan &p, const AttnG
 
 template <typename E, int DP>
 hipError_t attention_dp(const dc_attention_args &a, const AttnPlan &p, const AttnGrid &g, bool few, float *lse, hipStream_t s) {
-    const bool aligned = p.pool.page_size % (few ? Shape<E, DP, true>::BN : Shape<E, DP, false>::BN) == 0;
+    // tiles inside a page take their rows from one address; a page of 4 GiB has no 32-bit place in the pool
+    const bool aligned = p.pool.page_size % (few ? Shape<E, DP, true>::BN : Shape<E, DP, false>::BN) == 0 &&
+                         int64_t(p.kv_heads) * p.pool.page_size * p.dim * int(sizeof(E)) < (int64_t(1) << 32);
     hipError_t e = few ? aligned ? attention_go<E, DP, true, true>(a, p, g, lse, s) : attention_go<E, DP, true, false>(a, p, g, lse, s)
                        : aligned ? attention_go<E, DP, false, true>(a, p, g, lse, s) : attention_go<E, DP, false, false>(a, p, g, lse, s);
     if (e == hipSuccess && g.splits > 1) {
