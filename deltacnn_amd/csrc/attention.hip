@@ -95,7 +95,8 @@ struct AttnGrid {
     int32_t splits;         // pieces of the slot axis
     int32_t split_keys;     // slots of a piece
     int32_t unit;           // consecutive row blocks that run on one XCD
-    FastDiv by_group, by_unit, by_flat, by_blocks, by_kv;
+    int32_t pairs;          // heads x pieces
+    FastDiv by_group, by_unit, by_pairs, by_blocks, by_kv;
     float *part;            // [splits][T * q_heads][dim] sums over a piece, [splits][T * q_heads][2] their maximum and normaliser behind
 };
 
@@ -142,16 +143,20 @@ __device__ __forceinline__ bool find_block(const int32_t *starts, const AttnPlan
 }
 
 // Workgroups go to the 8 XCDs in turn, each with an L2 of its own: units of consecutive row blocks, which
-// read the same keys and values, stay on one.
+// read the same keys and values, stay on one.  With a causal mask a stream's row blocks are counted from
+// its end and every head's come before the next unit's, so that the longest start first (a 12240-token
+// clip: the longest of 1532 workgroups takes half of the time that all of them need); every other
+// round of units goes backwards over the XCDs, which evens out their sums.
 __device__ __forceinline__ bool find_work(const int32_t *starts, const AttnPlan &p, const AttnGrid &g, Work &w) {
     const int x = blockIdx.x & 7, j = blockIdx.x >> 3;
-    const int u = int(g.by_unit.quot(j));
-    const int o = (x + 8 * u) * g.unit + (j - u * g.unit);
-    const int pair = int(g.by_flat.quot(o));
-    if (pair >= p.kv_heads * g.splits) return false;
+    const int round = int(g.by_unit.quot(j));
+    const int u = (round & 1 ? 7 - x : x) + 8 * round;
+    const int group = int(g.by_pairs.quot(u)), pair = u - group * g.pairs;
+    const int f = group * g.unit + (j - round * g.unit);
+    if (f >= g.flat) return false;
     w.split = int(g.by_kv.quot(pair));
     w.h = pair - w.split * p.kv_heads;
-    if (!find_block(starts, p, g, o - pair * g.flat, w)) return false;
+    if (!find_block(starts, p, g, f, w)) return false;
     if (p.causal_block != 0) {  // the longest rows first
         const int blocks = int((int64_t(w.count) * p.group + g.block_rows - 1) / g.block_rows);
         w.rb = blocks - 1 - w.rb;
@@ -854,7 +859,8 @@ AttnGrid plan_grid(const AttnPlan &p, bool ragged, bool few, int bm) {
     while (g.unit < 16 && g.unit * 2 <= g.flat && total >= 8 * 2 * g.unit * 2) g.unit *= 2;
     g.by_group = FastDiv(uint32_t(p.group));
     g.by_unit = FastDiv(uint32_t(g.unit));
-    g.by_flat = FastDiv(uint32_t(g.flat));
+    g.pairs = p.kv_heads * g.splits;
+    g.by_pairs = FastDiv(uint32_t(g.pairs));
     g.by_blocks = FastDiv(uint32_t(max(1, g.stream_blocks)));
     g.by_kv = FastDiv(uint32_t(p.kv_heads));
     return g;
@@ -883,8 +889,7 @@ hipError_t attention_go(const dc_attention_args &a, const AttnPlan &p, const Att
     static thread_local uint64_t raised = 0;
     const hipError_t err = raise_lds((const void *)kernel, S::LDS, raised);
     if (err != hipSuccess) return err;
-    const int64_t total = int64_t(g.flat) * p.kv_heads * g.splits;
-    const int64_t blocks = ceil_div64(total, 8 * g.unit) * 8 * g.unit;
+    const int64_t blocks = ceil_div64(ceil_div64(g.flat, g.unit) * g.pairs, 8) * 8 * g.unit;
     if (blocks > (1 << 30)) return hipErrorInvalidConfiguration;
     note_kernel("attention_mfma_kernel");
     kernel<<<dim3(uint32_t(blocks)), S::NW * WAVE, S::LDS, s>>>(p, g, (const E *)a.q, (E *)a.out, lse, (const E *)a.keys, (const E *)a.values,
