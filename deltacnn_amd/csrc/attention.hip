@@ -100,6 +100,11 @@ struct AttnGrid {
     float *part;            // [splits][T * q_heads][dim] sums over a piece, [splits][T * q_heads][2] their maximum and normaliser behind
 };
 
+template <bool B>
+struct Flag {
+    static constexpr bool value = B;
+};
+
 struct Work {
     int b, h, split, rb, first, count;
 };
@@ -184,6 +189,11 @@ __device__ __forceinline__ void fetch(const void *from, uint32_t to) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "memory");
 }
 __device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// .. all but the newest N requests
+template <int N>
+__device__ __forceinline__ void arrived_but() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
 
 // Where 16-byte chunk c of row r of a tile lies: at place c ^ swizzle(r) of the row.  The LDS serves 256 bytes a
 // cycle from 64 banks: of keys 16 rows' chunks side by side, of values 32 lanes of the transposing read,
@@ -235,7 +245,8 @@ struct TileLoader {
     }
     // The page of the next tile, a step ahead of its request.
     __device__ __forceinline__ void look() {
-        if constexpr (ALIGNED) page = table[index];
+        // (nothing writes the table meanwhile: a scalar load, which the counted waits do not see)
+        if constexpr (ALIGNED) page = *(const __attribute__((address_space(4))) int32_t *)(table + index);
     }
     __device__ __forceinline__ void advance(int by) {
         if constexpr (ALIGNED) {
@@ -243,42 +254,53 @@ struct TileLoader {
             while (inside >= page_size) inside -= page_size, ++index;
         }
     }
-    // Slots [k0, end) of the tile into LDS places kt, vt (of this wavefront's first row)
-    __device__ __forceinline__ void request(const AttnPlan &p, int loader, int k0, int end, uint32_t kt, uint32_t vt) {
+    // Where a tile's rows are: ALIGNED its first byte from the head's first page and the bytes in use, else a row of each request (or -1)
+    struct Place {
+        uint64_t at;
+        uint32_t bytes;
+        int64_t row[ALIGNED ? 1 : REQ];
+    };
+    // Slots [k0, end); behind `end` nothing
+    __device__ __forceinline__ Place find(const AttnPlan &p, int loader, int k0, int end) {
+        Place x;
         if constexpr (ALIGNED) {
             const uint32_t pg = uint32_t(uniform(page));
-            const bool ok = pg < uint32_t(num_pages);
-            bad = bad || !ok;
-            const uint64_t at = ok ? uint64_t(pg) * page_bytes + uint32_t(inside) * row_bytes : 0;
-            const uint64_t ka = uint64_t(uintptr_t(keys)) + at, va = uint64_t(uintptr_t(values)) + at;
-            u32x4_t rk, rv;
-            rk[0] = uniform(uint32_t(ka)), rk[1] = uniform(uint32_t(ka >> 32) & 0xffffu);
-            rv[0] = uniform(uint32_t(va)), rv[1] = uniform(uint32_t(va >> 32) & 0xffffu);
-            rk[2] = rv[2] = uniform(ok ? min(BN, end - k0) * row_bytes : 0u), rk[3] = rv[3] = 0x00027000u;
+            const bool in = k0 < end, ok = in && pg < uint32_t(num_pages);
+            bad = bad || (in && !ok);
+            x.at = ok ? uint64_t(pg) * page_bytes + uint32_t(inside) * row_bytes : 0;
+            x.bytes = uniform(ok ? min(BN, end - k0) * row_bytes : 0u);
+        } else {
+            const int row0 = loader * REQ * RPI + lane_id() / CPR;
 #pragma unroll
-            for (int j = 0; j < REQ; ++j) fetch_bounded(rk, koffset[j], kt + j * 1024);
+            for (int j = 0; j < REQ; ++j) {
+                const int s = k0 + row0 + j * RPI;
+                x.row[j] = -1;
+                if (s < end) {
+                    x.row[j] = slot_row(p.pool, table, s, p.kv_heads, h);
+                    bad = bad || x.row[j] < 0;
+                }
+            }
+        }
+        return x;
+    }
+    // .. into LDS from place `to` (of this wavefront's first row)
+    template <bool VALUES>
+    __device__ __forceinline__ void request(const Place &x, int loader, uint32_t to) {
+        const E *from = VALUES ? values : keys;
+        if constexpr (ALIGNED) {
+            const uint64_t a = uint64_t(uintptr_t(from)) + x.at;
+            u32x4_t r;
+            r[0] = uniform(uint32_t(a)), r[1] = uniform(uint32_t(a >> 32) & 0xffffu), r[2] = x.bytes, r[3] = 0x00027000u;
 #pragma unroll
-            for (int j = 0; j < REQ; ++j) fetch_bounded(rv, voffset[j], vt + j * 1024);
+            for (int j = 0; j < REQ; ++j) fetch_bounded(r, VALUES ? voffset[j] : koffset[j], to + j * 1024);
         } else {
             const E *zero = reinterpret_cast<const E *>(&zero_chunk);
-            const E *kp[REQ], *vp[REQ];
             const int c = lane_id() % CPR, row0 = loader * REQ * RPI + lane_id() / CPR;
 #pragma unroll
             for (int j = 0; j < REQ; ++j) {
-                const int row = row0 + j * RPI, s = k0 + row;
-                int64_t at = -1;
-                if (s < end) {
-                    at = slot_row(p.pool, table, s, p.kv_heads, h);
-                    bad = bad || at < 0;
-                }
-                const int ck = c ^ key_swizzle<E, DP>(row), cv = c ^ value_swizzle<E, DP>(row);
-                kp[j] = at >= 0 && ck * N < dim ? keys + at * dim + ck * N : zero;
-                vp[j] = at >= 0 && cv * N < dim ? values + at * dim + cv * N : zero;
+                const int row = row0 + j * RPI, e = (c ^ (VALUES ? value_swizzle<E, DP>(row) : key_swizzle<E, DP>(row))) * N;
+                fetch(x.row[j] >= 0 && e < dim ? from + x.row[j] * dim + e : zero, to + j * 1024);
             }
-#pragma unroll
-            for (int j = 0; j < REQ; ++j) fetch(kp[j], kt + j * 1024);
-#pragma unroll
-            for (int j = 0; j < REQ; ++j) fetch(vp[j], vt + j * 1024);
         }
     }
 };
@@ -376,6 +398,103 @@ struct RowState {
         }
     }
 
+    // The products with the values of a block, requested and rounded a step before.
+    template <bool MASK>
+    __device__ __forceinline__ void add_values(chunk (&vf)[2][DB], const chunk (&pr)[2], uint32_t vt, int k0, int limit) {
+        bool odd = false;
+        if constexpr (MASK) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) odd = odd || odd_value(E(vf[t][d][i]));
+            odd = ballot(odd) != 0;
+            if (odd) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int d = 0; d < DB; ++d)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (odd_value(E(vf[t][d][i]))) vf[t][d][i] = E(0.f);
+                add_odd(vt, k0, limit);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int d = 0; d < DB; ++d) o[d] = Chunk<E>::mma(vf[t][d], pr[t], o[d]);
+    }
+
+    // One turn of the pipeline: the scores s of block i become probabilities while the matrix cores work on
+    // the scores of block i + 1 and the values of block i - 1.  The wavefront issues products and vector
+    // instructions side by side this way: one after the other, as the two wavefronts of a SIMD fall into
+    // step on the matrix cores, the kernel took their sum.
+    //   kt: keys of i + 1;  vt_old, k_old: values and first slot of i - 1;  vt: values of i, which starts at k0
+    template <bool MASK>
+    __device__ __forceinline__ void turn(float16_t &s, float16_t &next, chunk (&vf)[2][DB], chunk (&pr)[2], uint32_t kt, uint32_t vt_old,
+                                         uint32_t vt, float scale, int k_old, int k0, int limit) {
+        const int half = lane_id() >> 5;
+        chunk kf[STEPS];
+#pragma unroll
+        for (int t = 0; t < STEPS; ++t) kf[t] = kfrag(kt, 0, t);
+        add_values<MASK>(vf, pr, vt_old, k_old, limit);
+        if constexpr (MASK) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (k0 + 8 * (r / 4) + 4 * half + r % 4 >= limit) s[r] = -INFINITY;
+        }
+        float top = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+        top = max_halves(top) * scale;
+        follow(top);
+        const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int d = 0; d < DB; ++d) vf[t][d] = vfrag(vt, t, d);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) next[r] = 0.f;
+#pragma unroll
+        for (int t = 0; t < STEPS; ++t) next = Chunk<E>::mma(kf[t], q[t], next);
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], scale, -ref));
+            part[r & 3] += s[r];
+        }
+        l += (part[0] + part[1]) + (part[2] + part[3]);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            u32x4_t u;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) u[i] = pack2(s[8 * t + 2 * i], s[8 * t + 2 * i + 1], E());
+            pr[t] = __builtin_bit_cast(chunk, u);
+        }
+#pragma unroll
+        for (int t = 0; t < STEPS; ++t) {  // a product, then vector instructions in its shadow
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 4 * DB / STEPS, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 64 / STEPS, 0);
+        }
+    }
+
+    // The reference of the exponentials follows the maximum only when that outgrows it by 2^8: any reference
+    // gives the same quotient, and a step without a new one leaves the sums alone.
+    __device__ __forceinline__ void follow(float top) {
+        if (ballot(top > m + 8.f) != 0) {
+            const float m2 = fmaxf(m, top), fade = m2 == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - m2);
+            m = m2;
+            l *= fade;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[d][r] *= fade;
+        }
+    }
+
     // One tile: slots [k0, k0 + BN); this lane's row sees slots below `limit` (MASK: some row does not see some of the tile's)
     template <bool MASK>
     __device__ __forceinline__ void step(uint32_t kt, uint32_t vt, float scale, int k0, int limit) {
@@ -418,17 +537,7 @@ struct RowState {
 #pragma unroll
             for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
         top = max_halves(top) * scale;
-        // The reference of the exponentials follows the maximum only when that outgrows it by 2^8: any
-        // reference gives the same quotient, and a step without a new one leaves the sums alone.
-        if (ballot(top > m + 8.f) != 0) {
-            const float m2 = fmaxf(m, top), fade = m2 == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - m2);
-            m = m2;
-            l *= fade;
-#pragma unroll
-            for (int d = 0; d < DB; ++d)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) o[d][r] *= fade;
-        }
+        follow(top);
         const float ref = m == -INFINITY ? 0.f : m;
         float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -507,20 +616,24 @@ struct RowState {
     }
 };
 
-// Slots of a tile and wavefronts of a workgroup (KEYS: every wavefront has two stages of tiles of its own).
+// How a workgroup goes about its slots.
+//   PIPE (16-bit types, many rows): 4 wavefronts own different rows and share blocks of 32 slots, rings of 3
+//   blocks of keys and 4 of values; see pipeline().
+//   KEYS (few rows): the wavefronts own the same rows and blocks of 32 slots each in turn, two stages of
+//   their own, without a barrier between them, and join their sums at the end.
+//   else (fp32, whose products take sixteen times as long as anything beside them): 4 wavefronts own
+//   different rows and share two stages of 32 slots.
 template <typename E, int DP, bool KEYS>
 struct Shape {
-    static constexpr int ROW = DP * int(sizeof(E)), BN = KEYS || sizeof(E) == 4 ? 32 : 64, TILE = BN * ROW;
+    static constexpr int ROW = DP * int(sizeof(E)), BN = 32, TILE = BN * ROW;
+    static constexpr bool PIPE = !KEYS && sizeof(E) == 2;
     static constexpr int NW = !KEYS ? 4 : ROW <= 256 ? 4 : ROW <= 512 ? 2 : 1;
-    static constexpr int TILES = 4 * TILE * (KEYS ? NW : 1), JOIN = KEYS ? NW * 32 * (DP + 6) * 4 : 0;
+    static constexpr int TILES = PIPE ? 7 * TILE : 4 * TILE * (KEYS ? NW : 1), JOIN = KEYS ? NW * 32 * (DP + 6) * 4 : 0;
     static constexpr int LDS = TILES > JOIN ? TILES : JOIN;
-    static constexpr int GROUPS = LDS <= 80 << 10 && ROW <= 256 ? 2 : 1;  // workgroups a compute unit is to hold
+    static constexpr int GROUPS = LDS <= 79 << 10 && ROW <= 256 ? 2 : 1;  // workgroups a compute unit is to hold
 };
 
 // Attention on the matrix cores.  A wavefront owns 32 rows.
-//   KEYS == false: the workgroup's 4 wavefronts own different rows and share tiles of 64 slots (fp32: 32).
-//   KEYS == true (few rows): they own the same rows and tiles of 32 slots each in turn, without a
-//   barrier between them, and join their sums at the end.
 template <typename E, int DP, bool KEYS, bool ALIGNED>
 __global__ void __launch_bounds__((WAVE * Shape<E, DP, KEYS>::NW), (Shape<E, DP, KEYS>::GROUPS))
 attention_mfma_kernel(AttnPlan p, AttnGrid g, const E *__restrict__ q, E *__restrict__ out, float *__restrict__ lse,
@@ -566,33 +679,106 @@ attention_mfma_kernel(AttnPlan p, AttnGrid g, const E *__restrict__ q, E *__rest
     const int loader = KEYS ? 0 : wv, first = kb + (KEYS ? wv * BN : 0), stride = KEYS ? NW * BN : BN;
     load.init(p, table, keys, values, w.h, loader, first);
     const uint32_t place = lds_place(lds) + (KEYS ? wv * 4 * TILE : 0), mine = place + loader * Loader::REQ * 1024;  // [stage][K, V]
-    if (first < ke) {
-        load.look();
-        load.request(p, loader, first, ke, mine, mine + TILE);
-        load.advance(stride);
-        if (first + stride < ke) load.look();
-    }
-    uint32_t stage = 0;
-    int k0 = first;
-    // the next tile's requests and the page of the one behind it, once this tile is there
-    auto turn = [&]() {
-        arrived();                             // this tile, of this wavefront's requests
-        if constexpr (!KEYS) __syncthreads();  // .. of everybody's, and the other stage is free
-        if (k0 + stride < ke) {
-            const uint32_t to = mine + (stage ^ 2 * TILE);
-            load.request(p, loader, k0 + stride, ke, to, to + TILE);
-            load.advance(stride);
-            if (k0 + 2 * stride < ke) load.look();
+    if constexpr (S::PIPE) {
+        // Group i of requests, {keys of i + 3, values of i + 2}, goes out in turn i, behind the barrier at which
+        // everybody has left turn i - 1 (and with it the keys of i and the values of i - 2, whose places it
+        // takes); what turn i reads came with group i - 2, so one group stays in flight.  Blocks behind the
+        // last are requested as nothing, which keeps the count.
+        constexpr int FLIGHT = 2 * Loader::REQ;
+        const uint32_t vplace = place + 3 * TILE, vmine = mine + 3 * TILE;
+        typename Loader::Place held;
+        auto next_place = [&](int k0) {
+            const auto x = load.find(p, loader, k0, ke);
+            load.advance(BN);
+            if (k0 + BN < ke) load.look();  // a turn ahead
+            return x;
+        };
+        if (kb < ke) load.look();
+        held = next_place(kb);
+        load.template request<false>(held, loader, mine);
+        for (int i = 1; i < 3; ++i) {
+            const auto x = next_place(kb + i * BN);
+            load.template request<false>(x, loader, mine + i * TILE);
+            load.template request<true>(held, loader, vmine + (i - 1) * TILE);
+            held = x;
         }
-    };
-    // tiles that every row of the workgroup sees as a whole, then the rest
-    for (; k0 + BN <= all; k0 += stride, stage ^= 2 * TILE) {
-        turn();
-        st.template step<false>(place + stage, place + stage + TILE, p.scale, k0, limit);
-    }
-    for (; k0 < ke; k0 += stride, stage ^= 2 * TILE) {
-        turn();
-        if (k0 < wave_end) st.template step<true>(place + stage, place + stage + TILE, p.scale, k0, limit);
+        auto meet = [&]() {  // all but the newest group are there, everybody's
+            arrived_but<FLIGHT>();
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+        };
+        meet();
+        float16_t sa, sb;
+        chunk vf[2][DP / 32], pr[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            pr[t] = __builtin_bit_cast(chunk, make_uint4(0, 0, 0, 0));
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d) vf[t][d] = pr[t];
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sa[r] = 0.f;
+#pragma unroll
+        for (int t = 0; t < RowState<E, DP, BN>::STEPS; ++t) sa = Chunk<E>::mma(st.kfrag(place, 0, t), st.q[t], sa);
+        uint32_t kslot = 0, vslot = 0;  // of block i
+        int k0 = kb;
+        auto turn = [&](auto mask, float16_t &s, float16_t &next) {
+            meet();
+            const uint32_t knext = kslot == 2 * TILE ? 0 : kslot + TILE;
+            const auto x = next_place(k0 + 3 * BN);
+            load.template request<false>(x, loader, mine + kslot);
+            load.template request<true>(held, loader, vmine + ((vslot + 2 * TILE) & 3 * TILE));
+            held = x;
+            st.template turn<decltype(mask)::value>(s, next, vf, pr, place + knext, vplace + ((vslot + 3 * TILE) & 3 * TILE), vplace + vslot,
+                                                    p.scale, k0 - BN, k0, limit);
+            kslot = knext;
+            vslot = (vslot + TILE) & 3 * TILE;
+            k0 += BN;
+        };
+        // blocks that every row of the workgroup sees, two by two so that scores need not be copied, then the rest
+        while (k0 + 2 * BN <= all) {
+            turn(Flag<false>(), sa, sb);
+            turn(Flag<false>(), sb, sa);
+        }
+        while (k0 < ke) {
+            turn(Flag<true>(), sa, sb);
+            sa = sb;
+        }
+        st.template add_values<true>(vf, pr, vplace + ((vslot + 3 * TILE) & 3 * TILE), k0 - BN, limit);
+        arrived();  // nothing may reach this LDS after the workgroup has left it
+    } else {
+        if (first < ke) {
+            load.look();
+            const auto x = load.find(p, loader, first, ke);
+            load.template request<false>(x, loader, mine);
+            load.template request<true>(x, loader, mine + TILE);
+            load.advance(stride);
+            if (first + stride < ke) load.look();
+        }
+        uint32_t stage = 0;
+        int k0 = first;
+        // the next tile's requests and the page of the one behind it, once this tile is there
+        auto turn = [&]() {
+            arrived();                             // this tile, of this wavefront's requests
+            if constexpr (!KEYS) __syncthreads();  // .. of everybody's, and the other stage is free
+            if (k0 + stride < ke) {
+                const uint32_t to = mine + (stage ^ 2 * TILE);
+                const auto x = load.find(p, loader, k0 + stride, ke);
+                load.template request<false>(x, loader, to);
+                load.template request<true>(x, loader, to + TILE);
+                load.advance(stride);
+                if (k0 + 2 * stride < ke) load.look();
+            }
+        };
+        // tiles that every row of the workgroup sees as a whole, then the rest
+        for (; k0 + BN <= all; k0 += stride, stage ^= 2 * TILE) {
+            turn();
+            st.template step<false>(place + stage, place + stage + TILE, p.scale, k0, limit);
+        }
+        for (; k0 < ke; k0 += stride, stage ^= 2 * TILE) {
+            turn();
+            if (k0 < wave_end) st.template step<true>(place + stage, place + stage + TILE, p.scale, k0, limit);
+        }
     }
 
     float l = sum_halves(st.l);
