@@ -66,10 +66,20 @@ struct Chunk<float> {
     }
 };
 
-// Infinity or NaN?
-__device__ __forceinline__ bool odd_value(half_t x) { return (__builtin_bit_cast(uint16_t, x) & 0x7c00u) == 0x7c00u; }
-__device__ __forceinline__ bool odd_value(bf16_t x) { return (__builtin_bit_cast(uint16_t, x) & 0x7f80u) == 0x7f80u; }
-__device__ __forceinline__ bool odd_value(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
+// The sign bit of each infinite or NaN element of a 32-bit word: zero elements of the complemented exponents
+// (an element behind a zero one would have to be 1 to be taken for zero too, and exponents have no bit there).
+template <typename E>
+__device__ __forceinline__ uint32_t odd_bits(uint32_t w) {
+    constexpr uint32_t EXPONENT = sizeof(E) == 4 ? 0x7f800000u : __is_same(E, half_t) ? 0x7c007c00u : 0x7f807f80u;
+    constexpr uint32_t ONES = sizeof(E) == 4 ? 1u : 0x00010001u, SIGNS = sizeof(E) == 4 ? 0x80000000u : 0x80008000u;
+    const uint32_t x = (w & EXPONENT) ^ EXPONENT;
+    return (x - ONES) & ~x & SIGNS;
+}
+template <typename E>
+__device__ __forceinline__ uint32_t without_odd(uint32_t w) {
+    const uint32_t b = odd_bits<E>(w);
+    return w & ~(sizeof(E) == 4 ? 0u - (b >> 31) : (b >> 15) * 0xffffu);
+}
 
 // The larger of the two halves' values, in both.
 __device__ __forceinline__ float max_halves(float x) {
@@ -220,9 +230,12 @@ struct TileLoader {
     const E *keys, *values;  // ALIGNED: from this head's first row of a page
     int dim, h, page_size, num_pages;
     bool bad = false;
-    // ALIGNED: bytes of a lane from the tile's first element; page and place in it of the tile to be requested next
+    // ALIGNED: bytes of a lane from the tile's first element; the tile to be found next: its page (`fresh`: not
+    // looked at yet), the bytes in front of that in the pool, its place inside
     uint32_t koffset[REQ], voffset[REQ], page_bytes, row_bytes;
     int index, inside, page;
+    uint64_t page_at;
+    bool fresh, lost;
 
     __device__ __forceinline__ void init(const AttnPlan &p, const int32_t *table_, const E *k, const E *v, int h_, int loader, int k0) {
         table = table_, dim = p.dim, h = h_, page_size = p.pool.page_size, num_pages = p.pool.num_pages;
@@ -233,7 +246,7 @@ struct TileLoader {
             page_bytes = uint32_t(p.kv_heads) * page_size * row_bytes;
             index = uniform(p.pool.by_page.quot(uint32_t(k0)));
             inside = uniform(k0 - index * page_size);
-            page = 0;
+            page = 0, page_at = 0, fresh = true, lost = false;
             const int c = lane_id() % CPR, row0 = loader * REQ * RPI + lane_id() / CPR;
 #pragma unroll
             for (int j = 0; j < REQ; ++j) {
@@ -246,15 +259,16 @@ struct TileLoader {
     // The page of the next tile, a step ahead of its request.
     __device__ __forceinline__ void look() {
         // (nothing writes the table meanwhile: a scalar load, which the counted waits do not see)
-        if constexpr (ALIGNED) page = *(const __attribute__((address_space(4))) int32_t *)(table + index);
+        if constexpr (ALIGNED)
+            if (fresh) page = *(const __attribute__((address_space(4))) int32_t *)(table + index);
     }
     __device__ __forceinline__ void advance(int by) {
         if constexpr (ALIGNED) {
             inside += by;
-            while (inside >= page_size) inside -= page_size, ++index;
+            while (inside >= page_size) inside -= page_size, ++index, fresh = true;
         }
     }
-    // Where a tile's rows are: ALIGNED its first byte from the head's first page and the bytes in use, else a row of each request (or -1)
+    // Where a tile's rows are: ALIGNED its bytes from the head's first page and how many are in use, else a row of each request (or -1)
     struct Place {
         uint64_t at;
         uint32_t bytes;
@@ -264,11 +278,14 @@ struct TileLoader {
     __device__ __forceinline__ Place find(const AttnPlan &p, int loader, int k0, int end) {
         Place x;
         if constexpr (ALIGNED) {
-            const uint32_t pg = uint32_t(uniform(page));
-            const bool in = k0 < end, ok = in && pg < uint32_t(num_pages);
-            bad = bad || (in && !ok);
-            x.at = ok ? uint64_t(pg) * page_bytes + uint32_t(inside) * row_bytes : 0;
-            x.bytes = uniform(ok ? min(BN, end - k0) * row_bytes : 0u);
+            if (fresh && k0 < end) {
+                lost = uint32_t(page) >= uint32_t(num_pages);
+                bad = bad || lost;
+                page_at = lost ? 0 : uint64_t(uint32_t(page)) * page_bytes;
+                fresh = false;
+            }
+            x.at = page_at + uint32_t(inside) * row_bytes;
+            x.bytes = lost ? 0u : uint32_t(max(min(BN, end - k0), 0)) * row_bytes;
         } else {
             const int row0 = loader * REQ * RPI + lane_id() / CPR;
 #pragma unroll
@@ -290,7 +307,7 @@ struct TileLoader {
         if constexpr (ALIGNED) {
             const uint64_t a = uint64_t(uintptr_t(from)) + x.at;
             u32x4_t r;
-            r[0] = uniform(uint32_t(a)), r[1] = uniform(uint32_t(a >> 32) & 0xffffu), r[2] = x.bytes, r[3] = 0x00027000u;
+            r[0] = uniform(uint32_t(a)), r[1] = uniform(uint32_t(a >> 32)), r[2] = uniform(x.bytes), r[3] = 0x00027000u;  // addresses have 48 bits
 #pragma unroll
             for (int j = 0; j < REQ; ++j) fetch_bounded(r, VALUES ? voffset[j] : koffset[j], to + j * 1024);
         } else {
@@ -356,33 +373,40 @@ struct RowState {
 
     // Slots that some rows see and others do not may hold infinities or NaN, and 0 * inf would carry them
     // over: such elements leave the product and join the rows that see them one by one.
+    static __device__ __forceinline__ uint32_t chunk_odd(chunk v) {
+        const u32x4_t w = __builtin_bit_cast(u32x4_t, v);
+        return odd_bits<E>(w[0]) | odd_bits<E>(w[1]) | odd_bits<E>(w[2]) | odd_bits<E>(w[3]);
+    }
+    static __device__ __forceinline__ chunk chunk_even(chunk v) {
+        u32x4_t w = __builtin_bit_cast(u32x4_t, v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = without_odd<E>(w[i]);
+        return __builtin_bit_cast(chunk, w);
+    }
     __device__ __forceinline__ bool any_odd(uint32_t vt) const {
-        bool odd = false;
+        uint32_t odd = 0;
         if constexpr (sizeof(E) == 2) {
 #pragma unroll
             for (int t = 0; t < BN / 16; ++t)
 #pragma unroll
-                for (int d = 0; d < DB; ++d) {
-                    const chunk v = vfrag(vt, t, d);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) odd = odd || odd_value(E(v[i]));
-                }
+                for (int d = 0; d < DB; ++d) odd |= chunk_odd(vfrag(vt, t, d));
         } else {
 #pragma unroll
             for (int b = 0; b < BLK; ++b)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
 #pragma unroll
-                    for (int d = 0; d < DB; ++d) odd = odd || odd_value(vword(vt, b, r, d));
+                    for (int d = 0; d < DB; ++d) odd |= odd_bits<E>(__float_as_uint(vword(vt, b, r, d)));
         }
-        return ballot(odd) != 0;
+        return ballot(odd != 0) != 0;
     }
     __device__ __forceinline__ void add_odd(uint32_t vt, int k0, int limit) {
         constexpr int N = Chunk<E>::N;
+        typedef typename Chunk<E>::v4 v4;
         const int half = lane_id() >> 5;
 #pragma unroll 1
         for (int k = 0; k < BN; ++k) {
-            if (k0 + k >= limit) continue;
+            const uint32_t seen = k0 + k < limit ? ~0u : 0u;
             const int swz = value_swizzle<E, DP>(k) << 4;
             const uint32_t row = vt + k * ROW;
 #pragma unroll
@@ -390,10 +414,15 @@ struct RowState {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int e = 32 * d + 8 * j + 4 * half;  // four elements side by side in one chunk
-                    const typename Chunk<E>::v4 v = lds_read<typename Chunk<E>::v4>(row + (((e / N) << 4) ^ swz) + (e % N) * int(sizeof(E)));
+                    union {
+                        v4 v;
+                        uint32_t w[sizeof(v4) / 4];
+                    } x;
+                    x.v = lds_read<v4>(row + (((e / N) << 4) ^ swz) + (e % N) * int(sizeof(E)));
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (odd_value(E(v[i]))) o[d][4 * j + i] += float(E(v[i]));
+                    for (int i = 0; i < int(sizeof(v4) / 4); ++i) x.w[i] = (x.w[i] ^ without_odd<E>(x.w[i])) & seen;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[d][4 * j + i] += float(E(x.v[i]));
                 }
         }
     }
@@ -401,23 +430,17 @@ struct RowState {
     // The products with the values of a block, requested and rounded a step before.
     template <bool MASK>
     __device__ __forceinline__ void add_values(chunk (&vf)[2][DB], const chunk (&pr)[2], uint32_t vt, int k0, int limit) {
-        bool odd = false;
         if constexpr (MASK) {
+            uint32_t odd = 0;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int d = 0; d < DB; ++d)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) odd = odd || odd_value(E(vf[t][d][i]));
-            odd = ballot(odd) != 0;
-            if (odd) {
+                for (int d = 0; d < DB; ++d) odd |= chunk_odd(vf[t][d]);
+            if (__builtin_expect(ballot(odd != 0) != 0, 0)) {
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
-                    for (int d = 0; d < DB; ++d)
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            if (odd_value(E(vf[t][d][i]))) vf[t][d][i] = E(0.f);
+                    for (int d = 0; d < DB; ++d) vf[t][d] = chunk_even(vf[t][d]);
                 add_odd(vt, k0, limit);
             }
         }
@@ -472,12 +495,6 @@ struct RowState {
 #pragma unroll
             for (int i = 0; i < 4; ++i) u[i] = pack2(s[8 * t + 2 * i], s[8 * t + 2 * i + 1], E());
             pr[t] = __builtin_bit_cast(chunk, u);
-        }
-#pragma unroll
-        for (int t = 0; t < STEPS; ++t) {  // a product, then vector instructions in its shadow
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, 4 * DB / STEPS, 0);
-            __builtin_amdgcn_sched_group_barrier(0x002, 64 / STEPS, 0);
         }
     }
 
@@ -566,18 +583,14 @@ struct RowState {
                     for (int i = 0; i < 4; ++i) f.u[i] = pack2(s[b][8 * t + 2 * i], s[b][8 * t + 2 * i + 1], E());
                     pr[b][t] = f.v;
                 }
-            if (MASK && odd) {
+            if (MASK && __builtin_expect(odd, 0)) {
 #pragma unroll
                 for (int b = 0; b < BLK; ++b)
 #pragma unroll
                     for (int t = 0; t < 2; ++t)
 #pragma unroll
                         for (int d = 0; d < DB; ++d) {
-                            chunk v = vfrag(vt, 2 * b + t, d);
-#pragma unroll
-                            for (int i = 0; i < 8; ++i)
-                                if (odd_value(E(v[i]))) v[i] = E(0.f);
-                            o[d] = Chunk<E>::mma(v, pr[b][t], o[d]);
+                            o[d] = Chunk<E>::mma(chunk_even(vfrag(vt, 2 * b + t, d)), pr[b][t], o[d]);
                         }
                 add_odd(vt, k0, limit);
                 return;
@@ -593,15 +606,15 @@ struct RowState {
                 __builtin_amdgcn_sched_barrier(0);
             }
         } else {
-            if (MASK && odd) {
+            if (MASK && __builtin_expect(odd, 0)) {
 #pragma unroll
                 for (int b = 0; b < BLK; ++b)
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
 #pragma unroll
                         for (int d = 0; d < DB; ++d) {
-                            const float v = vword(vt, b, r, d);
-                            o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(odd_value(v) ? 0.f : v, s[b][r], o[d], 0, 0, 0);
+                            const float v = __uint_as_float(without_odd<E>(__float_as_uint(vword(vt, b, r, d))));
+                            o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[b][r], o[d], 0, 0, 0);
                         }
                 add_odd(vt, k0, limit);
                 return;
@@ -615,6 +628,22 @@ struct RowState {
         }
     }
 };
+
+struct AttnCall {
+    AttnPlan p;
+    AttnGrid g;
+    const void *q, *keys, *values;
+    void *out;
+    float *lse;
+    const int32_t *lens, *starts;
+};
+
+// The kernel's arguments, loaded anew: what is needed behind a loop alone does not take scalar registers in it.
+__device__ __forceinline__ const AttnCall &call_again() {
+    uint64_t at = uint64_t(__builtin_amdgcn_kernarg_segment_ptr());
+    asm volatile("" : "+s"(at));
+    return *(const AttnCall *)(const __attribute__((address_space(4))) AttnCall *)at;
+}
 
 // How a workgroup goes about its slots.
 //   PIPE (16-bit types, many rows): 4 wavefronts own different rows and share blocks of 32 slots, rings of 3
@@ -636,9 +665,11 @@ struct Shape {
 // Attention on the matrix cores.  A wavefront owns 32 rows.
 template <typename E, int DP, bool KEYS, bool ALIGNED>
 __global__ void __launch_bounds__((WAVE * Shape<E, DP, KEYS>::NW), (Shape<E, DP, KEYS>::GROUPS))
-attention_mfma_kernel(AttnPlan p, AttnGrid g, const E *__restrict__ q, E *__restrict__ out, float *__restrict__ lse,
-                      const E *__restrict__ keys, const E *__restrict__ values, const int32_t *__restrict__ lens,
-                      const int32_t *__restrict__ starts) {
+attention_mfma_kernel(AttnCall call) {
+    const AttnPlan &p = call.p;
+    const AttnGrid &g = call.g;
+    const E *q = static_cast<const E *>(call.q), *keys = static_cast<const E *>(call.keys), *values = static_cast<const E *>(call.values);
+    const int32_t *lens = call.lens, *starts = call.starts;
     typedef Shape<E, DP, KEYS> S;
     typedef typename Chunk<E>::v chunk;
     constexpr int BN = S::BN, TILE = S::TILE, NW = S::NW, N = Chunk<E>::N;
@@ -782,9 +813,14 @@ attention_mfma_kernel(AttnPlan p, AttnGrid g, const E *__restrict__ q, E *__rest
     }
 
     float l = sum_halves(st.l);
+    const AttnCall &again = call_again();
+    const AttnPlan &tp = again.p;
+    const AttnGrid &tg = again.g;
+    E *out = static_cast<E *>(again.out);
+    float *lse = again.lse;
     const bool bad = __syncthreads_or(load.bad) != 0;
-    const int64_t grow = int64_t(w.first + tok) * p.q_heads + head;  // this row among all
-    const int64_t all_rows = int64_t(p.tokens) * p.q_heads;
+    const int64_t grow = int64_t(w.first + tok) * tp.q_heads + head;  // this row among all
+    const int64_t all_rows = int64_t(tp.tokens) * tp.q_heads;
     if constexpr (KEYS) {
         // the four wavefronts' sums meet in LDS: [wavefront][row][DP + 4] and their (m, l)
         constexpr int PITCH = DP + 4;
@@ -798,7 +834,7 @@ attention_mfma_kernel(AttnPlan p, AttnGrid g, const E *__restrict__ q, E *__rest
                     float4_t{st.o[d][4 * j], st.o[d][4 * j + 1], st.o[d][4 * j + 2], st.o[d][4 * j + 3]};
         __syncthreads();
         const int here = min(32, rows - r0);
-        const int vecs = p.dim / 4;
+        const int vecs = tp.dim / 4;
         for (int i = threadIdx.x; i < here * vecs; i += NW * WAVE) {
             const int rr = i / vecs, c = (i - rr * vecs) * 4;
             float mm = -INFINITY;
@@ -815,13 +851,13 @@ attention_mfma_kernel(AttnPlan p, AttnGrid g, const E *__restrict__ q, E *__rest
 #pragma unroll
                 for (int j = 0; j < 4; ++j) o[j] = fmaf(f, v[j], o[j]);
             }
-            const int tk = int(g.by_group.quot(uint32_t(r0 + rr))), hd = w.h * p.group + r0 + rr - tk * p.group;
-            const int64_t gr = int64_t(w.first + tk) * p.q_heads + hd;
+            const int tk = int(tg.by_group.quot(uint32_t(r0 + rr))), hd = w.h * tp.group + r0 + rr - tk * tp.group;
+            const int64_t gr = int64_t(w.first + tk) * tp.q_heads + hd;
             if (bad) ll = NAN;
-            if (g.splits > 1) {
-                *reinterpret_cast<float4_t *>(g.part + (w.split * all_rows + gr) * p.dim + c) = o;
+            if (tg.splits > 1) {
+                *reinterpret_cast<float4_t *>(tg.part + (w.split * all_rows + gr) * tp.dim + c) = o;
                 if (c == 0) {
-                    float *x = g.part + g.splits * all_rows * p.dim + (w.split * all_rows + gr) * 2;
+                    float *x = tg.part + tg.splits * all_rows * tp.dim + (w.split * all_rows + gr) * 2;
                     x[0] = mm, x[1] = ll;
                 }
             } else {
@@ -829,7 +865,7 @@ attention_mfma_kernel(AttnPlan p, AttnGrid g, const E *__restrict__ q, E *__rest
                 Vec<E, 4> v;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v.v[j] = E(o[j] * inv);
-                E *dst = out + int64_t(w.first + tk) * p.ot + hd * p.oh + c;
+                E *dst = out + int64_t(w.first + tk) * tp.ot + hd * tp.oh + c;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) dst[j] = v.v[j];
                 if (c == 0 && lse != nullptr) lse[gr] = ll == 0.f ? -INFINITY : (ref + __builtin_amdgcn_logf(ll)) * 0.693147180559945309f;
@@ -838,28 +874,28 @@ attention_mfma_kernel(AttnPlan p, AttnGrid g, const E *__restrict__ q, E *__rest
     } else {
         if (!real) return;
         if (bad) l = NAN;
-        if (g.splits > 1) {
-            float *dst = g.part + (w.split * all_rows + grow) * p.dim;
+        if (tg.splits > 1) {
+            float *dst = tg.part + (w.split * all_rows + grow) * tp.dim;
 #pragma unroll
             for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (32 * d + 8 * j + 4 * half < p.dim)
+                    if (32 * d + 8 * j + 4 * half < tp.dim)
                         *reinterpret_cast<float4_t *>(dst + 32 * d + 8 * j + 4 * half) =
                             float4_t{st.o[d][4 * j], st.o[d][4 * j + 1], st.o[d][4 * j + 2], st.o[d][4 * j + 3]};
             if (half == 0) {
-                float *x = g.part + g.splits * all_rows * p.dim + (w.split * all_rows + grow) * 2;
+                float *x = tg.part + tg.splits * all_rows * tp.dim + (w.split * all_rows + grow) * 2;
                 x[0] = st.m, x[1] = l;
             }
             return;
         }
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        E *dst = out + int64_t(w.first + tok) * p.ot + head * p.oh;
+        E *dst = out + int64_t(w.first + tok) * tp.ot + head * tp.oh;
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                if (32 * d + 8 * j + 4 * half >= p.dim) continue;
+                if (32 * d + 8 * j + 4 * half >= tp.dim) continue;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) dst[32 * d + 8 * j + 4 * half + i] = E(st.o[d][4 * j + i] * inv);
             }
@@ -1033,8 +1069,8 @@ AttnGrid plan_grid(const AttnPlan &p, bool ragged, bool few, int bm) {
     g.flat = ragged ? int(rows / bm) + p.streams : g.stream_blocks * p.streams;
     const int64_t cap = int64_t(p.pool.max_pages) * p.pool.page_size;
     const int64_t base = int64_t(g.flat) * p.kv_heads;
-    // pieces of the slot axis until about two workgroups a compute unit are there, none below 8 tiles
-    const int64_t want = few ? 512 : 768, least = few ? 256 : 512;
+    // pieces of the slot axis until two workgroups a compute unit are there, none below some tiles
+    const int64_t want = 512, least = few ? 256 : 512;
     int64_t splits = base >= want ? 1 : ceil_div64(want, base);
     int64_t keys = max(least, ceil_div64(ceil_div64(cap, splits), 128) * 128);
     splits = ceil_div64(cap, keys);
@@ -1050,6 +1086,11 @@ AttnGrid plan_grid(const AttnPlan &p, bool ragged, bool few, int bm) {
     g.by_blocks = FastDiv(uint32_t(max(1, g.stream_blocks)));
     g.by_kv = FastDiv(uint32_t(p.kv_heads));
     return g;
+}
+
+// Rows of a workgroup: 32 a wavefront, of which those of KEYS share theirs.
+int block_rows(bool few) {
+    return few ? 32 : 128;
 }
 
 bool few_rows(const AttnPlan &p) { return int64_t(p.tokens) * p.group <= int64_t(32) * p.streams; }
@@ -1078,8 +1119,8 @@ hipError_t attention_go(const dc_attention_args &a, const AttnPlan &p, const Att
     const int64_t blocks = ceil_div64(ceil_div64(g.flat, g.unit) * g.pairs, 8) * 8 * g.unit;
     if (blocks > (1 << 30)) return hipErrorInvalidConfiguration;
     note_kernel("attention_mfma_kernel");
-    kernel<<<dim3(uint32_t(blocks)), S::NW * WAVE, S::LDS, s>>>(p, g, (const E *)a.q, (E *)a.out, lse, (const E *)a.keys, (const E *)a.values,
-                                                               a.lens, a.starts);
+    const AttnCall call = {p, g, a.q, a.keys, a.values, a.out, lse, a.lens, a.starts};
+    kernel<<<dim3(uint32_t(blocks)), S::NW * WAVE, S::LDS, s>>>(call);
     return hipGetLastError();
 }
 
@@ -1133,7 +1174,7 @@ Room room(const dc_attention_args &a) {
     const AttnPlan p = make_plan(a);
     Room r = {0, 0};
     const bool few = few_rows(p);
-    r.part = part_bytes(p, plan_grid(p, a.starts != nullptr, few, few ? 32 : 128));
+    r.part = part_bytes(p, plan_grid(p, a.starts != nullptr, few, block_rows(few)));
     if (a.weights != nullptr && a.lse == nullptr) r.lse = int64_t(a.tokens) * a.q_heads * 4;
     return r;
 }
@@ -1143,7 +1184,7 @@ hipError_t attention_t(const dc_attention_args &a, AttnPlan p, hipStream_t s) {
     const Room r = room(a);
     float *lse = a.lse != nullptr || a.weights == nullptr ? a.lse : (float *)((char *)a.workspace + r.part);
     const bool few = few_rows(p);
-    AttnGrid g = plan_grid(p, a.starts != nullptr, few, few ? 32 : 128);
+    AttnGrid g = plan_grid(p, a.starts != nullptr, few, block_rows(few));
     g.part = (float *)a.workspace;
     // exponentials are powers of two; with a negative scale q changes its signs instead, so that the largest
     // product has the largest score
