@@ -9,7 +9,7 @@ from .hip_kernels import (sparse_conv, sparse_deconv, sparse_pooling, sparse_act
 from .sparse_layers import (DCConv2d, DCConvTranspose2d, DCMaxPooling, DCAdaptiveAveragePooling,
                             DCDensify, DCAdd, DCActivation, DCUpsamplingNearest2d, DCSparsify,
                             DCThreshold, DCBackend, DCModule, DCBatchNorm2d, DCConcatenate,
-                            DCTruncation)
+                            DCTruncation, DCFrameAttention)
 
 __all__ = [
     "sparse_conv", "sparse_deconv", "sparse_pooling", "sparse_activation", "sparsify",
@@ -18,5 +18,5 @@ __all__ = [
     "rotary_frequencies", "rotary", "rotary_append", "paged_attention", "cache_slots",
     "DCConv2d", "DCConvTranspose2d", "DCMaxPooling", "DCAdaptiveAveragePooling", "DCDensify",
     "DCAdd", "DCActivation", "DCUpsamplingNearest2d", "DCSparsify", "DCThreshold", "DCBackend",
-    "DCModule", "DCBatchNorm2d", "DCConcatenate", "DCTruncation",
+    "DCModule", "DCBatchNorm2d", "DCConcatenate", "DCTruncation", "DCFrameAttention",
 ]

@@ -1108,6 +1108,84 @@ class Linear(nn.Linear):
         return F.linear(input, w, self.bias)
 
 
+class DCFrameAttention(DCModule):
+    """Attention of every frame over the last frames of its stream -- a stateful layer like the others,
+    for dense maps (behind a DCDensify or a ``dense_out`` layer); the reference's layers look back one
+    frame.  Every position of a ``[B, C, H, W]`` map is a token; the layer keeps the keys and values of
+    ``frames * H * W`` tokens of each of the B streams.  Once that is used up, the tokens that have
+    received the least attention (``decay`` per frame) give way, separately for each kv head; those of
+    the last ``keep_frames`` frames give way last.  Positions are rotary over (time, row, column).
+
+    Parameters: ``qkv`` and ``proj``, plain linear layers.  Returns a new ``[B, C, H, W]`` tensor in
+    channels_last; no residual.  Inference only.  Nothing depends on the host's count of frames, so a
+    frame behind the first can be captured (FrameGraph, VideoGraph) like the other layers' frames."""
+
+    def __init__(self, channels, heads, kv_heads=None, head_dim=None, frames=64, keep_frames=1, decay=1.0, sections=None,
+                 base=10000.0, page_size=64, bias=True, name=""):
+        super().__init__()
+        self.name = name
+        self.channels, self.heads = channels, heads
+        self.kv_heads = heads if kv_heads is None else kv_heads
+        self.head_dim = channels // heads if head_dim is None else head_dim
+        if sections is None:  # a quarter of the pairs for time, the rest for rows and columns
+            time = self.head_dim // 4 // 2 * 2
+            rest = (self.head_dim - time) // 4 * 2
+            sections = (time, rest, rest)
+        self.sections = tuple(int(n) for n in sections)
+        if len(self.sections) != 3 or heads % self.kv_heads or self.head_dim % 8 or not 0 < sum(self.sections) <= self.head_dim:
+            raise ValueError(f"DCFrameAttention: {heads} heads over {self.kv_heads}, head_dim {self.head_dim}, sections {self.sections}")
+        self.frames, self.keep_frames, self.decay, self.base, self.page_size = frames, keep_frames, decay, base, page_size
+        self.qkv = Linear(channels, (heads + 2 * self.kv_heads) * self.head_dim, bias=bias)
+        self.proj = Linear(heads * self.head_dim, channels, bias=bias)
+        self._state = None
+
+    def _start(self, x):
+        b, _, h, w = x.shape
+        budget = self.frames * h * w
+        per = -(-budget // self.page_size)
+        pages, kv, page, dev = b * per, self.kv_heads, self.page_size, x.device
+        grid = torch.stack(torch.meshgrid(torch.zeros(b, dtype=torch.int32), torch.arange(h, dtype=torch.int32),
+                                          torch.arange(w, dtype=torch.int32), indexing="ij"), -1)
+        return {
+            "key": (tuple(x.shape), x.dtype, x.device), "budget": budget,
+            "keys": self._cache(torch.zeros(pages, kv, page, self.head_dim, dtype=x.dtype, device=dev)),
+            "values": self._cache(torch.zeros(pages, kv, page, self.head_dim, dtype=x.dtype, device=dev)),
+            "weights": self._cache(torch.zeros(pages, kv, page, device=dev)),
+            "stamps": self._cache(torch.zeros(pages, kv, page, dtype=torch.int32, device=dev)),
+            "table": torch.arange(pages, dtype=torch.int32, device=dev).view(b, per),
+            "lens": torch.zeros(b, dtype=torch.int32, device=dev),
+            "positions": grid.reshape(-1, 3).contiguous().to(dev),  # column 0: the frame, counted on the device
+            "keep_from": torch.full((b,), 1 - self.keep_frames, dtype=torch.int32, device=dev),
+            "frequencies": hk.rotary_frequencies(self.sections, self.base, device=dev),
+        }
+
+    def forward(self, input):
+        if not isinstance(input, Tensor):
+            raise TypeError("DCFrameAttention attends over dense maps: put a DCDensify in front of it")
+        b, c, h, w = input.shape
+        if self._state is None or self._state["key"] != (tuple(input.shape), input.dtype, input.device):
+            self._state = self._start(input)
+        s = self._state
+        tokens = b * h * w
+        q_end, k_end = self.heads * self.head_dim, (self.heads + self.kv_heads) * self.head_dim
+        fused = self.qkv(input.permute(0, 2, 3, 1).reshape(tokens, c))
+        q = fused[:, :q_end].view(tokens, self.heads, self.head_dim)
+        k = fused[:, q_end:k_end].view(tokens, self.kv_heads, self.head_dim)
+        v = fused[:, k_end:].view(tokens, self.kv_heads, self.head_dim)
+        slots, new_lens = hk.cache_slots(s["weights"], s["table"], s["lens"], tokens, s["budget"], stamps=s["stamps"],
+                                         keep_from=s["keep_from"])
+        q = hk.rotary_append(q, k, v, s["positions"], s["frequencies"], self.sections, s["keys"], s["values"], s["table"], slots,
+                             weights=s["weights"], stamps=s["stamps"], lens=s["lens"], new_lens=new_lens)
+        out = hk.paged_attention(q, s["keys"], s["values"], s["table"], s["lens"], weights=s["weights"], decay=self.decay)
+        s["positions"][:, 0].add_(1)
+        s["keep_from"].add_(1)
+        return self.proj(out.view(tokens, q_end)).view(b, h, w, c).permute(0, 3, 1, 2)
+
+    def reset(self):
+        super().reset()
+        self._state = None
+
+
 class DCUpsamplingNearest2d(DCModule):
     """Nearest upsampling by an integer factor (sparse_layers.py:1336-1359): an updated pixel
     updates its scale x scale copies."""

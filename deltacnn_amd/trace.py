@@ -38,6 +38,13 @@ m = 4-byte mask word, P pixels, n_x = number of active pixels of mask x):
                      W = n_keep*2*Ch*s + (n_mid-n_keep)*Ch*s + n_out*Cp*s + P*m
                          [+ n_ex*3*Ce*s + (n_out-n_ex)*Ce*s + P*m]
                      flops = 2*9*Ch*n_mid (as tap pairs) + 2*Ch*Cp*n_keep + 2*Cp*Ce*n_out
+  rotary             (T tokens, H heads of D elements, A axes)
+                     R = T*H*D*s + T*A*4                 W = T*H*D*s                      flops = 3*T*H*D
+  rotary_append      (H query and K kv heads) R = T*(H + 2*K)*D*s + T*(A + K)*4   W = T*(H + 2*K)*D*s
+                     [+ T*K*4 each for weights and stamps]                        flops = 3*T*(H + K)*D
+  paged_attention    (n cached slots of all streams, N visible (token, slot) pairs)
+                     R = T*H*D*s + 2*n*K*D*s [+ n*K*4]   W = T*H*D*s [+ n*K*4]    flops = 4*N*H*D
+  cache_slots        R = n*K*4 [+ n*K*4 stamps]          W = T*K*4
 """
 from __future__ import annotations
 
@@ -71,6 +78,9 @@ class Tracer:
                             for i in meta["items"]]
         if op == "concat_conv":
             rec["n_seg"] = [self._count(m) for m in meta["seg_masks"]]
+        if "lens" in meta:  # attention over cached frames: what the streams hold at the call
+            rec["lens"] = meta["lens"].clone()
+            rec["starts"] = None if meta.get("starts") is None else meta["starts"].clone()
         rec["n_in"] = self._count(meta.get("in_mask"))
         rec["n_in_b"] = self._count(meta.get("in_mask_b"))
         if self.count_pairs and op in ("conv", "deconv", "deconv_add", "conv_act", "conv_add", "block"):
@@ -177,6 +187,13 @@ class Tracer:
             one_wave = steps <= 12 and g.out_c <= 32 and g.out_c % 4 == 0
             flags.append(im["kind"] == "conv_act" and not one_wave)
         return flags
+
+    @staticmethod
+    def _visible(counts, lens, block):
+        """(token, slot) pairs of an attention call over all streams."""
+        if block == 0:
+            return sum(c * n for c, n in zip(counts, lens))
+        return sum(min(block, c - i) * max(0, min(n, n - c + i + block)) for c, n in zip(counts, lens) for i in range(0, c, block))
 
     @staticmethod
     def _covered(g, out_mask):
@@ -357,6 +374,30 @@ class Tracer:
                 flops = 2 * g.out_c * sum(n * c for n, c in zip(n_seg, meta["seg_channels"]))
                 shape = f"{'+'.join(str(c) for c in meta['seg_channels'])}->{g.out_c} k1 @{g.in_h}x{g.in_w}"
                 dens = (sum(n_seg) / (P * len(n_seg)), n_out / P)
+            elif op in ("rotary", "rotary_append"):
+                t, hq, kv, d = meta["tokens"], meta["q_heads"], meta["kv_heads"], meta["dim"]
+                rows = t * (hq + 2 * kv) * d * s
+                rd = rows + t * (meta["axes"] + kv) * 4
+                wr = rows + t * kv * 4 * (bool(meta.get("with_weights")) + bool(meta.get("with_stamps")))
+                flops = 3 * t * (hq + kv) * d
+                shape = f"{t} x {hq}+{kv} heads of {d}"
+                dens = (1.0, 1.0)
+            elif op == "paged_attention":
+                t, hq, kv, d = meta["tokens"], meta["q_heads"], meta["kv_heads"], meta["dim"]
+                lens = r["lens"].tolist()
+                starts = [t // len(lens) * b for b in range(len(lens) + 1)] if r["starts"] is None else r["starts"].tolist()
+                pairs = self._visible([starts[b + 1] - starts[b] for b in range(len(lens))], lens, meta["causal_block"])
+                n = sum(lens)
+                weights = n * kv * 4 if meta["with_weights"] else 0
+                rd, wr = t * hq * d * s + 2 * n * kv * d * s + weights, t * hq * d * s + weights
+                flops = 4 * pairs * hq * d
+                shape = f"{t} x {hq}/{kv} heads of {d} over {n}"
+                dens = (1.0, 1.0)
+            elif op == "cache_slots":
+                n = int(r["lens"].sum())
+                rd, wr = n * meta["kv_heads"] * (8 if meta["with_stamps"] else 4), meta["tokens"] * meta["kv_heads"] * 4
+                shape = f"{meta['tokens']} of {n} x {meta['kv_heads']}"
+                dens = (1.0, 1.0)
             elif op in ("pool", "pool_update"):
                 g = meta["g"]
                 p_in, p_out = g.batch * g.in_h * g.in_w, g.batch * g.out_h * g.out_w

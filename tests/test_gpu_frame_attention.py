@@ -362,3 +362,215 @@ def test_cache_slots(lib, kind, shape):
                                   stamps=on(st), keep_from=on(keep))
     n = sum(counts)
     assert torch.equal(got.cpu()[:, :n], want[:, :n]) and torch.equal(got_new.cpu(), new)
+
+
+# ---- the operators together ----
+
+class PlainFrames:
+    """The layer in 64 bits, token by token lists instead of slots: what a stream holds, per kv head."""
+
+    def __init__(self, layer, shape):
+        self.l, self.shape = layer, shape
+        self.kept = [[[] for _ in range(layer.kv_heads)] for _ in range(shape[0])]  # lists by slot: [key, value, weight, stamp]
+        self.t, self.gap = 0, math.inf  # gap: between the last weight that went and the first that stayed
+
+    def frame(self, x):
+        l, (b, c, h, w) = self.l, self.shape
+        n, dim = h * w, l.head_dim
+        fused = x.permute(0, 2, 3, 1).reshape(b * n, c).double() @ l.qkv.weight.double().cpu().T + l.qkv.bias.double().cpu()
+        q, k, v = fused.split([l.heads * dim, l.kv_heads * dim, l.kv_heads * dim], 1)
+        grid = torch.stack(torch.meshgrid(torch.arange(b) * 0 + self.t, torch.arange(h), torch.arange(w), indexing="ij"), -1).reshape(-1, 3)
+        from deltacnn_amd import hip_kernels as hk
+        freq = hk.rotary_frequencies(l.sections, l.base)
+        q = ref.rotary(q.reshape(b * n, l.heads, dim), grid, freq, l.sections, False)[0]
+        k = ref.rotary(k.reshape(b * n, l.kv_heads, dim), grid, freq, l.sections, False)[0]
+        v = v.reshape(b * n, l.kv_heads, dim)
+        out = torch.zeros(b * n, l.heads, dim, dtype=torch.float64)
+        group = l.heads // l.kv_heads
+        for s in range(b):
+            for g in range(l.kv_heads):
+                cells = self.kept[s][g]
+                rows = range(s * n, (s + 1) * n)
+                e = max(0, len(cells) + n - l.frames * n)
+                order = sorted(range(len(cells)), key=lambda i: (cells[i][3] >= self.t - l.keep_frames + 1, cells[i][2], i))
+                freed = sorted(order[:e])
+                if 0 < e < len(order) and (cells[order[e - 1]][3] >= self.t - l.keep_frames + 1) == (cells[order[e]][3] >= self.t - l.keep_frames + 1):
+                    self.gap = min(self.gap, cells[order[e]][2] - cells[order[e - 1]][2])
+                for j, r in enumerate(rows):
+                    cell = [k[r, g], v[r, g], 0.0, self.t]
+                    if j < e:
+                        cells[freed[j]] = cell
+                    else:
+                        cells.append(cell)
+                kk, vv = torch.stack([x[0] for x in cells]), torch.stack([x[1] for x in cells])
+                got = torch.zeros(len(cells), dtype=torch.float64)
+                for r in rows:
+                    for hd in range(g * group, (g + 1) * group):
+                        p = torch.softmax(kk @ q[r, hd] * dim ** -0.5, 0)
+                        out[r, hd] = p @ vv
+                        got += p
+                for i, cell in enumerate(cells):
+                    cell[2] = l.decay * cell[2] + float(got[i])
+        self.t += 1
+        y = out.reshape(b * n, -1) @ l.proj.weight.double().cpu().T + l.proj.bias.double().cpu()
+        return y.view(b, h, w, c).permute(0, 3, 1, 2)
+
+
+def _layer(dtype, frames=3, kv=2):
+    from deltacnn_amd.sparse_layers import DCFrameAttention
+    torch.manual_seed(4)
+    return DCFrameAttention(48, 4, kv_heads=kv, head_dim=24, frames=frames, keep_frames=1, decay=0.5, page_size=16).eval().to(DEV).to(dtype)
+
+
+def test_layer_follows_its_definition(lib):
+    """fp32, two streams, five frames of which three fit: slots, positions, weights and eviction as a whole.
+
+    The layer's numbers are sums of at most 48 (projections) and 60 (slots) terms of magnitude about 1 in
+    fp32 behind two projections: 10 (48 + 60) w relative to outputs below 1; weights that decide an eviction
+    have to differ by more than twice that, or the choice would be the rounding's."""
+    layer = _layer(torch.float32)
+    shape = (2, 48, 4, 5)
+    plain = PlainFrames(layer, shape)
+    gen = torch.Generator().manual_seed(8)
+    with torch.no_grad():
+        for t in range(5):
+            x = torch.randn(shape, generator=gen)
+            want = plain.frame(x)
+            got = layer(x.to(DEV).contiguous(memory_format=torch.channels_last))
+            assert got.is_contiguous(memory_format=torch.channels_last)
+            assert float((got.double().cpu() - want).abs().max()) < 10 * 108 * ref.W, f"frame {t}"
+            s = layer._state
+            assert s["lens"].tolist() == [min(t + 1, 3) * 20] * 2
+            for b in range(2):
+                for h in range(2):
+                    cells = plain.kept[b][h]
+                    stamps = ref.gather(s["stamps"].cpu()[..., None], s["table"].cpu()[b], len(cells), h, 16)[:, 0]
+                    assert stamps.tolist() == [c[3] for c in cells], f"frame {t}: other tokens were kept"
+    assert 20 * 108 * ref.W < plain.gap < math.inf
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("size", [(1, 1), (7, 7), (12, 9)], ids=str)
+def test_layer_replays_from_a_graph(lib, dtype, size):
+    """Frames replayed from a captured graph, eager work of another layer in between, equal eager frames
+    bit for bit; two graphs of two layers do not disturb each other."""
+    from deltacnn_amd.graph import FrameGraph
+    shape = (2, 48) + size
+    gen = torch.Generator().manual_seed(21)
+    video = [torch.randn(shape, generator=gen).to(dtype).to(DEV).contiguous(memory_format=torch.channels_last) for _ in range(8)]
+    eager, first, second = _layer(dtype), _layer(dtype), _layer(dtype)
+    with torch.no_grad():
+        wanted = [eager(x).clone() for x in video]
+        for layer in (first, second):
+            assert torch.equal(layer(video[0]), wanted[0])
+        graphs = [FrameGraph(first, video[0]), FrameGraph(second, video[0])]
+        other = _layer(dtype)
+        for t in range(1, 8):
+            a, b = graphs[0](video[t]).clone(), graphs[1](video[t]).clone()
+            other(video[t])
+            torch.cuda.synchronize()
+            assert torch.equal(a, wanted[t]) and torch.equal(b, wanted[t]), f"frame {t}"
+
+
+def test_layer_starts_anew(lib):
+    layer = _layer(torch.float16)
+    x = torch.randn(1, 48, 3, 3, device=DEV).half().contiguous(memory_format=torch.channels_last)
+    with torch.no_grad():
+        a = layer(x).clone()
+        layer(x)
+        layer.reset()
+        assert torch.equal(layer(x), a)
+        layer(torch.cat([x, x]))                    # another number of streams: another state
+        assert layer._state["lens"].tolist() == [9, 9]
+        with pytest.raises(TypeError):
+            layer((x, None))
+    from deltacnn_amd import _lib
+    with pytest.raises(_lib.DeltaCNNError, match="gradient"):
+        layer(x)
+
+
+def test_layer_under_the_tracer(lib):
+    from deltacnn_amd import hip_kernels as hk
+    from deltacnn_amd.trace import Tracer
+    layer = _layer(torch.float16)
+    x = torch.randn(2, 48, 4, 4, device=DEV).half().contiguous(memory_format=torch.channels_last)
+    tracer = Tracer()
+    with torch.no_grad():
+        layer(x)
+        hk.set_tracer(tracer)
+        try:
+            layer(x)
+        finally:
+            hk.set_tracer(None)
+    rows = {r["call"]: r for r in tracer.finish()}
+    assert {"cache_slots", "rotary_append", "paged_attention"} <= set(rows)
+    assert rows["paged_attention"]["flops"] == 4 * (2 * 16 * 32) * 4 * 24
+    assert rows["rotary_append"]["bytes"] == 2 * 32 * 8 * 24 * 2 + 32 * (3 + 2) * 4 + 32 * 2 * 8
+
+
+def test_operators_on_another_stream(lib):
+    """Operands made on one stream, the operators on another that waits for it."""
+    from deltacnn_amd import hip_kernels as hk
+    gen = torch.Generator().manual_seed(2)
+    keys, values, weights, _, table = (t.to(DEV) for t in make_pool(gen, 1, 4000, 2, 64, 64, torch.float16))
+    q = torch.randn(60, 4, 64, generator=gen).half().to(DEV)
+    lens = torch.tensor([4000], dtype=torch.int32, device=DEV)
+    want, w_want = hk.paged_attention(q, keys, values, table, lens), weights.clone()
+    hk.paged_attention(q, keys, values, table, lens, weights=w_want)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    late = torch.zeros_like(q)
+    w = weights.clone()
+    big = torch.randn(4096, 4096, device=DEV)
+    for _ in range(4):
+        big = big @ big * 1e-2
+    late.copy_(q)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = hk.paged_attention(late, keys, values, table, lens, weights=w)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want) and torch.equal(w, w_want)
+
+
+def test_results_do_not_change_from_run_to_run(lib):
+    from deltacnn_amd import hip_kernels as hk
+    gen = torch.Generator().manual_seed(6)
+    keys, values, weights, stamps, table = (t.to(DEV) for t in make_pool(gen, 2, 9000, 2, 64, 128, torch.bfloat16))
+    lens = torch.tensor([9000, 7777], dtype=torch.int32, device=DEV)
+    for tokens in (2, 2 * 200):
+        q = torch.randn(tokens, 8, 128, generator=gen).bfloat16().to(DEV)
+        seen = []
+        for _ in range(4):
+            w = weights.clone()
+            seen.append((hk.paged_attention(q, keys, values, table, lens, weights=w, decay=0.5), w))
+        assert all(torch.equal(a, seen[0][0]) and torch.equal(b, seen[0][1]) for a, b in seen)
+
+
+@pytest.mark.parametrize("page", [64, 60])
+def test_pool_beyond_32_bit_offsets(lib, page):
+    """The last pages of a pool of more than 2^31 elements: the same results as a small pool's."""
+    from deltacnn_amd import hip_kernels as hk
+    dim, kv, n = 256, 2, 4 * page
+    pages = (1 << 31) // (kv * page * dim) + 40
+    dtype = torch.float16
+    gen = torch.Generator().manual_seed(1)
+    small_k, small_v = (torch.randn(4, kv, page, dim, generator=gen).to(dtype).to(DEV) for _ in range(2))
+    keys = torch.zeros(pages, kv, page, dim, dtype=dtype, device=DEV)
+    values = torch.zeros_like(keys)
+    keys[-4:], values[-4:] = small_k, small_v
+    far = torch.arange(pages - 4, pages, dtype=torch.int32, device=DEV)[None]
+    near = torch.arange(4, dtype=torch.int32, device=DEV)[None]
+    lens = torch.tensor([n], dtype=torch.int32, device=DEV)
+    for tokens in (1, 70):
+        q = torch.randn(tokens, 2, dim, generator=gen).to(dtype).to(DEV)
+        w_far, w_near = torch.zeros(pages, kv, page, device=DEV), torch.zeros(4, kv, page, device=DEV)
+        a = hk.paged_attention(q, keys, values, far, lens, weights=w_far)
+        b = hk.paged_attention(q, small_k, small_v, near, lens, weights=w_near)
+        assert torch.equal(a, b) and torch.equal(w_far[-4:], w_near)
+    # and writing there
+    k = torch.randn(5, kv, dim, generator=gen).to(dtype).to(DEV)
+    pos = torch.arange(5, dtype=torch.int32, device=DEV)[:, None].contiguous()
+    slots = torch.arange(n - 5, n, dtype=torch.int32, device=DEV).expand(kv, 5).contiguous()
+    freq = hk.rotary_frequencies((dim,), device=DEV)
+    hk.rotary_append(k, k, k, pos, freq, (dim,), keys, values, far, slots)
+    assert torch.equal(values[-1, :, page - 5:], k.transpose(0, 1)) and torch.equal(keys[:-4].view(torch.int16).amax(), keys.new_zeros((), dtype=torch.int16))
