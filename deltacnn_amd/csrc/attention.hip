@@ -650,27 +650,28 @@ __device__ __forceinline__ const AttnCall &call_again() {
 //   blocks of keys and 4 of values; see pipeline().
 //   KEYS (few rows): the wavefronts own the same rows and blocks of 32 slots each in turn, two stages of
 //   their own, without a barrier between them, and join their sums at the end.
+//   NARROW: 2 wavefronts, for streams of at most 64 rows.
 //   else (fp32, whose products take sixteen times as long as anything beside them): 4 wavefronts own
 //   different rows and share two stages of 32 slots.
-template <typename E, int DP, bool KEYS>
+template <typename E, int DP, bool KEYS, bool NARROW = false>
 struct Shape {
     static constexpr int ROW = DP * int(sizeof(E)), BN = 32, TILE = BN * ROW;
     static constexpr bool PIPE = !KEYS && sizeof(E) == 2;
-    static constexpr int NW = !KEYS ? 4 : ROW <= 256 ? 4 : ROW <= 512 ? 2 : 1;
+    static constexpr int NW = !KEYS ? NARROW ? 2 : 4 : ROW <= 256 ? 4 : ROW <= 512 ? 2 : 1;
     static constexpr int TILES = PIPE ? 7 * TILE : 4 * TILE * (KEYS ? NW : 1), JOIN = KEYS ? NW * 32 * (DP + 6) * 4 : 0;
     static constexpr int LDS = TILES > JOIN ? TILES : JOIN;
     static constexpr int GROUPS = LDS <= 79 << 10 && ROW <= 256 ? 2 : 1;  // workgroups a compute unit is to hold
 };
 
 // Attention on the matrix cores.  A wavefront owns 32 rows.
-template <typename E, int DP, bool KEYS, bool ALIGNED>
-__global__ void __launch_bounds__((WAVE * Shape<E, DP, KEYS>::NW), (Shape<E, DP, KEYS>::GROUPS))
+template <typename E, int DP, bool KEYS, bool NARROW, bool ALIGNED>
+__global__ void __launch_bounds__((WAVE * Shape<E, DP, KEYS, NARROW>::NW), (Shape<E, DP, KEYS, NARROW>::GROUPS))
 attention_mfma_kernel(AttnCall call) {
     const AttnPlan &p = call.p;
     const AttnGrid &g = call.g;
     const E *q = static_cast<const E *>(call.q), *keys = static_cast<const E *>(call.keys), *values = static_cast<const E *>(call.values);
     const int32_t *lens = call.lens, *starts = call.starts;
-    typedef Shape<E, DP, KEYS> S;
+    typedef Shape<E, DP, KEYS, NARROW> S;
     typedef typename Chunk<E>::v chunk;
     constexpr int BN = S::BN, TILE = S::TILE, NW = S::NW, N = Chunk<E>::N;
     extern __shared__ __attribute__((aligned(1024))) char lds[];  // whole rows of any tile: see kfrag()
@@ -1042,21 +1043,60 @@ attention_join_kernel(AttnPlan p, AttnGrid g, T *__restrict__ out, float *__rest
     const int n = visible(stream_len(p, lens, b), count, t - first, p.causal_block);
     const int pieces = min(g.splits, max(1, (n + g.split_keys - 1) / g.split_keys));
     const float *ml = g.part + g.splits * all_rows * p.dim;
-    float top = -INFINITY;
-    for (int s = 0; s < pieces; ++s) top = fmaxf(top, ml[(s * all_rows + row) * 2]);
-    const float ref = top == -INFINITY ? 0.f : top;
-    float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < pieces; ++s) {
-        const float f = __builtin_amdgcn_exp2f(ml[(s * all_rows + row) * 2] - ref);
-        l = fmaf(f, ml[(s * all_rows + row) * 2 + 1], l);
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-            if (c * WAVE + lane < p.dim) o[c] = fmaf(f, g.part[(s * all_rows + row) * p.dim + c * WAVE + lane], o[c]);
+    // a lane per piece: their maxima and sums in one request
+    float top = -INFINITY, m_here = -INFINITY, l_here = 0.f;
+    for (int s = lane; s < pieces; s += WAVE) top = fmaxf(top, ml[(s * all_rows + row) * 2]);
+    if (lane < pieces) {
+        const float2 x = *reinterpret_cast<const float2 *>(ml + (lane * all_rows + row) * 2);
+        m_here = x.x, l_here = x.y;
     }
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, WAVE));
+    const float ref = top == -INFINITY ? 0.f : top;
+    const int vecs = p.dim / 4, c = lane % 16 * 4;  // 16 lanes hold 64 elements of a piece's row, 4 pieces at a time
+    float l = 0.f;
+    float4_t o[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] = float4_t{0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < pieces; s0 += WAVE) {
+        if (s0 > 0) {
+            const int s = s0 + lane;
+            m_here = -INFINITY, l_here = 0.f;
+            if (s < pieces) m_here = ml[(s * all_rows + row) * 2], l_here = ml[(s * all_rows + row) * 2 + 1];
+        }
+        const float f_here = s0 + lane < pieces ? __builtin_amdgcn_exp2f(m_here - ref) : 0.f;
+        l = fmaf(f_here, l_here, l);
+        const int n4 = min(WAVE, pieces - s0);
+#pragma unroll 2
+        for (int s = lane / 16; s < (n4 + 3) / 4 * 4; s += 4) {
+            const float f = __shfl(f_here, s, WAVE);
+            if (s >= n4) continue;
+            const float *src = g.part + ((s0 + s) * all_rows + row) * p.dim;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (k * 16 + lane % 16 < vecs) {
+                    const float4_t v = *reinterpret_cast<const float4_t *>(src + k * 64 + c);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[k][i] = fmaf(f, v[i], o[k][i]);
+                }
+        }
+    }
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) l += __shfl_xor(l, d, WAVE);
     const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-        if (c * WAVE + lane < p.dim) out[t * p.ot + head * p.oh + c * WAVE + lane] = T(o[c] * inv);
+    for (int k = 0; k < 4; ++k) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            o[k][i] += __shfl_xor(o[k][i], 16, WAVE);
+            o[k][i] += __shfl_xor(o[k][i], 32, WAVE);
+        }
+        if (lane < 16 && k * 16 + lane < vecs) {
+            T *dst = out + t * p.ot + head * p.oh + k * 64 + c;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dst[i] = T(o[k][i] * inv);
+        }
+    }
     if (lane == 0 && lse != nullptr) lse[row] = l == 0.f ? -INFINITY : (ref + __builtin_amdgcn_logf(l)) * 0.693147180559945309f;
 }
 
@@ -1069,8 +1109,8 @@ AttnGrid plan_grid(const AttnPlan &p, bool ragged, bool few, int bm) {
     g.flat = ragged ? int(rows / bm) + p.streams : g.stream_blocks * p.streams;
     const int64_t cap = int64_t(p.pool.max_pages) * p.pool.page_size;
     const int64_t base = int64_t(g.flat) * p.kv_heads;
-    // pieces of the slot axis until two workgroups a compute unit are there, none below some tiles
-    const int64_t want = 512, least = few ? 256 : 512;
+    // pieces of the slot axis until two workgroups a compute unit are there, none below 128 slots
+    const int64_t want = 512, least = 128;
     int64_t splits = base >= want ? 1 : ceil_div64(want, base);
     int64_t keys = max(least, ceil_div64(ceil_div64(cap, splits), 128) * 128);
     splits = ceil_div64(cap, keys);
@@ -1088,12 +1128,10 @@ AttnGrid plan_grid(const AttnPlan &p, bool ragged, bool few, int bm) {
     return g;
 }
 
-// Rows of a workgroup: 32 a wavefront, of which those of KEYS share theirs.
-int block_rows(bool few) {
-    return few ? 32 : 128;
-}
-
+// Rows of a workgroup by those of a stream (of all streams on average): 32 a wavefront, which share theirs
+// where there are no more.
 bool few_rows(const AttnPlan &p) { return int64_t(p.tokens) * p.group <= int64_t(32) * p.streams; }
+int block_rows(const AttnPlan &p) { return few_rows(p) ? 32 : int64_t(p.tokens) * p.group <= int64_t(64) * p.streams ? 64 : 128; }
 
 int64_t part_bytes(const AttnPlan &p, const AttnGrid &g) {
     return g.splits > 1 ? int64_t(g.splits) * p.tokens * p.q_heads * (p.dim + 2) * 4 : 0;
@@ -1109,10 +1147,10 @@ hipError_t raise_lds(const void *kernel, int bytes, uint64_t &raised) {
     return err;
 }
 
-template <typename E, int DP, bool KEYS, bool ALIGNED>
+template <typename E, int DP, bool KEYS, bool NARROW, bool ALIGNED>
 hipError_t attention_go(const dc_attention_args &a, const AttnPlan &p, const AttnGrid &g, float *lse, hipStream_t s) {
-    typedef Shape<E, DP, KEYS> S;
-    auto kernel = attention_mfma_kernel<E, DP, KEYS, ALIGNED>;
+    typedef Shape<E, DP, KEYS, NARROW> S;
+    auto kernel = attention_mfma_kernel<E, DP, KEYS, NARROW, ALIGNED>;
     static thread_local uint64_t raised = 0;
     const hipError_t err = raise_lds((const void *)kernel, S::LDS, raised);
     if (err != hipSuccess) return err;
@@ -1143,8 +1181,11 @@ hipError_t attention_dp(const dc_attention_args &a, const AttnPlan &p, const Att
     // tiles inside a page take their rows from one address; a page of 4 GiB has no 32-bit place in the pool
     const bool aligned = p.pool.page_size % (few ? Shape<E, DP, true>::BN : Shape<E, DP, false>::BN) == 0 &&
                          int64_t(p.kv_heads) * p.pool.page_size * p.dim * int(sizeof(E)) < (int64_t(1) << 32);
-    hipError_t e = few ? aligned ? attention_go<E, DP, true, true>(a, p, g, lse, s) : attention_go<E, DP, true, false>(a, p, g, lse, s)
-                       : aligned ? attention_go<E, DP, false, true>(a, p, g, lse, s) : attention_go<E, DP, false, false>(a, p, g, lse, s);
+    const bool narrow = g.block_rows == 64;
+    hipError_t e;
+    if (few) e = aligned ? attention_go<E, DP, true, false, true>(a, p, g, lse, s) : attention_go<E, DP, true, false, false>(a, p, g, lse, s);
+    else if (narrow) e = aligned ? attention_go<E, DP, false, true, true>(a, p, g, lse, s) : attention_go<E, DP, false, true, false>(a, p, g, lse, s);
+    else e = aligned ? attention_go<E, DP, false, false, true>(a, p, g, lse, s) : attention_go<E, DP, false, false, false>(a, p, g, lse, s);
     if (e == hipSuccess && g.splits > 1) {
         note_kernel("attention_join_kernel");
         attention_join_kernel<E><<<ceil_div(p.tokens * p.q_heads, 4), 256, 0, s>>>(p, g, (E *)a.out, lse, a.lens, a.starts);
@@ -1174,7 +1215,7 @@ Room room(const dc_attention_args &a) {
     const AttnPlan p = make_plan(a);
     Room r = {0, 0};
     const bool few = few_rows(p);
-    r.part = part_bytes(p, plan_grid(p, a.starts != nullptr, few, block_rows(few)));
+    r.part = part_bytes(p, plan_grid(p, a.starts != nullptr, few, block_rows(p)));
     if (a.weights != nullptr && a.lse == nullptr) r.lse = int64_t(a.tokens) * a.q_heads * 4;
     return r;
 }
@@ -1184,7 +1225,7 @@ hipError_t attention_t(const dc_attention_args &a, AttnPlan p, hipStream_t s) {
     const Room r = room(a);
     float *lse = a.lse != nullptr || a.weights == nullptr ? a.lse : (float *)((char *)a.workspace + r.part);
     const bool few = few_rows(p);
-    AttnGrid g = plan_grid(p, a.starts != nullptr, few, block_rows(few));
+    AttnGrid g = plan_grid(p, a.starts != nullptr, few, block_rows(p));
     g.part = (float *)a.workspace;
     // exponentials are powers of two; with a negative scale q changes its signs instead, so that the largest
     // product has the largest score

@@ -97,11 +97,21 @@ __device__ __forceinline__ uint32_t final_key(uint32_t key, bool prot, bool amon
     return prot == among_protected ? key : prot ? 0xffffffffu : 0u;
 }
 
+// A histogram and the places of its scan for every level, so that a level need not wait for the one before.
 struct SlotsLds {
-    uint32_t hist[2 * SLOT_BINS];
+    uint32_t hist[3 * SLOT_BINS];
+    uint32_t scan[3][SLOT_WAVES], found[3][2];
     uint32_t wave_sum[SLOT_WAVES], wave_sum2[SLOT_WAVES];
-    uint32_t found[2];
 };
+
+// Sum of x[i] over the wavefronts in front of this one (all of them read at once).
+__device__ __forceinline__ uint32_t sum_front(const uint32_t *x) {
+    const int wv = wave_id();
+    uint32_t sum = 0;
+#pragma unroll
+    for (int i = 0; i < SLOT_WAVES; ++i) sum += i < wv ? x[i] : 0;
+    return sum;
+}
 
 __device__ __forceinline__ uint32_t block_sum(SlotsLds &l, uint32_t x) {
 #pragma unroll
@@ -116,33 +126,30 @@ __device__ __forceinline__ uint32_t block_sum(SlotsLds &l, uint32_t x) {
 
 // Bin of rank `want` (1 ..) among the counts h0, h1 of this thread's bins 2 t, 2 t + 1: returns the bin
 // and lowers `want` by what lies in front of it.
-__device__ __forceinline__ uint32_t find_bin(SlotsLds &l, uint32_t h0, uint32_t h1, uint32_t &want) {
+__device__ __forceinline__ uint32_t find_bin(SlotsLds &l, int level, uint32_t h0, uint32_t h1, uint32_t &want) {
     uint32_t sum = h0 + h1;
-    const int lane = lane_id(), wv = wave_id();
+    const int lane = lane_id();
 #pragma unroll
     for (int d = 1; d < WAVE; d <<= 1) {
         const uint32_t o = __shfl_up(sum, d, WAVE);
         if (lane >= d) sum += o;
     }
-    if (lane == WAVE - 1) l.wave_sum[wv] = sum;
+    if (lane == WAVE - 1) l.scan[level][wave_id()] = sum;
     __syncthreads();
-    uint32_t before = sum - h0 - h1;
-    for (int i = 0; i < wv; ++i) before += l.wave_sum[i];
-    if (before < want && want <= before + h0) l.found[0] = 2 * threadIdx.x, l.found[1] = before;
-    if (before + h0 < want && want <= before + h0 + h1) l.found[0] = 2 * threadIdx.x + 1, l.found[1] = before + h0;
+    const uint32_t before = sum - h0 - h1 + sum_front(l.scan[level]);
+    if (before < want && want <= before + h0) l.found[level][0] = 2 * threadIdx.x, l.found[level][1] = before;
+    if (before + h0 < want && want <= before + h0 + h1) l.found[level][0] = 2 * threadIdx.x + 1, l.found[level][1] = before + h0;
     __syncthreads();
-    const uint32_t bin = l.found[0];
-    want -= l.found[1];
-    __syncthreads();
-    return bin;
+    want -= l.found[level][1];
+    return l.found[level][0];
 }
 
 constexpr int level_shift(int level) { return level == 0 ? 21 : level == 1 ? 10 : 0; }
 constexpr int level_bits(int level) { return level == 2 ? 10 : 11; }
 
-__device__ __forceinline__ void count_key(SlotsLds &l, int level, uint32_t prefix, uint32_t key) {
+__device__ __forceinline__ void count_key(uint32_t *hist, int level, uint32_t prefix, uint32_t key) {
     const int shift = level_shift(level), bits = level_bits(level);
-    if (level == 0 || (key >> (shift + bits)) == prefix) atomicAdd(&l.hist[(key >> shift) & ((1u << bits) - 1)], 1u);
+    if (level == 0 || (key >> (shift + bits)) == prefix) atomicAdd(&hist[(key >> shift) & ((1u << bits) - 1)], 1u);
 }
 
 // This wavefront's 64 slots from s0: those that go are written at `at`, ascending; `eq` counts the slots
@@ -172,6 +179,7 @@ cache_slots_kernel(SlotsPlan p, const float *__restrict__ weights, const int32_t
     // runs in whole rows of 64, spread over the wavefronts
     const int run = ((j.n + SLOT_WAVES - 1) / SLOT_WAVES + WAVE - 1) / WAVE * WAVE;
     const int lo = min(wv * run, j.n), hi = min(lo + run, j.n);
+    for (int i = threadIdx.x; i < 3 * SLOT_BINS; i += SLOT_THREADS) l.hist[i] = 0;
     Eight v[EIGHTS];
     uint32_t open = 0;
 #pragma unroll
@@ -192,15 +200,14 @@ cache_slots_kernel(SlotsPlan p, const float *__restrict__ weights, const int32_t
     uint32_t prefix = 0, want = uint32_t(j.e);
 #pragma unroll
     for (int level = 0; level < 3; ++level) {
-        for (int i = threadIdx.x; i < SLOT_BINS; i += SLOT_THREADS) l.hist[i] = 0;
-        __syncthreads();
+        uint32_t *hist = l.hist + level * SLOT_BINS;
 #pragma unroll
         for (int i = 0; i < EIGHTS; ++i)
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-                if (lo + (i * 8 + k) * WAVE + lane < hi) count_key(l, level, prefix, v[i].key[k]);
+                if (lo + (i * 8 + k) * WAVE + lane < hi) count_key(hist, level, prefix, v[i].key[k]);
         __syncthreads();
-        prefix = prefix << level_bits(level) | find_bin(l, l.hist[2 * threadIdx.x], l.hist[2 * threadIdx.x + 1], want);
+        prefix = prefix << level_bits(level) | find_bin(l, level, hist[2 * threadIdx.x], hist[2 * threadIdx.x + 1], want);
     }
     uint32_t less = 0, same = 0;
 #pragma unroll
@@ -213,9 +220,8 @@ cache_slots_kernel(SlotsPlan p, const float *__restrict__ weights, const int32_t
         }
     if (lane == 0) l.wave_sum[wv] = less, l.wave_sum2[wv] = same;
     __syncthreads();
-    uint32_t at = 0, eq = 0;
-    for (int i = 0; i < wv; ++i) at += l.wave_sum[i], eq += l.wave_sum2[i];
-    at += min(eq, want);
+    uint32_t eq = sum_front(l.wave_sum2);
+    uint32_t at = sum_front(l.wave_sum) + min(eq, want);
 #pragma unroll
     for (int i = 0; i < EIGHTS; ++i)
 #pragma unroll
@@ -274,7 +280,7 @@ cache_slots_piece_kernel(SlotsPlan p, const float *__restrict__ weights, const i
                 h0 += x.x, h1 += x.y;
                 f0 += i < piece ? x.x : 0, f1 += i < piece ? x.y : 0;
             }
-            const uint32_t bin = find_bin(l, h0, h1, want);
+            const uint32_t bin = find_bin(l, level, h0, h1, want);
             if (PHASE == 3) {
                 front += block_sum(l, (uint32_t(t2) < bin ? f0 : 0) + (uint32_t(t2 + 1) < bin ? f1 : 0));
                 if (level == 2) eq = block_sum(l, (uint32_t(t2) == bin ? f0 : 0) + (uint32_t(t2 + 1) == bin ? f1 : 0));
@@ -295,7 +301,7 @@ cache_slots_piece_kernel(SlotsPlan p, const float *__restrict__ weights, const i
                 const bool prot = v.prot >> k & 1;
                 open += prot ? 0 : 1;
                 if (PHASE == 0) atomicAdd(&l.hist[(prot ? SLOT_BINS : 0) + (v.key[k] >> level_shift(0))], 1u);
-                else if (prot == among_protected) count_key(l, PHASE, prefix, v.key[k]);
+                else if (prot == among_protected) count_key(l.hist, PHASE, prefix, v.key[k]);
             }
         }
         if (PHASE == 0) {
@@ -319,9 +325,8 @@ cache_slots_piece_kernel(SlotsPlan p, const float *__restrict__ weights, const i
         }
         if (lane == 0) l.wave_sum[wv] = less, l.wave_sum2[wv] = same;
         __syncthreads();
-        uint32_t at = front;
-        for (int i = 0; i < wv; ++i) at += l.wave_sum[i], eq += l.wave_sum2[i];
-        at += min(eq, want);
+        eq += sum_front(l.wave_sum2);
+        uint32_t at = front + sum_front(l.wave_sum) + min(eq, want);
         for (int s0 = lo; s0 < hi; s0 += 8 * WAVE) {
             const Eight v = load_eight(p, j, weights, stamps, h, s0 + lane, hi);
 #pragma unroll
