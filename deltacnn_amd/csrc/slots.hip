@@ -98,8 +98,11 @@ __device__ __forceinline__ uint32_t final_key(uint32_t key, bool prot, bool amon
 }
 
 // A histogram and the places of its scan for every level, so that a level need not wait for the one before.
+// The first one, whose keys share few leading bits, has four copies: four lanes in a row that meet in a bin
+// do not wait for each other, and the copies start in different banks.
+constexpr int COPY = SLOT_BINS + 16, COPIES = 4;
 struct SlotsLds {
-    uint32_t hist[3 * SLOT_BINS];
+    uint32_t hist[COPIES * COPY + 2 * SLOT_BINS];
     uint32_t scan[3][SLOT_WAVES], found[3][2];
     uint32_t wave_sum[SLOT_WAVES], wave_sum2[SLOT_WAVES];
 };
@@ -179,17 +182,14 @@ cache_slots_kernel(SlotsPlan p, const float *__restrict__ weights, const int32_t
     // runs in whole rows of 64, spread over the wavefronts
     const int run = ((j.n + SLOT_WAVES - 1) / SLOT_WAVES + WAVE - 1) / WAVE * WAVE;
     const int lo = min(wv * run, j.n), hi = min(lo + run, j.n);
-    for (int i = threadIdx.x; i < 3 * SLOT_BINS; i += SLOT_THREADS) l.hist[i] = 0;
+    for (int i = threadIdx.x; i < COPIES * COPY + 2 * SLOT_BINS; i += SLOT_THREADS) l.hist[i] = 0;
     Eight v[EIGHTS];
     uint32_t open = 0;
 #pragma unroll
     for (int i = 0; i < EIGHTS; ++i) {
-        v[i].prot = 0;
-        if (lo + i * 8 * WAVE < hi) {
-            v[i] = load_eight(p, j, weights, stamps, h, lo + i * 8 * WAVE + lane, hi);
+        v[i] = load_eight(p, j, weights, stamps, h, lo + i * 8 * WAVE + lane, hi);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) open += lo + (i * 8 + k) * WAVE + lane < hi && !(v[i].prot >> k & 1) ? 1 : 0;
-        }
+        for (int k = 0; k < 8; ++k) open += lo + (i * 8 + k) * WAVE + lane < hi && !(v[i].prot >> k & 1) ? 1 : 0;
     }
     const bool among_protected = uint32_t(j.e) > block_sum(l, open);
 #pragma unroll
@@ -200,14 +200,22 @@ cache_slots_kernel(SlotsPlan p, const float *__restrict__ weights, const int32_t
     uint32_t prefix = 0, want = uint32_t(j.e);
 #pragma unroll
     for (int level = 0; level < 3; ++level) {
-        uint32_t *hist = l.hist + level * SLOT_BINS;
+        uint32_t *hist = level == 0 ? l.hist + (lane & 3) * COPY : l.hist + COPIES * COPY + (level - 1) * SLOT_BINS;
 #pragma unroll
         for (int i = 0; i < EIGHTS; ++i)
 #pragma unroll
             for (int k = 0; k < 8; ++k)
                 if (lo + (i * 8 + k) * WAVE + lane < hi) count_key(hist, level, prefix, v[i].key[k]);
         __syncthreads();
-        prefix = prefix << level_bits(level) | find_bin(l, level, hist[2 * threadIdx.x], hist[2 * threadIdx.x + 1], want);
+        uint32_t h0 = 0, h1 = 0;
+        const int t2 = 2 * threadIdx.x;
+        if (level == 0) {
+#pragma unroll
+            for (int c = 0; c < COPIES; ++c) h0 += l.hist[c * COPY + t2], h1 += l.hist[c * COPY + t2 + 1];
+        } else {
+            h0 = hist[t2], h1 = hist[t2 + 1];
+        }
+        prefix = prefix << level_bits(level) | find_bin(l, level, h0, h1, want);
     }
     uint32_t less = 0, same = 0;
 #pragma unroll
@@ -231,13 +239,14 @@ cache_slots_kernel(SlotsPlan p, const float *__restrict__ weights, const int32_t
         }
 }
 
-// Words of a piece in the workspace: its number of unprotected slots, the first level's histograms of the
-// unprotected and of the protected, those of the second and the third level.
+// Words of a piece in the workspace: its number of unprotected slots and what is known so far, the first
+// level's histograms of the unprotected and of the protected, those of the second and the third level.
+constexpr int PIECE_OPEN = 0, PIECE_AMONG = 1, PIECE_PREFIX = 2, PIECE_WANT = 3, PIECE_FRONT = 4;
 constexpr int PIECE_L0 = 16, PIECE_L1 = PIECE_L0 + 2 * SLOT_BINS, PIECE_L2 = PIECE_L1 + SLOT_BINS;
 constexpr int PIECE_WORDS = PIECE_L2 + SLOT_BINS;
 
 // Launch PHASE of four over (piece, head, stream): the histograms of levels 0, 1 and 2, then the slots.
-// Each sums the earlier launches' histograms over all pieces and finds the bins for itself.
+// Each sums the histogram of the launch before over all pieces and finds the bin for itself.
 template <int PHASE>
 __global__ void __launch_bounds__(SLOT_THREADS)
 cache_slots_piece_kernel(SlotsPlan p, const float *__restrict__ weights, const int32_t *__restrict__ stamps,
@@ -252,41 +261,51 @@ cache_slots_piece_kernel(SlotsPlan p, const float *__restrict__ weights, const i
     const int t2 = 2 * threadIdx.x;
     const int lo = int(min((int64_t(piece) * SLOT_WAVES + wv) * p.run, int64_t(j.n))), hi = int(min(int64_t(lo) + p.run, int64_t(j.n)));
 
-    // what the launches before found: whether the choice is among the protected, the threshold's leading
-    // bits, its rank, and how many slots in front of this piece go for certain or lie at the threshold
+    // Everything that is read is asked for at once: the first eight slots of a thread (all of them in caches up
+    // to 2^19 slots) and the counts of the launch before.
+    const Eight front_keys = load_eight(p, j, weights, stamps, h, lo + lane, hi);
+    auto eight = [&](int s0) { return s0 == lo ? front_keys : load_eight(p, j, weights, stamps, h, s0 + lane, hi); };
+
+    // What is known so far: whether the choice is among the protected, the threshold's leading bits, its rank
+    // among the keys that share them, and how many slots in front of this piece go for certain or (at last)
+    // lie at the threshold.  Each launch adds the level of the one before and leaves its piece the sum.
     bool among_protected = false;
     uint32_t prefix = 0, want = uint32_t(j.e), front = 0, eq = 0;
     if constexpr (PHASE > 0) {
+        constexpr int KINDS = PHASE == 1 ? 2 : 1, FIRST = PHASE == 1 ? PIECE_L0 : PHASE == 2 ? PIECE_L1 : PIECE_L2;
+        uint2 all[KINDS], before[KINDS];
         uint32_t open = 0, open_front = 0;
-        for (int i = threadIdx.x; i < p.pieces; i += SLOT_THREADS) {
-            const uint32_t x = space[int64_t(i) * PIECE_WORDS];
-            open += x;
-            open_front += i < piece ? x : 0;
-        }
-        open = block_sum(l, open);
-        among_protected = uint32_t(j.e) > open;
-        if (among_protected) want -= open;
-        if (PHASE == 3) {
-            open_front = block_sum(l, open_front);
-            front = among_protected ? open_front : 0;
-        }
 #pragma unroll
-        for (int level = 0; level < PHASE; ++level) {
-            const int base = level == 0 ? PIECE_L0 + (among_protected ? SLOT_BINS : 0) : level == 1 ? PIECE_L1 : PIECE_L2;
-            uint32_t h0 = 0, h1 = 0, f0 = 0, f1 = 0;
+        for (int q = 0; q < KINDS; ++q) all[q] = before[q] = make_uint2(0, 0);
+        if (PHASE > 1) among_protected = mine[PIECE_AMONG] != 0, prefix = mine[PIECE_PREFIX], want = mine[PIECE_WANT], front = mine[PIECE_FRONT];
 #pragma unroll 8
-            for (int i = 0; i < p.pieces; ++i) {
-                const uint2 x = *reinterpret_cast<const uint2 *>(space + int64_t(i) * PIECE_WORDS + base + t2);
-                h0 += x.x, h1 += x.y;
-                f0 += i < piece ? x.x : 0, f1 += i < piece ? x.y : 0;
+        for (int i = 0; i < p.pieces; ++i) {
+            const uint32_t *from = space + int64_t(i) * PIECE_WORDS;
+            if (PHASE == 1 && threadIdx.x == 0) {
+                open += from[PIECE_OPEN];
+                open_front += i < piece ? from[PIECE_OPEN] : 0;
             }
-            const uint32_t bin = find_bin(l, level, h0, h1, want);
-            if (PHASE == 3) {
-                front += block_sum(l, (uint32_t(t2) < bin ? f0 : 0) + (uint32_t(t2 + 1) < bin ? f1 : 0));
-                if (level == 2) eq = block_sum(l, (uint32_t(t2) == bin ? f0 : 0) + (uint32_t(t2 + 1) == bin ? f1 : 0));
+#pragma unroll
+            for (int q = 0; q < KINDS; ++q) {
+                const uint2 x = *reinterpret_cast<const uint2 *>(from + FIRST + q * SLOT_BINS + t2);
+                all[q].x += x.x, all[q].y += x.y;
+                before[q].x += i < piece ? x.x : 0, before[q].y += i < piece ? x.y : 0;
             }
-            prefix = prefix << level_bits(level) | bin;
         }
+        uint32_t below = 0;
+        if (PHASE == 1) {
+            open = block_sum(l, open);
+            among_protected = uint32_t(j.e) > open;
+            if (among_protected) want -= open, below = open_front;
+        }
+        const uint2 x = among_protected ? all[KINDS - 1] : all[0], y = among_protected ? before[KINDS - 1] : before[0];
+        const uint32_t bin = find_bin(l, PHASE - 1, x.x, x.y, want);
+        below += (uint32_t(t2) < bin ? y.x : 0) + (uint32_t(t2 + 1) < bin ? y.y : 0);
+        front += block_sum(l, below);
+        if (PHASE == 3) eq = block_sum(l, (uint32_t(t2) == bin ? y.x : 0) + (uint32_t(t2 + 1) == bin ? y.y : 0));
+        prefix = prefix << level_bits(PHASE - 1) | bin;
+        if (PHASE < 3 && threadIdx.x == 0)
+            mine[PIECE_AMONG] = among_protected, mine[PIECE_PREFIX] = prefix, mine[PIECE_WANT] = want, mine[PIECE_FRONT] = front;
     }
     if constexpr (PHASE < 3) {
         constexpr int HISTS = PHASE == 0 ? 2 : 1;
@@ -294,7 +313,7 @@ cache_slots_piece_kernel(SlotsPlan p, const float *__restrict__ weights, const i
         __syncthreads();
         uint32_t open = 0;
         for (int s0 = lo; s0 < hi; s0 += 8 * WAVE) {
-            const Eight v = load_eight(p, j, weights, stamps, h, s0 + lane, hi);
+            const Eight v = eight(s0);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 if (s0 + k * WAVE + lane >= hi) continue;
@@ -306,7 +325,7 @@ cache_slots_piece_kernel(SlotsPlan p, const float *__restrict__ weights, const i
         }
         if (PHASE == 0) {
             open = block_sum(l, open);
-            if (threadIdx.x == 0) mine[0] = open;
+            if (threadIdx.x == 0) mine[PIECE_OPEN] = open;
         }
         __syncthreads();
         uint32_t *to = mine + (PHASE == 0 ? PIECE_L0 : PHASE == 1 ? PIECE_L1 : PIECE_L2);
@@ -314,7 +333,7 @@ cache_slots_piece_kernel(SlotsPlan p, const float *__restrict__ weights, const i
     } else {
         uint32_t less = 0, same = 0;
         for (int s0 = lo; s0 < hi; s0 += 8 * WAVE) {
-            const Eight v = load_eight(p, j, weights, stamps, h, s0 + lane, hi);
+            const Eight v = eight(s0);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 const bool in = s0 + k * WAVE + lane < hi;
@@ -328,7 +347,7 @@ cache_slots_piece_kernel(SlotsPlan p, const float *__restrict__ weights, const i
         eq += sum_front(l.wave_sum2);
         uint32_t at = front + sum_front(l.wave_sum) + min(eq, want);
         for (int s0 = lo; s0 < hi; s0 += 8 * WAVE) {
-            const Eight v = load_eight(p, j, weights, stamps, h, s0 + lane, hi);
+            const Eight v = eight(s0);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 const int s = s0 + k * WAVE + lane;
