@@ -946,13 +946,38 @@ attention_weights_kernel(AttnPlan p, FastDiv by_group, const E *__restrict__ q, 
     }
     const int rows = count * p.group, r_first = min(begin * p.group, rows) / BM * BM;
     const E *zero = reinterpret_cast<const E *>(&zero_chunk);
-    auto request = [&](int r0, char *to) {
+    const int ahead_tok = int(by_group.quot(BM)), ahead_head = BM - ahead_tok * p.group;  // a tile of rows further on
+    // A lane's way through the rows, BM at a time, without a division: its token and head of the group, and what it
+    // reads there.
+    struct Walk {
+        int tok, g;
+    };
+    auto start = [&](int r) {
+        Walk w;
+        w.tok = int(by_group.quot(uint32_t(r)));
+        w.g = r - w.tok * p.group;
+        return w;
+    };
+    auto step = [&](Walk &w, auto *&at, int64_t by_tok, int64_t by_head) {  // strides of a token and of a head
+        w.tok += ahead_tok, w.g += ahead_head;
+        const bool carry = w.g >= p.group;
+        w.tok += carry ? 1 : 0, w.g -= carry ? p.group : 0;
+        at += ahead_tok * by_tok + ahead_head * by_head + (carry ? by_tok - p.group * by_head : 0);
+    };
+    Walk qw[REQ];
+    const E *qp[REQ];
+#pragma unroll
+    for (int j = 0; j < REQ; ++j) {
+        const int rr = (wv * REQ + j) * RPI + lane / CPR;
+        qw[j] = start(r_first + rr);
+        qp[j] = q + int64_t(first + qw[j].tok) * p.qt + (h * p.group + qw[j].g) * p.qh + ((lane % CPR) ^ key_swizzle<E, DP>(rr)) * N;
+    }
+    auto request = [&](uint32_t to) {  // the next tile of rows
 #pragma unroll
         for (int j = 0; j < REQ; ++j) {
-            const int rr = (wv * REQ + j) * RPI + lane / CPR, r = r0 + rr, e = ((lane % CPR) ^ key_swizzle<E, DP>(rr)) * N;
-            const int tok = int(by_group.quot(uint32_t(min(r, rows - 1))));
-            const E *src = r < rows && e < p.dim ? q + int64_t(first + tok) * p.qt + (h * p.group + r - tok * p.group) * p.qh + e : zero;
-            fetch(src, lds_place(to) + (wv * REQ + j) * 1024);
+            const int rr = (wv * REQ + j) * RPI + lane / CPR, e = ((lane % CPR) ^ key_swizzle<E, DP>(rr)) * N;
+            fetch(qw[j].tok < count && e < p.dim ? qp[j] : zero, to + (wv * REQ + j) * 1024);
+            step(qw[j], qp[j], p.qt, p.qh);
         }
     };
     const float scale = p.flip != 0 ? -p.scale : p.scale;
@@ -961,53 +986,78 @@ attention_weights_kernel(AttnPlan p, FastDiv by_group, const E *__restrict__ q, 
     for (int i = 0; i < NB; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
-    if (r_first < rows) request(r_first, lds);
-    int stage = 0;
-    for (int r0 = r_first; r0 < rows; r0 += BM, stage ^= 1) {
-        // this lane's rows: minus their log-sum in powers of two (no row, or one that sees nothing: -inf), and what they see
-        float less[BM / 32];
-        int limit[BM / 32];
+    // this lane's row of a tile: its log-sum (-inf: no row, or one that sees nothing) and what it sees
+    struct Row {
+        float lse;
+        int limit;
+    };
+    Walk lw[BM / 32];
+    const float *lp[BM / 32];
 #pragma unroll
-        for (int i = 0; i < BM / 32; ++i) {
-            const int r = r0 + 32 * i + col, tok = int(by_group.quot(uint32_t(min(r, rows - 1))));
-            less[i] = -INFINITY, limit[i] = 0;
-            if (r < rows) {
-                const float z = lse[int64_t(first + tok) * p.q_heads + h * p.group + r - tok * p.group];
-                less[i] = z == -INFINITY ? -INFINITY : z * -1.44269504088896341f;
-                limit[i] = visible(len, count, tok, p.causal_block);
-            }
-        }
-        arrived();
-        __syncthreads();
-        const uint32_t qt = lds_place(lds) + stage * TILE;
-        if (r0 + BM < rows) request(r0 + BM, lds + (stage ^ 1) * TILE);
-        const bool whole = s0 + 32 * NB <= visible(len, count, int(by_group.quot(uint32_t(r0))), p.causal_block);
+    for (int i = 0; i < BM / 32; ++i) {
+        lw[i] = start(r_first + 32 * i + col);
+        lp[i] = lse + int64_t(first + lw[i].tok) * p.q_heads + h * p.group + lw[i].g;
+    }
+    auto next_row = [&](int i) {
+        Row x = {-INFINITY, len};
+        if (lw[i].tok < count) x.lse = *lp[i];
+        if (p.causal_block != 0) x.limit = visible(len, count, lw[i].tok, p.causal_block);
+        step(lw[i], lp[i], p.q_heads, 1);
+        return x;
+    };
+    const uint32_t place = lds_place(lds);
+    auto scores = [&](float16_t(&s)[NB], uint32_t qt) {
+        chunk qf[STEPS];
 #pragma unroll
-        for (int j = 0; j < BM / 32; ++j) {
-            float16_t s[NB];
+        for (int t = 0; t < STEPS; ++t) qf[t] = lds_read<chunk>((qt + col * ROW + ((half ^ key_swizzle<E, DP>(col)) << 4)) ^ (t << 5));
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[i][r] = 0.f;
+#pragma unroll
+        for (int t = 0; t < STEPS; ++t)
+#pragma unroll
+            for (int i = 0; i < NB; ++i) s[i] = Chunk<E>::mma(k[i][t], qf[t], s[i]);
+    };
+    auto add = [&](const float16_t(&s)[NB], Row x, bool whole) {
+        const float less = x.lse == -INFINITY ? -INFINITY : x.lse * -1.44269504088896341f;
+        if (whole) {
 #pragma unroll
             for (int i = 0; i < NB; ++i)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[i][r] = 0.f;
+                for (int r = 0; r < 16; ++r) acc[i][r] += __builtin_amdgcn_exp2f(fmaf(s[i][r], scale, less));
+        } else {
 #pragma unroll
-            for (int t = 0; t < STEPS; ++t) {
-                const chunk qf = lds_read<chunk>(((qt + col * ROW + ((half ^ key_swizzle<E, DP>(col)) << 4)) ^ (t << 5)) + 32 * j * ROW);
+            for (int i = 0; i < NB; ++i)
 #pragma unroll
-                for (int i = 0; i < NB; ++i) s[i] = Chunk<E>::mma(k[i][t], qf, s[i]);
-            }
-            if (whole) {
+                for (int r = 0; r < 16; ++r) {
+                    const float e = __builtin_amdgcn_exp2f(fmaf(s[i][r], scale, less));
+                    acc[i][r] += s0 + 32 * i + 8 * (r / 4) + 4 * half + r % 4 < x.limit ? e : 0.f;
+                }
+        }
+    };
+    if (r_first < rows) {
+        request(place);
+        Row x[BM / 32];
 #pragma unroll
-                for (int i = 0; i < NB; ++i)
+        for (int i = 0; i < BM / 32; ++i) x[i] = next_row(i);
+        uint32_t stage = 0;
+        for (int r0 = r_first; r0 < rows; r0 += BM, stage ^= 1) {
+            arrived();
+            __syncthreads();
+            // the next tile and its rows' log-sums are on their way while this one is worked on (asked for where
+            // they are needed, the log-sums alone made every tile wait for memory)
+            Row y[BM / 32];
+            if (r0 + BM < rows) request(place + (stage ^ 1) * TILE);
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) acc[i][r] += __builtin_amdgcn_exp2f(fmaf(s[i][r], scale, less[j]));
-            } else {
+            for (int i = 0; i < BM / 32; ++i) y[i] = next_row(i);
+            const bool whole = s0 + 32 * NB <= visible(len, count, int(by_group.quot(uint32_t(r0))), p.causal_block);
 #pragma unroll
-                for (int i = 0; i < NB; ++i)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const float e = __builtin_amdgcn_exp2f(fmaf(s[i][r], scale, less[j]));
-                        acc[i][r] += s0 + 32 * i + 8 * (r / 4) + 4 * half + r % 4 < limit[j] ? e : 0.f;
-                    }
+            for (int i = 0; i < BM / 32; ++i) {
+                float16_t s[NB];
+                scores(s, place + stage * TILE + 32 * i * ROW);
+                add(s, x[i], whole);
+                x[i] = y[i];
             }
         }
     }
