@@ -1006,10 +1006,13 @@ attention_weights_kernel(AttnPlan p, FastDiv by_group, const E *__restrict__ q, 
         return x;
     };
     const uint32_t place = lds_place(lds);
-    auto scores = [&](float16_t(&s)[NB], uint32_t qt) {
-        chunk qf[STEPS];
+    chunk qf[STEPS];
+    auto rows_of = [&](uint32_t qt) {
 #pragma unroll
         for (int t = 0; t < STEPS; ++t) qf[t] = lds_read<chunk>((qt + col * ROW + ((half ^ key_swizzle<E, DP>(col)) << 4)) ^ (t << 5));
+        __builtin_amdgcn_sched_barrier(0);  // all requested before anything else
+    };
+    auto scores = [&](float16_t(&s)[NB]) {
 #pragma unroll
         for (int i = 0; i < NB; ++i)
 #pragma unroll
@@ -1045,8 +1048,8 @@ attention_weights_kernel(AttnPlan p, FastDiv by_group, const E *__restrict__ q, 
         for (int r0 = r_first; r0 < rows; r0 += BM, stage ^= 1) {
             arrived();
             __syncthreads();
-            // the next tile and its rows' log-sums are on their way while this one is worked on (asked for where
-            // they are needed, the log-sums alone made every tile wait for memory)
+            rows_of(place + stage * TILE);
+            // the next tile and its rows' log-sums are on their way while this one is worked on
             Row y[BM / 32];
             if (r0 + BM < rows) request(place + (stage ^ 1) * TILE);
 #pragma unroll
@@ -1055,7 +1058,8 @@ attention_weights_kernel(AttnPlan p, FastDiv by_group, const E *__restrict__ q, 
 #pragma unroll
             for (int i = 0; i < BM / 32; ++i) {
                 float16_t s[NB];
-                scores(s, place + stage * TILE + 32 * i * ROW);
+                scores(s);
+                if (i + 1 < BM / 32) rows_of(place + stage * TILE + 32 * (i + 1) * ROW);  // in time for the exponentials
                 add(s, x[i], whole);
                 x[i] = y[i];
             }
