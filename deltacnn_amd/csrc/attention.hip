@@ -199,6 +199,9 @@ __device__ __forceinline__ void fetch(const void *from, uint32_t to) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "memory");
 }
 __device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// The loads that the compiler knows of: waited for in front of a loop they do not make it wait in there, where
+// it would be for the newest requests above.
+__device__ __forceinline__ void loaded() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
 // .. all but the newest N requests
 template <int N>
 __device__ __forceinline__ void arrived_but() {
@@ -779,6 +782,7 @@ attention_mfma_kernel(AttnCall call) {
         st.template add_values<true>(vf, pr, vplace + ((vslot + 3 * TILE) & 3 * TILE), k0 - BN, limit);
         arrived();  // nothing may reach this LDS after the workgroup has left it
     } else {
+        loaded();
         if (first < ke) {
             load.look();
             const auto x = load.find(p, loader, first, ke);
@@ -1045,6 +1049,7 @@ attention_weights_kernel(AttnPlan p, FastDiv by_group, const E *__restrict__ q, 
 #pragma unroll
         for (int i = 0; i < BM / 32; ++i) x[i] = next_row(i);
         uint32_t stage = 0;
+        loaded();
         for (int r0 = r_first; r0 < rows; r0 += BM, stage ^= 1) {
             arrived();
             __syncthreads();
