@@ -221,66 +221,75 @@ __device__ __forceinline__ int value_swizzle(int row) {
     return sizeof(E) == 4 ? 0 : DP >= 128 ? (row & 3) << 2 : (row & 2) << 1;
 }
 
+// How many pages a tile of slots may touch: in ONE its rows follow each other, in TWO there is one seam, and
+// the pages' numbers are the same for all lanes; only for MANY does every row look for its page.
+enum Pages { ONE, TWO, MANY };
+
 // BN slots of one head on their way into LDS.  The lanes choose what they fetch, the places they fill are
 // fixed.  What lies behind `end` or in no page of the pool, and the elements from dim to DP, arrive as
-// zeros: from the bound of the buffer resource where a tile lies in one page (ALIGNED), else from a
-// chunk of zeros.
-template <typename E, int DP, int BN, int LOADERS, bool ALIGNED>
+// zeros: from the bound of the buffer resource (ONE), else from a chunk of zeros.
+template <typename E, int DP, int BN, int LOADERS, Pages PAGES>
 struct TileLoader {
     static constexpr int N = Chunk<E>::N, CPR = DP / N, RPI = WAVE / CPR, REQ = BN / RPI / LOADERS;
     static_assert(REQ >= 1, "one request a wavefront at least");
     const int32_t *table;
-    const E *keys, *values;  // ALIGNED: from this head's first row of a page
+    const E *keys, *values;  // ONE, TWO: from this head's first row of a page
     int dim, h, page_size, num_pages;
     bool bad = false;
-    // ALIGNED: bytes of a lane from the tile's first element; the tile to be found next: its page (`fresh`: not
-    // looked at yet), the bytes in front of that in the pool, its place inside
+    // ONE, TWO: bytes of a lane from the tile's first element; the tile to be found next: its page (ONE, `fresh`:
+    // not looked at yet) and the one behind it, the bytes in front in the pool, its place inside
     uint32_t koffset[REQ], voffset[REQ], page_bytes, row_bytes;
-    int index, inside, page;
+    int index, inside, page, behind;
     uint64_t page_at;
     bool fresh, lost;
+    static constexpr uint32_t NOWHERE = 0x40000000u;  // behind any tile: elements from dim on
 
     __device__ __forceinline__ void init(const AttnPlan &p, const int32_t *table_, const E *k, const E *v, int h_, int loader, int k0) {
         table = table_, dim = p.dim, h = h_, page_size = p.pool.page_size, num_pages = p.pool.num_pages;
-        const int64_t head = ALIGNED ? int64_t(h) * page_size * dim : 0;
+        const int64_t head = PAGES != MANY ? int64_t(h) * page_size * dim : 0;
         keys = k + head, values = v + head;
-        if constexpr (ALIGNED) {
+        if constexpr (PAGES != MANY) {
             row_bytes = uint32_t(dim) * sizeof(E);
             page_bytes = uint32_t(p.kv_heads) * page_size * row_bytes;
             index = uniform(p.pool.by_page.quot(uint32_t(k0)));
             inside = uniform(k0 - index * page_size);
-            page = 0, page_at = 0, fresh = true, lost = false;
+            page = behind = 0, page_at = 0, fresh = true, lost = false;
             const int c = lane_id() % CPR, row0 = loader * REQ * RPI + lane_id() / CPR;
 #pragma unroll
             for (int j = 0; j < REQ; ++j) {
                 const int row = row0 + j * RPI, ck = c ^ key_swizzle<E, DP>(row), cv = c ^ value_swizzle<E, DP>(row);
-                koffset[j] = ck * N < dim ? uint32_t(row * dim + ck * N) * sizeof(E) : 0x40000000u;
-                voffset[j] = cv * N < dim ? uint32_t(row * dim + cv * N) * sizeof(E) : 0x40000000u;
+                koffset[j] = ck * N < dim ? uint32_t(row * dim + ck * N) * sizeof(E) : NOWHERE;
+                voffset[j] = cv * N < dim ? uint32_t(row * dim + cv * N) * sizeof(E) : NOWHERE;
             }
         }
     }
-    // The page of the next tile, a step ahead of its request.
-    __device__ __forceinline__ void look() {
-        // (nothing writes the table meanwhile: a scalar load, which the counted waits do not see)
-        if constexpr (ALIGNED)
-            if (fresh) page = *(const __attribute__((address_space(4))) int32_t *)(table + index);
+    // The pages of the next tile, which starts at slot k, a step ahead of its request.  (Nothing writes the table
+    // meanwhile: scalar loads, which the counted waits do not see.)
+    __device__ __forceinline__ void look(int k, int end) {
+        if constexpr (PAGES != MANY) {
+            const auto *at = (const __attribute__((address_space(4))) int32_t *)(table + index);
+            if (PAGES == TWO || fresh) page = at[0];
+            if (PAGES == TWO && k + min(BN, page_size - inside) < min(k + BN, end)) behind = at[1];
+        }
     }
     __device__ __forceinline__ void advance(int by) {
-        if constexpr (ALIGNED) {
+        if constexpr (PAGES != MANY) {
             inside += by;
             while (inside >= page_size) inside -= page_size, ++index, fresh = true;
         }
     }
-    // Where a tile's rows are: ALIGNED its bytes from the head's first page and how many are in use, else a row of each request (or -1)
+    // Where a tile's rows are: ONE its bytes from the head's first page and how many are in use; TWO the same for the
+    // rows up to the seam and behind it, and the rows in use of both; MANY a row of each request (or -1).
     struct Place {
-        uint64_t at;
+        uint64_t at, at_behind;
         uint32_t bytes;
-        int64_t row[ALIGNED ? 1 : REQ];
+        int seam, rows, rows_behind;
+        int64_t row[PAGES == MANY ? REQ : 1];
     };
     // Slots [k0, end); behind `end` nothing
     __device__ __forceinline__ Place find(const AttnPlan &p, int loader, int k0, int end) {
         Place x;
-        if constexpr (ALIGNED) {
+        if constexpr (PAGES == ONE) {
             if (fresh && k0 < end) {
                 lost = uint32_t(page) >= uint32_t(num_pages);
                 bad = bad || lost;
@@ -289,6 +298,15 @@ struct TileLoader {
             }
             x.at = page_at + uint32_t(inside) * row_bytes;
             x.bytes = lost ? 0u : uint32_t(max(min(BN, end - k0), 0)) * row_bytes;
+        } else if constexpr (PAGES == TWO) {
+            const int rows = max(min(BN, end - k0), 0);
+            x.seam = page_size - inside;
+            const bool lost0 = rows > 0 && uint32_t(page) >= uint32_t(num_pages), lost1 = rows > x.seam && uint32_t(behind) >= uint32_t(num_pages);
+            bad = bad || lost0 || lost1;
+            x.at = lost0 ? 0 : uint64_t(uint32_t(page)) * page_bytes + uint32_t(inside) * row_bytes;
+            x.at_behind = lost1 ? 0 : uint64_t(uint32_t(behind)) * page_bytes - uint64_t(x.seam) * row_bytes;  // row `seam` is its first
+            x.rows = lost0 ? 0 : min(rows, x.seam);
+            x.rows_behind = lost1 ? 0 : rows;
         } else {
             const int row0 = loader * REQ * RPI + lane_id() / CPR;
 #pragma unroll
@@ -307,15 +325,26 @@ struct TileLoader {
     template <bool VALUES>
     __device__ __forceinline__ void request(const Place &x, int loader, uint32_t to) {
         const E *from = VALUES ? values : keys;
-        if constexpr (ALIGNED) {
+        const int row0 = loader * REQ * RPI + lane_id() / CPR;
+        if constexpr (PAGES == ONE) {
             const uint64_t a = uint64_t(uintptr_t(from)) + x.at;
             u32x4_t r;
             r[0] = uniform(uint32_t(a)), r[1] = uniform(uint32_t(a >> 32)), r[2] = uniform(x.bytes), r[3] = 0x00027000u;  // addresses have 48 bits
 #pragma unroll
             for (int j = 0; j < REQ; ++j) fetch_bounded(r, VALUES ? voffset[j] : koffset[j], to + j * 1024);
+        } else if constexpr (PAGES == TWO) {
+            const uint64_t zero = uint64_t(uintptr_t(&zero_chunk)), a = uint64_t(uintptr_t(from)) + x.at, b = uint64_t(uintptr_t(from)) + x.at_behind;
+#pragma unroll
+            for (int j = 0; j < REQ; ++j) {
+                const int row = row0 + j * RPI;
+                const uint32_t offset = VALUES ? voffset[j] : koffset[j];
+                const bool over = row >= x.seam, in = row < (over ? x.rows_behind : x.rows) && offset != NOWHERE;
+                const uint64_t at = (over ? b : a) + offset;
+                fetch(reinterpret_cast<const void *>(uintptr_t(in ? at : zero)), to + j * 1024);
+            }
         } else {
             const E *zero = reinterpret_cast<const E *>(&zero_chunk);
-            const int c = lane_id() % CPR, row0 = loader * REQ * RPI + lane_id() / CPR;
+            const int c = lane_id() % CPR;
 #pragma unroll
             for (int j = 0; j < REQ; ++j) {
                 const int row = row0 + j * RPI, e = (c ^ (VALUES ? value_swizzle<E, DP>(row) : key_swizzle<E, DP>(row))) * N;
@@ -667,7 +696,7 @@ struct Shape {
 };
 
 // Attention on the matrix cores.  A wavefront owns 32 rows.
-template <typename E, int DP, bool KEYS, bool NARROW, bool ALIGNED>
+template <typename E, int DP, bool KEYS, bool NARROW, Pages PAGES>
 __global__ void __launch_bounds__((WAVE * Shape<E, DP, KEYS, NARROW>::NW), (Shape<E, DP, KEYS, NARROW>::GROUPS))
 attention_mfma_kernel(AttnCall call) {
     const AttnPlan &p = call.p;
@@ -709,7 +738,7 @@ attention_mfma_kernel(AttnCall call) {
         st.q[t] = __builtin_bit_cast(chunk, u);
     }
     const int32_t *table = p.pool.table + int64_t(w.b) * p.pool.max_pages;
-    typedef TileLoader<E, DP, BN, KEYS ? 1 : NW, ALIGNED> Loader;
+    typedef TileLoader<E, DP, BN, KEYS ? 1 : NW, PAGES> Loader;
     Loader load;
     const int loader = KEYS ? 0 : wv, first = kb + (KEYS ? wv * BN : 0), stride = KEYS ? NW * BN : BN;
     load.init(p, table, keys, values, w.h, loader, first);
@@ -725,10 +754,10 @@ attention_mfma_kernel(AttnCall call) {
         auto next_place = [&](int k0) {
             const auto x = load.find(p, loader, k0, ke);
             load.advance(BN);
-            if (k0 + BN < ke) load.look();  // a turn ahead
+            if (k0 + BN < ke) load.look(k0 + BN, ke);  // a turn ahead
             return x;
         };
-        if (kb < ke) load.look();
+        if (kb < ke) load.look(kb, ke);
         held = next_place(kb);
         load.template request<false>(held, loader, mine);
         for (int i = 1; i < 3; ++i) {
@@ -784,12 +813,12 @@ attention_mfma_kernel(AttnCall call) {
     } else {
         loaded();
         if (first < ke) {
-            load.look();
+            load.look(first, ke);
             const auto x = load.find(p, loader, first, ke);
             load.template request<false>(x, loader, mine);
             load.template request<true>(x, loader, mine + TILE);
             load.advance(stride);
-            if (first + stride < ke) load.look();
+            if (first + stride < ke) load.look(first + stride, ke);
         }
         uint32_t stage = 0;
         int k0 = first;
@@ -803,7 +832,7 @@ attention_mfma_kernel(AttnCall call) {
                 load.template request<false>(x, loader, to);
                 load.template request<true>(x, loader, to + TILE);
                 load.advance(stride);
-                if (k0 + 2 * stride < ke) load.look();
+                if (k0 + 2 * stride < ke) load.look(k0 + 2 * stride, ke);
             }
         };
         // tiles that every row of the workgroup sees as a whole, then the rest
@@ -1003,9 +1032,8 @@ attention_weights_kernel(AttnPlan p, FastDiv by_group, const E *__restrict__ q, 
         lp[i] = lse + int64_t(first + lw[i].tok) * p.q_heads + h * p.group + lw[i].g;
     }
     auto next_row = [&](int i) {
-        Row x = {-INFINITY, len};
-        if (lw[i].tok < count) x.lse = *lp[i];
-        if (p.causal_block != 0) x.limit = visible(len, count, lw[i].tok, p.causal_block);
+        Row x = {-INFINITY, 0};
+        if (lw[i].tok < count) x.lse = *lp[i], x.limit = visible(len, count, lw[i].tok, p.causal_block);
         step(lw[i], lp[i], p.q_heads, 1);
         return x;
     };
@@ -1059,7 +1087,8 @@ attention_weights_kernel(AttnPlan p, FastDiv by_group, const E *__restrict__ q, 
             if (r0 + BM < rows) request(place + (stage ^ 1) * TILE);
 #pragma unroll
             for (int i = 0; i < BM / 32; ++i) y[i] = next_row(i);
-            const bool whole = s0 + 32 * NB <= visible(len, count, int(by_group.quot(uint32_t(r0))), p.causal_block);
+            // (no row behind the last: its scores are zeros, or NaN of an infinite key that gives a real row a weight of 0)
+            const bool whole = r0 + BM <= rows && s0 + 32 * NB <= visible(len, count, int(by_group.quot(uint32_t(r0))), p.causal_block);
 #pragma unroll
             for (int i = 0; i < BM / 32; ++i) {
                 float16_t s[NB];
@@ -1126,7 +1155,6 @@ attention_join_kernel(AttnPlan p, AttnGrid g, T *__restrict__ out, float *__rest
         const float f_here = s0 + lane < pieces ? __builtin_amdgcn_exp2f(m_here - ref) : 0.f;
         l = fmaf(f_here, l_here, l);
         const int n4 = min(WAVE, pieces - s0);
-#pragma unroll 2
         for (int s = lane / 16; s < (n4 + 3) / 4 * 4; s += 4) {
             const float f = __shfl(f_here, s, WAVE);
             if (s >= n4) continue;
@@ -1206,10 +1234,10 @@ hipError_t raise_lds(const void *kernel, int bytes, uint64_t &raised) {
     return err;
 }
 
-template <typename E, int DP, bool KEYS, bool NARROW, bool ALIGNED>
+template <typename E, int DP, bool KEYS, bool NARROW, Pages PAGES>
 hipError_t attention_go(const dc_attention_args &a, const AttnPlan &p, const AttnGrid &g, float *lse, hipStream_t s) {
     typedef Shape<E, DP, KEYS, NARROW> S;
-    auto kernel = attention_mfma_kernel<E, DP, KEYS, NARROW, ALIGNED>;
+    auto kernel = attention_mfma_kernel<E, DP, KEYS, NARROW, PAGES>;
     static thread_local uint64_t raised = 0;
     const hipError_t err = raise_lds((const void *)kernel, S::LDS, raised);
     if (err != hipSuccess) return err;
@@ -1235,16 +1263,28 @@ hipError_t weights_go(const dc_attention_args &a, const AttnPlan &p, const AttnG
     return hipGetLastError();
 }
 
+template <typename E, int DP, Pages PAGES>
+hipError_t attention_pages(const dc_attention_args &a, const AttnPlan &p, const AttnGrid &g, bool few, bool narrow, float *lse, hipStream_t s) {
+    if (few) return attention_go<E, DP, true, false, PAGES>(a, p, g, lse, s);
+    return narrow ? attention_go<E, DP, false, true, PAGES>(a, p, g, lse, s) : attention_go<E, DP, false, false, PAGES>(a, p, g, lse, s);
+}
+
 template <typename E, int DP>
 hipError_t attention_dp(const dc_attention_args &a, const AttnPlan &p, const AttnGrid &g, bool few, float *lse, hipStream_t s) {
-    // tiles inside a page take their rows from one address; a page of 4 GiB has no 32-bit place in the pool
-    const bool aligned = p.pool.page_size % (few ? Shape<E, DP, true>::BN : Shape<E, DP, false>::BN) == 0 &&
-                         int64_t(p.kv_heads) * p.pool.page_size * p.dim * int(sizeof(E)) < (int64_t(1) << 32);
+    // Tiles start at multiples of 32: in pages of a multiple of 32 slots they touch one page, in larger ones two at
+    // most, and two in pages of 16.  A token of 32 streams over 32640 slots, 128 elements, 16 bit: 156 us in ONE
+    // (64 slots a page), 164 / 167 us in TWO and 337 / 318 us in MANY (49 / 16 slots), where a lane's look at the
+    // table waits for the tiles on their way; 16320 tokens in 32 frames: 645, 775 / 754 and 913 / 884 us.
+    // A page of 4 GiB has no 32-bit size.
+    const int ps = p.pool.page_size;
+    const Pages pages = int64_t(p.kv_heads) * ps * p.dim * int(sizeof(E)) >= (int64_t(1) << 32) ? MANY
+                        : ps % 32 == 0                                                    ? ONE
+                        : ps > 32 || ps == 16                                             ? TWO
+                                                                                         : MANY;
     const bool narrow = g.block_rows == 64;
-    hipError_t e;
-    if (few) e = aligned ? attention_go<E, DP, true, false, true>(a, p, g, lse, s) : attention_go<E, DP, true, false, false>(a, p, g, lse, s);
-    else if (narrow) e = aligned ? attention_go<E, DP, false, true, true>(a, p, g, lse, s) : attention_go<E, DP, false, true, false>(a, p, g, lse, s);
-    else e = aligned ? attention_go<E, DP, false, false, true>(a, p, g, lse, s) : attention_go<E, DP, false, false, false>(a, p, g, lse, s);
+    hipError_t e = pages == ONE   ? attention_pages<E, DP, ONE>(a, p, g, few, narrow, lse, s)
+                   : pages == TWO ? attention_pages<E, DP, TWO>(a, p, g, few, narrow, lse, s)
+                                  : attention_pages<E, DP, MANY>(a, p, g, few, narrow, lse, s);
     if (e == hipSuccess && g.splits > 1) {
         note_kernel("attention_join_kernel");
         attention_join_kernel<E><<<ceil_div(p.tokens * p.q_heads, 4), 256, 0, s>>>(p, g, (E *)a.out, lse, a.lens, a.starts);

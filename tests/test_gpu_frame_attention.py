@@ -292,7 +292,37 @@ def test_paged_attention_masked_infinities(lib, dtype, tokens):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids)
-@pytest.mark.parametrize("tokens,page", [(2, 32), (2, 20), (80, 64), (80, 20)])
+@pytest.mark.parametrize("tokens", [1, 3, 70])
+@pytest.mark.parametrize("block", [0, 1])
+def test_paged_attention_visible_infinity(lib, dtype, tokens, block):
+    """A key that gives every row a score of -inf: as if the slot were not there, and no weight for it."""
+    from deltacnn_amd import hip_kernels as hk
+    gen = torch.Generator().manual_seed(15)
+    dim, page, n, bad = 64, 32, 400, 127
+    keys, values, weights, _, table = make_pool(gen, 1, n, 1, page, dim, dtype)
+    q = torch.randn(tokens, 2, dim, generator=gen).to(dtype)
+    q[:, :, 0] = q[:, :, 0].abs() + 0.5
+    lens_t = torch.tensor([n], dtype=torch.int32)
+    pg, off = ref.place(table[0], bad, page)
+    keys[pg, 0, off] = 0
+    keys[pg, 0, off, 0] = -60000.0 / 8  # a score below -400 in the oracle, whose probability is below 2^-500
+    out, tol, lse, lse_tol, ww, w_tol = ref.attention(q, keys, values, table, lens_t, None, None, block, weights, 0.5)
+    small = keys.clone()
+    small[pg, 0, off, 0] = 0  # the bounds: of the scores that count
+    tol, lse_tol, w_tol = (ref.attention(q, small, values, table, lens_t, None, None, block, weights, 0.5)[i] for i in (1, 3, 5))
+    keys[pg, 0, off, 0] = -math.inf
+    w = weights.to(DEV)
+    got, got_lse = hk.paged_attention(q.to(DEV), keys.to(DEV), values.to(DEV), table.to(DEV), lens_t.to(DEV), causal_block=block, weights=w,
+                                      decay=0.5, return_lse=True)
+    assert float(w[pg, 0, off]) == 0.5 * float(weights[pg, 0, off])
+    ref.assert_within(got_lse, lse, lse_tol, "lse")
+    ref.assert_within(w, ww, w_tol, "weights")
+    # (a bound with the slot's value in it is the larger one; both are within half a percent of sum p |v|)
+    ref.assert_within(got, out, 1.01 * tol, "out")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("tokens,page", [(2, 32), (2, 20), (80, 64), (80, 20), (2, 48), (80, 48), (2, 16), (80, 16)])
 def test_paged_attention_lost_page_and_rows_behind(lib, dtype, tokens, page):
     """A page outside the pool makes its own stream NaN and no other; rows behind the last stream stay."""
     from deltacnn_amd import hip_kernels as hk
@@ -487,6 +517,18 @@ def test_layer_starts_anew(lib):
     from deltacnn_amd import _lib
     with pytest.raises(_lib.DeltaCNNError, match="gradient"):
         layer(x)
+
+
+def test_numbers_beyond_32_bits_are_refused(lib):
+    from deltacnn_amd import _lib
+    from deltacnn_amd import hip_kernels as hk
+    pool, table, lens = torch.zeros(2, 1, 8, 16, device=DEV), torch.zeros(1, 2, dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    q = torch.zeros(1, 1, 16, device=DEV)
+    for call in (lambda: hk.paged_attention(q, pool, pool, table, lens, causal_block=1 << 32),
+                 lambda: hk.cache_slots(pool[..., 0].contiguous(), table, lens, (1 << 32) + 1, 8),
+                 lambda: hk.cache_slots(pool[..., 0].contiguous(), table, lens, 1, (1 << 32) + 8)):
+        with pytest.raises(_lib.DeltaCNNError, match="32 bits"):
+            call()
 
 
 def test_layer_under_the_tracer(lib):
