@@ -971,6 +971,30 @@ int check_rows(const char *fn, const char *what, const void *p, int32_t heads, i
     return DC_OK;
 }
 
+// Rows that are written: no two of them share an element.
+int check_apart(const char *fn, const char *what, int32_t tokens, int32_t heads, int32_t dim, int64_t token_stride, int64_t head_stride) {
+    if (tokens > 1 && heads > 1 && token_stride < (heads - 1) * head_stride + dim && head_stride < (tokens - 1) * token_stride + dim)
+        return fail(DC_ERR_UNSUPPORTED, "%s: rows of %s overlap each other", fn, what);
+    return DC_OK;
+}
+
+// Do rows x and y share an element?  Columns of one wider buffer may interleave.
+struct RowSet {
+    const void *p;
+    int32_t tokens, heads, dim;
+    int64_t token_stride, head_stride;
+    int dtype;
+    Span span() const { return Span(p, rows_span(tokens, heads, dim, token_stride, head_stride, dtype)); }
+    int64_t width() const { return (heads - 1) * head_stride + dim; }
+    bool meets(const RowSet &o) const {
+        if (!span().meets(o.span())) return false;
+        if (token_stride != o.token_stride) return true;
+        const int64_t off = (static_cast<const char *>(p) - static_cast<const char *>(o.p)) / (int64_t)esize(dtype);
+        const int64_t column = (off % token_stride + token_stride) % token_stride;
+        return column < o.width() || column + width() > token_stride;
+    }
+};
+
 int check_pool(const char *fn, int32_t streams, int32_t num_pages, int32_t page_size, int32_t max_pages, int32_t tokens,
                const int32_t *page_table, const int32_t *starts) {
     if (streams <= 0 || num_pages <= 0 || page_size <= 0 || max_pages <= 0)
@@ -992,6 +1016,8 @@ int check_heads(const char *fn, int32_t tokens, int32_t q_heads, int32_t kv_head
         return fail(DC_ERR_SHAPE, "%s: tokens=%d, heads=%d/%d, dim=%d must be positive", fn, tokens, q_heads, kv_heads, dim);
     if (tokens > (1 << 24) || q_heads > 1024 || kv_heads > 256)
         return fail(DC_ERR_UNSUPPORTED, "%s: more than 2^24 tokens, 1024 query heads or 256 kv heads", fn);
+    if ((int64_t)tokens * q_heads > (1 << 30) || (int64_t)tokens * kv_heads > (1 << 30))
+        return fail(DC_ERR_UNSUPPORTED, "%s: more than 2^30 rows", fn);
     return DC_OK;
 }
 
@@ -1045,17 +1071,11 @@ int dc_rotary(const dc_rotary_args *a, int dtype, void *stream) {
     DC_REQUIRE_PTR("dc_rotary", a->frequencies);
     DC_REQUIRE_ALIGNED("dc_rotary", a->positions, 4);
     DC_REQUIRE_ALIGNED("dc_rotary", a->frequencies, 8);
-    const Span q(a->q, rows_span(a->tokens, a->q_heads, a->dim, a->q_token_stride, a->q_head_stride, dtype));
-    const Span out(a->out, rows_span(a->tokens, a->q_heads, a->dim, a->out_token_stride, a->out_head_stride, dtype));
-    if (q.meets(out) && a->q != a->out) {  // columns of one wider buffer may interleave, nothing else
-        const int64_t width = (int64_t)(a->q_heads - 1) * a->q_head_stride + a->dim, ts = a->q_token_stride;
-        const int64_t off = (static_cast<const char *>(a->q) - static_cast<const char *>(a->out)) / (int64_t)esize(dtype);
-        const int64_t column = ((off % ts) + ts) % ts;
-        if (ts != a->out_token_stride || a->q_head_stride != a->out_head_stride || column < width || column + width > ts)
-            return fail(DC_ERR_UNSUPPORTED, "%s: out overlaps q without being q", fn);
-    }
-    if (a->q == a->out && (a->q_token_stride != a->out_token_stride || a->q_head_stride != a->out_head_stride))
-        return fail(DC_ERR_UNSUPPORTED, "%s: out overlaps q without being q", fn);
+    if ((rc = check_apart(fn, "out", a->tokens, a->q_heads, a->dim, a->out_token_stride, a->out_head_stride)) != DC_OK) return rc;
+    const RowSet q = {a->q, a->tokens, a->q_heads, a->dim, a->q_token_stride, a->q_head_stride, dtype};
+    const RowSet out = {a->out, a->tokens, a->q_heads, a->dim, a->out_token_stride, a->out_head_stride, dtype};
+    const bool in_place = a->q == a->out && a->q_token_stride == a->out_token_stride && a->q_head_stride == a->out_head_stride;
+    if (!in_place && q.meets(out)) return fail(DC_ERR_UNSUPPORTED, "%s: out overlaps q without being q", fn);
     if (a->keys != nullptr) {
         if ((rc = check_pool(fn, a->streams, a->num_pages, a->page_size, a->max_pages, a->tokens, a->page_table, a->starts)) != DC_OK) return rc;
         if ((rc = check_rows(fn, "k", a->k, a->kv_heads, a->dim, a->k_token_stride, a->k_head_stride, dtype)) != DC_OK) return rc;
@@ -1071,6 +1091,14 @@ int dc_rotary(const dc_rotary_args *a, int dtype, void *stream) {
         DC_REQUIRE_ALIGNED("dc_rotary", a->lens, 4);
         if (a->lens != nullptr) DC_REQUIRE_PTR("dc_rotary", a->new_lens);
         DC_REQUIRE_ALIGNED("dc_rotary", a->new_lens, 4);
+        const RowSet k = {a->k, a->tokens, a->kv_heads, a->dim, a->k_token_stride, a->k_head_stride, dtype};
+        const RowSet v = {a->v, a->tokens, a->kv_heads, a->dim, a->v_token_stride, a->v_head_stride, dtype};
+        if (out.meets(k) || out.meets(v)) return fail(DC_ERR_UNSUPPORTED, "%s: out overlaps k or v", fn);
+        const size_t slots = size_t(a->num_pages) * a->kv_heads * a->page_size, bytes = slots * a->dim * esize(dtype);
+        const Span keys(a->keys, bytes), values(a->values, bytes);
+        for (const Span &x : {q.span(), out.span(), k.span(), v.span(), Span(a->weights, slots * 4), Span(a->stamps, slots * 4)})
+            if (x.meets(keys) || x.meets(values)) return fail(DC_ERR_UNSUPPORTED, "%s: an operand overlaps the cache", fn);
+        if (keys.meets(values)) return fail(DC_ERR_UNSUPPORTED, "%s: keys and values overlap", fn);
     }
     return finish(dc::launch_rotary(*a, dtype, (hipStream_t)stream), fn);
 }
@@ -1102,6 +1130,7 @@ int dc_paged_attention(const dc_attention_args *a, int dtype, void *stream) {
     const Span q(a->q, rows_span(a->tokens, a->q_heads, a->dim, a->q_token_stride, a->q_head_stride, dtype));
     const Span out(a->out, rows_span(a->tokens, a->q_heads, a->dim, a->out_token_stride, a->out_head_stride, dtype));
     const size_t pool = size_t(a->num_pages) * a->kv_heads * a->page_size * a->dim * esize(dtype);
+    if ((rc = check_apart(fn, "out", a->tokens, a->q_heads, a->dim, a->out_token_stride, a->out_head_stride)) != DC_OK) return rc;
     if (out.meets(q) || out.meets(Span(a->keys, pool)) || out.meets(Span(a->values, pool)))
         return fail(DC_ERR_UNSUPPORTED, "%s: out overlaps an operand", fn);
     const int64_t need = dc::paged_attention_workspace(*a);

@@ -761,6 +761,12 @@ def _words(name, what, t, shape, dtype=torch.int32):
         _refuse(f"{name}: {what} must be a dense {str(dtype)[6:]} tensor {tuple(shape)}, got {str(t.dtype)[6:]} {tuple(t.shape)}")
 
 
+def _fits(name, *numbers):
+    """The numbers are 32-bit fields behind the C interface, which would drop their upper bits."""
+    if max(numbers) >= 1 << 31 or min(numbers) < -(1 << 31):
+        _refuse(f"{name}: {max(numbers, key=abs)} does not fit into 32 bits", -3)
+
+
 def _rows(name, what, t, shape, dtype):
     """(token, head) strides of [tokens, heads, dim] rows whose elements are dense; a dimension of one
     element may have any stride in torch, and gets the dense one here."""
@@ -850,6 +856,7 @@ def rotary(x, positions, frequencies, sections, *, interleaved=False, inverse=Fa
     tokens, heads, dim = shape
     if out is None:
         out = torch.empty(shape, dtype=dtype, device=x.device)
+    _fits("rotary", tokens, heads, dim, *sections)
     axes, sec = _sections("rotary", sections, tokens, positions, frequencies)
     xs, xh = _rows("rotary", "x", x, shape, dtype)
     os_, oh = _rows("rotary", "out", out, shape, dtype)
@@ -885,6 +892,7 @@ def rotary_append(q, k, v, positions, frequencies, sections, keys, values, page_
     pages, kv, page, cached_dim = pool
     if dim != cached_dim:
         _refuse(f"{name}: q has {dim} elements a head, the cache {cached_dim}")
+    _fits(name, tokens, heads, dim, pages, kv, page, streams, most, *sections)
     if out is None:
         out = torch.empty(shape, dtype=dtype, device=q.device)
     axes, sec = _sections(name, sections, tokens, positions, frequencies)
@@ -936,6 +944,8 @@ def paged_attention(q, keys, values, page_table, lens, *, starts=None, scale=Non
     pages, kv, page, cached_dim = pool
     if dim != cached_dim:
         _refuse(f"{name}: q has {dim} elements a head, the cache {cached_dim}")
+    causal_block = int(causal_block)
+    _fits(name, tokens, heads, dim, pages, kv, page, streams, most, causal_block)
     if out is None:
         out = torch.empty(shape, dtype=dtype, device=q.device)
     qs, qh = _rows(name, "q", q, shape, dtype)
@@ -946,7 +956,7 @@ def paged_attention(q, keys, values, page_table, lens, *, starts=None, scale=Non
     lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_lse else None
     a = _lib.AttentionArgs(tokens, heads, kv, dim, q.data_ptr(), qs, qh, out.data_ptr(), os_, oh, _ptr(lse), keys.data_ptr(),
                            values.data_ptr(), page_table.data_ptr(), lens.data_ptr(), _ptr(starts), streams, pages, page, most,
-                           int(causal_block), dim ** -0.5 if scale is None else float(scale), _ptr(weights), float(decay))
+                           causal_block, dim ** -0.5 if scale is None else float(scale), _ptr(weights), float(decay))
     ref = ctypes.byref(a)
     need = lib.dc_paged_attention_workspace(ref, dt)
     workspace = None
@@ -957,7 +967,7 @@ def paged_attention(q, keys, values, page_table, lens, *, starts=None, scale=Non
         a.workspace, a.workspace_bytes = workspace.data_ptr(), need
     _launch(name, lib.dc_paged_attention, device, (ref, dt), lambda: dict(
         tokens=tokens, q_heads=heads, kv_heads=kv, dim=dim, esize=q.element_size(), lens=lens, starts=starts,
-        causal_block=int(causal_block), with_weights=weights is not None, keep=(a, q, lse, out, workspace)))
+        causal_block=causal_block, with_weights=weights is not None, keep=(a, q, lse, out, workspace)))
     return (out, lse) if return_lse else out
 
 
@@ -984,6 +994,7 @@ def cache_slots(weights, page_table, lens, tokens, budget, *, starts=None, stamp
     tokens, budget = int(tokens), int(budget)
     if tokens <= 0:
         _refuse(f"{name}: tokens={tokens}")
+    _fits(name, tokens, budget, pages, kv, page, streams, most)
     _words(name, "lens", lens, (streams,))
     _words(name, "starts", starts, (streams + 1,))
     _words(name, "stamps", stamps, shape)

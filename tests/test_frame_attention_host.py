@@ -71,6 +71,15 @@ def test_rotary_refuses_types_alignment_and_overlap(lib):
     wide = dict(keys=None, q_token_stride=64, out_token_stride=64)
     assert lib.dc_rotary(rotary_args(p, out=p + 48 * 2, **wide), 1, None) == -3
     assert lib.dc_rotary(rotary_args(p, out=p + 16 * 2, **wide), 1, None) == -3
+    # the cache's write: out over k or v, anything over the cache, keys over values, rows of out over each other
+    apart = dict(k=p + 1024, v=p + 1024, keys=p + 4352, values=p + 6144, weights=p + 2048, stamps=p + 2048)  # a pool has 3 x 8 x 16 elements
+    for change, what in ((dict(out=p + 1024), b"out overlaps k"), (dict(out=p + 512, k=p + 256, v=p + 640), b"out overlaps k or v"),
+                         (dict(k=p + 4400), b"overlaps the cache"), (dict(keys=p + 64), b"overlaps the cache"), (dict(weights=p + 6144), b"overlaps the cache"),
+                         (dict(values=p + 4352), b"keys and values overlap")):
+        assert lib.dc_rotary(rotary_args(p, **{**apart, **change}), 1, None) == -3 and what in lib.dc_last_error(), change
+    assert lib.dc_rotary(rotary_args(p, keys=None, out_token_stride=16), 1, None) == -3
+    assert lib.dc_rotary(rotary_args(p, tokens=1 << 21, q_heads=1024), 1, None) == -3
+    assert lib.dc_last_kernels() == b""
 
 
 @pytest.mark.parametrize("change,code", [
@@ -96,6 +105,8 @@ def test_paged_attention_refuses_types_alignment_and_overlap(lib):
     assert lib.dc_paged_attention(attention_args(p, out=p + 4097), 1, None) == -5
     assert lib.dc_paged_attention(attention_args(p, out=p), 1, None) == -3
     assert lib.dc_paged_attention(attention_args(p, out=p + 64, keys=p + 2048, values=p + 2048), 1, None) == -3  # over q
+    assert lib.dc_paged_attention(attention_args(p, out_token_stride=16), 1, None) == -3  # rows of out over each other
+    assert lib.dc_paged_attention(attention_args(p, tokens=1 << 21, q_heads=1024), 1, None) == -3
     # a call that needs a workspace and has none, or too little
     big = dict(max_pages=4096, page_size=64, num_pages=1)
     need = lib.dc_paged_attention_workspace(attention_args(p, **big), 1)
@@ -145,6 +156,10 @@ def test_the_python_entry_points_refuse_host_tensors(lib):
     with pytest.raises(_lib.DeltaCNNError, match="even"):
         hk.rotary_frequencies((3, 4))
     assert hk.rotary_frequencies((4, 0, 2), base=100.0).tolist() == [1.0, 0.1, 1.0]
+    for bad in (1 << 31, -(1 << 31) - 1, 1 << 32):  # a field of the C interface would hold something else
+        with pytest.raises(_lib.DeltaCNNError, match="32 bits"):
+            hk._fits("paged_attention", 3, bad, 5)
+    hk._fits("paged_attention", (1 << 31) - 1, -(1 << 31))
     with pytest.raises(ValueError):
         from deltacnn_amd.sparse_layers import DCFrameAttention
         DCFrameAttention(64, 4, kv_heads=3)
