@@ -403,6 +403,15 @@ struct RowState {
         return lds_read<float>(vt + voff + (32 * b + 8 * (r / 4) + r % 4) * ROW + 128 * d);
     }
 
+    // .. of WORDS such slots from number `first` (16 b + r) on
+    template <int WORDS>
+    __device__ __forceinline__ void words(float (&w)[WORDS][DB], uint32_t vt, int first) const {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i)
+#pragma unroll
+            for (int d = 0; d < DB; ++d) w[i][d] = vword(vt, (first + i) / 16, (first + i) % 16, d);
+    }
+
     // Slots that some rows see and others do not may hold infinities or NaN, and 0 * inf would carry them
     // over: such elements leave the product and join the rows that see them one by one.
     static __device__ __forceinline__ uint32_t chunk_odd(chunk v) {
@@ -567,9 +576,13 @@ struct RowState {
             for (int t = 0; t < STEPS; ++t) s[b] = Chunk<E>::mma(kf[b & 1][t], q[t], s[b]);
         }
         chunk vf[2][sizeof(E) == 2 ? DB : 1];
+        constexpr int WORDS = sizeof(E) == 4 ? 16 / DB : 1;  // fp32: slots of a request
+        float vw[2][WORDS][DB];
         if constexpr (sizeof(E) == 2) {
 #pragma unroll
             for (int d = 0; d < DB; ++d) vf[0][d] = vfrag(vt, 0, d);
+        } else {
+            words<WORDS>(vw[0], vt, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
         const int half = lane_id() >> 5;
@@ -652,11 +665,15 @@ struct RowState {
                 return;
             }
 #pragma unroll
-            for (int b = 0; b < BLK; ++b)
+            for (int g = 0; g < 16 * BLK / WORDS; ++g) {
+                if (g + 1 < 16 * BLK / WORDS) words<WORDS>(vw[(g + 1) & 1], vt, (g + 1) * WORDS);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
+                for (int i = 0; i < WORDS; ++i)
 #pragma unroll
-                    for (int d = 0; d < DB; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vword(vt, b, r, d), s[b][r], o[d], 0, 0, 0);
+                    for (int d = 0; d < DB; ++d)
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vw[g & 1][i][d], s[(g * WORDS + i) / 16][(g * WORDS + i) % 16], o[d], 0, 0, 0);
+            }
         }
     }
 };
@@ -682,7 +699,7 @@ __device__ __forceinline__ const AttnCall &call_again() {
 //   blocks of keys and 4 of values; see pipeline().
 //   KEYS (few rows): the wavefronts own the same rows and blocks of 32 slots each in turn, two stages of
 //   their own, without a barrier between them, and join their sums at the end.
-//   NARROW: 2 wavefronts, for streams of at most 64 rows.
+//   NARROW: 2 wavefronts, for streams of at most 64 rows whose tiles leave no room for KEYS' four.
 //   else (fp32, whose products take sixteen times as long as anything beside them): 4 wavefronts own
 //   different rows and share two stages of 32 slots.
 template <typename E, int DP, bool KEYS, bool NARROW = false>
@@ -1187,8 +1204,24 @@ attention_join_kernel(AttnPlan p, AttnGrid g, T *__restrict__ out, float *__rest
     if (lane == 0 && lse != nullptr) lse[row] = l == 0.f ? -INFINITY : (ref + __builtin_amdgcn_logf(l)) * 0.693147180559945309f;
 }
 
+// Rows of a workgroup.  32 (KEYS) where a stream has no more, and, as long as four wavefronts' blocks have room in LDS
+// (rows of a tile up to 256 bytes), also up to 64 and where all the work is at most 28 blocks of 32 x 32 for each
+// wavefront of the card: fewer pieces, which end in shorter sums.  8 heads of 128 in bf16: 4 / 32 streams of 49
+// tokens over 4096 slots 23 / 106 us, with the narrow workgroups 25 / 115 us; one stream of 196 tokens over 4096 slots
+// (7 blocks) 21 us, with 128 rows 29 us; of 98 over 32640 (32 blocks) 44 us both; of 196 (56) 73 and 54 us.  64 in
+// fp32: 38 / 192 and 45 / 282 us; 30 and 36 us; 88 and 84 us; 165 and 144 us.  Rows of 512 bytes, two wavefronts a
+// workgroup in either form: 88 / 590 and 56 / 342 us for the first two.
+template <typename E>
+int block_rows(const AttnPlan &p) {
+    const int row_bytes = (p.dim <= 64 ? 64 : p.dim <= 128 ? 128 : 256) * int(sizeof(E));
+    const int64_t rows = int64_t(p.tokens) * p.group, streams = p.streams;
+    const int64_t work = ceil_div64(rows, 32 * streams) * streams * p.kv_heads * ceil_div64(int64_t(p.pool.max_pages) * p.pool.page_size, 32);
+    if (rows <= 32 * streams || (row_bytes <= 256 && (rows <= 64 * streams || work <= 28 * 1024))) return 32;
+    return rows <= 64 * streams ? 64 : 128;
+}
+
 // How the rows and the slots are divided.
-AttnGrid plan_grid(const AttnPlan &p, bool ragged, bool few, int bm) {
+AttnGrid plan_grid(const AttnPlan &p, bool ragged, int bm) {
     AttnGrid g = {};
     g.block_rows = bm;
     const int64_t rows = int64_t(p.tokens) * p.group;
@@ -1196,29 +1229,40 @@ AttnGrid plan_grid(const AttnPlan &p, bool ragged, bool few, int bm) {
     g.flat = ragged ? int(rows / bm) + p.streams : g.stream_blocks * p.streams;
     const int64_t cap = int64_t(p.pool.max_pages) * p.pool.page_size;
     const int64_t base = int64_t(g.flat) * p.kv_heads;
-    // pieces of the slot axis until two workgroups a compute unit are there, none below 128 slots
-    const int64_t want = 512, least = 128;
-    int64_t splits = base >= want ? 1 : ceil_div64(want, base);
-    int64_t keys = max(least, ceil_div64(ceil_div64(cap, splits), 128) * 128);
+    // Pieces of the slot axis until every compute unit has two workgroups, or one with few rows, whose LDS it
+    // takes (a token of 32 streams over 32640 slots: 146 us, with two 159 us and twice as much to join), and
+    // not more than are resident at once; none below 128 slots, in whole turns of a workgroup's blocks.
+    const bool few = bm == 32;
+    const int64_t want = few ? 256 : 512, least = 128, turn = few ? 128 : 32, per_xcd = want / 8;
+    int64_t splits = 1;
+    g.unit = 1;
+    if (base < want) {
+        // .. a unit of row blocks with the same slots on one XCD as a whole, as long as that leaves three quarters
+        // of the workgroups (392 rows over 32640 slots, one head of 128 in bf16: 13 row blocks in 16 pieces 24 us,
+        // in 19 pieces spread over all XCDs 38 us, or 8 to an XCD, some of which then get a second round, 37 us)
+        const int64_t most = want / base;
+        for (int k = 1; k <= g.stream_blocks; ++k) {
+            const int64_t unit = ceil_div64(g.stream_blocks, k), fit = 8 * (per_xcd / unit) / (ceil_div64(g.flat, unit) * p.kv_heads);
+            if (4 * fit < 3 * most && unit > 1) continue;
+            g.unit = int(unit);
+            splits = max(int64_t(1), fit);
+            break;
+        }
+    } else {
+        while (g.unit < 16 && g.unit * 2 <= g.flat && base >= 8 * 2 * g.unit * 2) g.unit *= 2;
+    }
+    const int64_t keys = max(least, ceil_div64(ceil_div64(cap, splits), turn) * turn);
     splits = ceil_div64(cap, keys);
     g.splits = int(splits);
     g.split_keys = int(keys);
-    const int64_t total = base * splits;
-    g.unit = 1;
-    while (g.unit < 16 && g.unit * 2 <= g.flat && total >= 8 * 2 * g.unit * 2) g.unit *= 2;
+    g.pairs = p.kv_heads * g.splits;
     g.by_group = FastDiv(uint32_t(p.group));
     g.by_unit = FastDiv(uint32_t(g.unit));
-    g.pairs = p.kv_heads * g.splits;
     g.by_pairs = FastDiv(uint32_t(g.pairs));
     g.by_blocks = FastDiv(uint32_t(max(1, g.stream_blocks)));
     g.by_kv = FastDiv(uint32_t(p.kv_heads));
     return g;
 }
-
-// Rows of a workgroup by those of a stream (of all streams on average): 32 a wavefront, which share theirs
-// where there are no more.
-bool few_rows(const AttnPlan &p) { return int64_t(p.tokens) * p.group <= int64_t(32) * p.streams; }
-int block_rows(const AttnPlan &p) { return few_rows(p) ? 32 : int64_t(p.tokens) * p.group <= int64_t(64) * p.streams ? 64 : 128; }
 
 int64_t part_bytes(const AttnPlan &p, const AttnGrid &g) {
     return g.splits > 1 ? int64_t(g.splits) * p.tokens * p.q_heads * (p.dim + 2) * 4 : 0;
@@ -1264,13 +1308,15 @@ hipError_t weights_go(const dc_attention_args &a, const AttnPlan &p, const AttnG
 }
 
 template <typename E, int DP, Pages PAGES>
-hipError_t attention_pages(const dc_attention_args &a, const AttnPlan &p, const AttnGrid &g, bool few, bool narrow, float *lse, hipStream_t s) {
-    if (few) return attention_go<E, DP, true, false, PAGES>(a, p, g, lse, s);
-    return narrow ? attention_go<E, DP, false, true, PAGES>(a, p, g, lse, s) : attention_go<E, DP, false, false, PAGES>(a, p, g, lse, s);
+hipError_t attention_pages(const dc_attention_args &a, const AttnPlan &p, const AttnGrid &g, float *lse, hipStream_t s) {
+    if (g.block_rows == 32) return attention_go<E, DP, true, false, PAGES>(a, p, g, lse, s);
+    if constexpr (DP * sizeof(E) > 256)
+        if (g.block_rows == 64) return attention_go<E, DP, false, true, PAGES>(a, p, g, lse, s);
+    return attention_go<E, DP, false, false, PAGES>(a, p, g, lse, s);
 }
 
 template <typename E, int DP>
-hipError_t attention_dp(const dc_attention_args &a, const AttnPlan &p, const AttnGrid &g, bool few, float *lse, hipStream_t s) {
+hipError_t attention_dp(const dc_attention_args &a, const AttnPlan &p, const AttnGrid &g, float *lse, hipStream_t s) {
     // Tiles start at multiples of 32: in pages of a multiple of 32 slots they touch one page, in larger ones two at
     // most, and two in pages of 16.  A token of 32 streams over 32640 slots, 128 elements, 16 bit: 156 us in ONE
     // (64 slots a page), 164 / 167 us in TWO and 337 / 318 us in MANY (49 / 16 slots), where a lane's look at the
@@ -1281,10 +1327,9 @@ hipError_t attention_dp(const dc_attention_args &a, const AttnPlan &p, const Att
                         : ps % 32 == 0                                                    ? ONE
                         : ps > 32 || ps == 16                                             ? TWO
                                                                                          : MANY;
-    const bool narrow = g.block_rows == 64;
-    hipError_t e = pages == ONE   ? attention_pages<E, DP, ONE>(a, p, g, few, narrow, lse, s)
-                   : pages == TWO ? attention_pages<E, DP, TWO>(a, p, g, few, narrow, lse, s)
-                                  : attention_pages<E, DP, MANY>(a, p, g, few, narrow, lse, s);
+    hipError_t e = pages == ONE   ? attention_pages<E, DP, ONE>(a, p, g, lse, s)
+                   : pages == TWO ? attention_pages<E, DP, TWO>(a, p, g, lse, s)
+                                  : attention_pages<E, DP, MANY>(a, p, g, lse, s);
     if (e == hipSuccess && g.splits > 1) {
         note_kernel("attention_join_kernel");
         attention_join_kernel<E><<<ceil_div(p.tokens * p.q_heads, 4), 256, 0, s>>>(p, g, (E *)a.out, lse, a.lens, a.starts);
@@ -1310,35 +1355,34 @@ AttnPlan make_plan(const dc_attention_args &a) {
 struct Room {
     int64_t part, lse;
 };
+template <typename E>
 Room room(const dc_attention_args &a) {
     const AttnPlan p = make_plan(a);
     Room r = {0, 0};
-    const bool few = few_rows(p);
-    r.part = part_bytes(p, plan_grid(p, a.starts != nullptr, few, block_rows(p)));
+    r.part = part_bytes(p, plan_grid(p, a.starts != nullptr, block_rows<E>(p)));
     if (a.weights != nullptr && a.lse == nullptr) r.lse = int64_t(a.tokens) * a.q_heads * 4;
     return r;
 }
 
 template <typename E>
 hipError_t attention_t(const dc_attention_args &a, AttnPlan p, hipStream_t s) {
-    const Room r = room(a);
+    const Room r = room<E>(a);
     float *lse = a.lse != nullptr || a.weights == nullptr ? a.lse : (float *)((char *)a.workspace + r.part);
-    const bool few = few_rows(p);
-    AttnGrid g = plan_grid(p, a.starts != nullptr, few, block_rows(p));
+    AttnGrid g = plan_grid(p, a.starts != nullptr, block_rows<E>(p));
     g.part = (float *)a.workspace;
     // exponentials are powers of two; with a negative scale q changes its signs instead, so that the largest
     // product has the largest score
     p.flip = p.scale < 0.f ? sizeof(E) == 2 ? 0x80008000u : 0x80000000u : 0u;
     // (a scale of zero: as good as zero, but -inf times it stays -inf)
     p.scale = fmaxf(fabsf(p.scale) * 1.44269504088896341f, 1.2e-38f);
-    return p.dim <= 64 ? attention_dp<E, 64>(a, p, g, few, lse, s) : p.dim <= 128 ? attention_dp<E, 128>(a, p, g, few, lse, s)
-                                                                                 : attention_dp<E, 256>(a, p, g, few, lse, s);
+    return p.dim <= 64 ? attention_dp<E, 64>(a, p, g, lse, s) : p.dim <= 128 ? attention_dp<E, 128>(a, p, g, lse, s)
+                                                                                 : attention_dp<E, 256>(a, p, g, lse, s);
 }
 
 }  // namespace
 
-int64_t paged_attention_workspace(const dc_attention_args &a) {
-    const Room r = room(a);
+int64_t paged_attention_workspace(const dc_attention_args &a, int dtype) {
+    const Room r = dtype == DC_F32 ? room<float>(a) : room<half_t>(a);
     return r.part + r.lse;
 }
 

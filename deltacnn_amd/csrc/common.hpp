@@ -431,7 +431,7 @@ hipError_t launch_linear(const void *x, const void *w, const void *bias, void *o
 // Attention over a paged cache of earlier frames (arguments already validated).
 hipError_t launch_rotary(const dc_rotary_args &a, int dtype, hipStream_t s);
 hipError_t launch_paged_attention(const dc_attention_args &a, int dtype, hipStream_t s);
-int64_t paged_attention_workspace(const dc_attention_args &a);
+int64_t paged_attention_workspace(const dc_attention_args &a, int dtype);
 hipError_t launch_cache_slots(const dc_slots_args &a, hipStream_t s);
 int64_t cache_slots_workspace(const dc_slots_args &a);
 

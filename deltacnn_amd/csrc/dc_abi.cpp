@@ -1105,7 +1105,7 @@ int dc_rotary(const dc_rotary_args *a, int dtype, void *stream) {
 
 int64_t dc_paged_attention_workspace(const dc_attention_args *a, int dtype) {
     int rc = check_attention(a, dtype);
-    return rc != DC_OK ? rc : dc::paged_attention_workspace(*a);
+    return rc != DC_OK ? rc : dc::paged_attention_workspace(*a, dtype);
 }
 
 int dc_paged_attention(const dc_attention_args *a, int dtype, void *stream) {
@@ -1133,7 +1133,7 @@ int dc_paged_attention(const dc_attention_args *a, int dtype, void *stream) {
     if ((rc = check_apart(fn, "out", a->tokens, a->q_heads, a->dim, a->out_token_stride, a->out_head_stride)) != DC_OK) return rc;
     if (out.meets(q) || out.meets(Span(a->keys, pool)) || out.meets(Span(a->values, pool)))
         return fail(DC_ERR_UNSUPPORTED, "%s: out overlaps an operand", fn);
-    const int64_t need = dc::paged_attention_workspace(*a);
+    const int64_t need = dc::paged_attention_workspace(*a, dtype);
     if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need))
         return fail(DC_ERR_NULL, "%s: needs %lld bytes of workspace", fn, (long long)need);
     if (need > 0) DC_REQUIRE_ALIGNED("dc_paged_attention", a->workspace, 16);
