@@ -238,7 +238,10 @@ struct TileLoader {
     bool bad = false;
     // ONE, TWO: bytes of a lane from the tile's first element; the tile to be found next: its page (ONE, `fresh`:
     // not looked at yet) and the one behind it, the bytes in front in the pool, its place inside
-    uint32_t koffset[REQ], voffset[REQ], page_bytes, row_bytes;
+    // Bytes of every request in registers, or (long rows, whose sums need them) formed when it goes out: a token of 8
+    // streams over 4096 slots, 8 heads of 256, bf16 148 -> 42 us, fp32 1125 -> 424 us.
+    static constexpr bool KEPT = REQ <= 8;
+    uint32_t koffset[KEPT ? REQ : 1], voffset[KEPT ? REQ : 1], page_bytes, row_bytes;
     int index, inside, page, behind;
     uint64_t page_at;
     bool fresh, lost;
@@ -254,14 +257,21 @@ struct TileLoader {
             index = uniform(p.pool.by_page.quot(uint32_t(k0)));
             inside = uniform(k0 - index * page_size);
             page = behind = 0, page_at = 0, fresh = true, lost = false;
-            const int c = lane_id() % CPR, row0 = loader * REQ * RPI + lane_id() / CPR;
+            if constexpr (KEPT) {
 #pragma unroll
-            for (int j = 0; j < REQ; ++j) {
-                const int row = row0 + j * RPI, ck = c ^ key_swizzle<E, DP>(row), cv = c ^ value_swizzle<E, DP>(row);
-                koffset[j] = ck * N < dim ? uint32_t(row * dim + ck * N) * sizeof(E) : NOWHERE;
-                voffset[j] = cv * N < dim ? uint32_t(row * dim + cv * N) * sizeof(E) : NOWHERE;
+                for (int j = 0; j < REQ; ++j) koffset[j] = form<false>(lane_id(), loader, j), voffset[j] = form<true>(lane_id(), loader, j);
             }
         }
+    }
+    template <bool VALUES>
+    __device__ __forceinline__ uint32_t form(int lane, int loader, int j) const {
+        const int row = loader * REQ * RPI + lane / CPR + j * RPI, c = lane % CPR ^ (VALUES ? value_swizzle<E, DP>(row) : key_swizzle<E, DP>(row));
+        return c * N < dim ? uint32_t(row) * row_bytes + uint32_t(c) * 16 : NOWHERE;
+    }
+    template <bool VALUES>
+    __device__ __forceinline__ uint32_t offset(int lane, int loader, int j) const {
+        if constexpr (KEPT) return VALUES ? voffset[j] : koffset[j];
+        else return form<VALUES>(lane, loader, j);
     }
     // The pages of the next tile, which starts at slot k, a step ahead of its request.  (Nothing writes the table
     // meanwhile: scalar loads, which the counted waits do not see.)
@@ -325,26 +335,28 @@ struct TileLoader {
     template <bool VALUES>
     __device__ __forceinline__ void request(const Place &x, int loader, uint32_t to) {
         const E *from = VALUES ? values : keys;
-        const int row0 = loader * REQ * RPI + lane_id() / CPR;
+        int lane = lane_id();
+        if constexpr (!KEPT) asm volatile("" : "+v"(lane));  // .. formed anew each time
+        const int row0 = loader * REQ * RPI + lane / CPR;
         if constexpr (PAGES == ONE) {
             const uint64_t a = uint64_t(uintptr_t(from)) + x.at;
             u32x4_t r;
             r[0] = uniform(uint32_t(a)), r[1] = uniform(uint32_t(a >> 32)), r[2] = uniform(x.bytes), r[3] = 0x00027000u;  // addresses have 48 bits
 #pragma unroll
-            for (int j = 0; j < REQ; ++j) fetch_bounded(r, VALUES ? voffset[j] : koffset[j], to + j * 1024);
+            for (int j = 0; j < REQ; ++j) fetch_bounded(r, offset<VALUES>(lane, loader, j), to + j * 1024);
         } else if constexpr (PAGES == TWO) {
             const uint64_t zero = uint64_t(uintptr_t(&zero_chunk)), a = uint64_t(uintptr_t(from)) + x.at, b = uint64_t(uintptr_t(from)) + x.at_behind;
 #pragma unroll
             for (int j = 0; j < REQ; ++j) {
                 const int row = row0 + j * RPI;
-                const uint32_t offset = VALUES ? voffset[j] : koffset[j];
-                const bool over = row >= x.seam, in = row < (over ? x.rows_behind : x.rows) && offset != NOWHERE;
-                const uint64_t at = (over ? b : a) + offset;
+                const uint32_t bytes = offset<VALUES>(lane, loader, j);
+                const bool over = row >= x.seam, in = row < (over ? x.rows_behind : x.rows) && bytes != NOWHERE;
+                const uint64_t at = (over ? b : a) + bytes;
                 fetch(reinterpret_cast<const void *>(uintptr_t(in ? at : zero)), to + j * 1024);
             }
         } else {
             const E *zero = reinterpret_cast<const E *>(&zero_chunk);
-            const int c = lane_id() % CPR;
+            const int c = lane % CPR;
 #pragma unroll
             for (int j = 0; j < REQ; ++j) {
                 const int row = row0 + j * RPI, e = (c ^ (VALUES ? value_swizzle<E, DP>(row) : key_swizzle<E, DP>(row))) * N;
@@ -559,21 +571,38 @@ struct RowState {
         // LDS answers after some hundred cycles, three products' time: a block's operands are requested in one
         // go, those of the next block before the products of this one, and the first values before the
         // exponentials (left to itself the compiler asks for two operands at a time and waits for each)
+        // (fp32: a chunk's products take longer than that, so four on their way are enough, and their registers go to
+        // the sums: 1568 rows of 64 heads of 128 / 256 over 4096 slots 2.25 -> 1.97 / 19.3 -> 8.7 ms)
         float16_t s[BLK];
-        chunk kf[2][STEPS];
+        if constexpr (sizeof(E) == 4) {
+            static_assert(BLK == 1 && STEPS >= 4, "one block");
+            chunk kf[4];
 #pragma unroll
-        for (int t = 0; t < STEPS; ++t) kf[0][t] = kfrag(kt, 0, t);
+            for (int t = 0; t < 4; ++t) kf[t] = kfrag(kt, 0, t);
 #pragma unroll
-        for (int b = 0; b < BLK; ++b) {
-            if (b + 1 < BLK) {
+            for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
 #pragma unroll
-                for (int t = 0; t < STEPS; ++t) kf[(b + 1) & 1][t] = kfrag(kt, b + 1, t);
+            for (int t = 0; t < STEPS; ++t) {
+                __builtin_amdgcn_sched_barrier(0);
+                s[0] = Chunk<E>::mma(kf[t & 3], q[t], s[0]);
+                if (t + 4 < STEPS) kf[t & 3] = kfrag(kt, 0, t + 4);
             }
-            __builtin_amdgcn_sched_barrier(0);
+        } else {
+            chunk kf[2][STEPS];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[b][r] = 0.f;
+            for (int t = 0; t < STEPS; ++t) kf[0][t] = kfrag(kt, 0, t);
 #pragma unroll
-            for (int t = 0; t < STEPS; ++t) s[b] = Chunk<E>::mma(kf[b & 1][t], q[t], s[b]);
+            for (int b = 0; b < BLK; ++b) {
+                if (b + 1 < BLK) {
+#pragma unroll
+                    for (int t = 0; t < STEPS; ++t) kf[(b + 1) & 1][t] = kfrag(kt, b + 1, t);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[b][r] = 0.f;
+#pragma unroll
+                for (int t = 0; t < STEPS; ++t) s[b] = Chunk<E>::mma(kf[b & 1][t], q[t], s[b]);
+            }
         }
         chunk vf[2][sizeof(E) == 2 ? DB : 1];
         constexpr int WORDS = sizeof(E) == 4 ? 16 / DB : 1;  // fp32: slots of a request
@@ -634,9 +663,7 @@ struct RowState {
 #pragma unroll
                     for (int t = 0; t < 2; ++t)
 #pragma unroll
-                        for (int d = 0; d < DB; ++d) {
-                            o[d] = Chunk<E>::mma(chunk_even(vfrag(vt, 2 * b + t, d)), pr[b][t], o[d]);
-                        }
+                        for (int d = 0; d < DB; ++d) o[d] = Chunk<E>::mma(chunk_even(vfrag(vt, 2 * b + t, d)), pr[b][t], o[d]);
                 add_odd(vt, k0, limit);
                 return;
             }
@@ -709,7 +736,9 @@ struct Shape {
     static constexpr int NW = !KEYS ? NARROW ? 2 : 4 : ROW <= 256 ? 4 : ROW <= 512 ? 2 : 1;
     static constexpr int TILES = PIPE ? 7 * TILE : 4 * TILE * (KEYS ? NW : 1), JOIN = KEYS ? NW * 32 * (DP + 6) * 4 : 0;
     static constexpr int LDS = TILES > JOIN ? TILES : JOIN;
-    static constexpr int GROUPS = LDS <= 79 << 10 && ROW <= 256 ? 2 : 1;  // workgroups a compute unit is to hold
+    // workgroups a compute unit is to hold (fp32 rows of 512 bytes: two, though some registers spill, 510 us instead of
+    // 568 us for 392 rows of 64 heads over 4096 slots, but one of the narrow ones, 82 instead of 130 us for 49 rows)
+    static constexpr int GROUPS = LDS <= 79 << 10 && ROW <= (sizeof(E) == 4 && !NARROW ? 512 : 256) ? 2 : 1;
 };
 
 // Attention on the matrix cores.  A wavefront owns 32 rows.
