@@ -26,6 +26,15 @@ def make_pool(gen, streams, slots, kv, page, dim, dtype, spare=3):
     return keys, values, weights, stamps, table
 
 
+def widened(table, page, tokens, heads, kv):
+    """The same pages in a table with room for so many slots that a workgroup takes 128 rows, where a stream has more than 64."""
+    streams = table.shape[0]
+    blocks = -(-tokens * (heads // kv) // (32 * streams)) * streams * kv
+    wide = torch.full((streams, max(table.shape[1], -(-29 * 1024 * 32 // (blocks * page)))), -12345, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    return wide
+
+
 def poison_unused(keys, values, weights, table, lens, page):
     """NaN wherever no stream has a slot in use."""
     used = torch.zeros(keys.shape[0], page, dtype=torch.bool)
@@ -235,6 +244,57 @@ def test_paged_attention(lib, dtype, shape):
     ref.assert_within(w, want0, tol0, "weights, decay 0")
 
 
+MANY = [  # the same, more than 64 rows a stream; the page table has room for so much that a workgroup takes 128 rows
+    ([130], [130], 2, 2, 64, 64, 1),
+    ([130], [100], 2, 1, 64, 64, 1),
+    ([300], [700], 2, 2, 128, 64, 0),
+    ([150], [333], 3, 1, 40, 33, 30),
+    ([200, 90, 170], [205, 400, 31], 4, 2, 72, 49, 7),
+    ([100, 100], [256, 256], 4, 4, 128, 16, 25),
+    ([95], [200], 1, 1, 96, 20, 0),
+    ([270], [1], 1, 1, 64, 1, 0),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("shape", MANY, ids=str)
+def test_paged_attention_many_rows(lib, dtype, shape):
+    from deltacnn_amd import hip_kernels as hk
+    counts, lens, heads, kv, dim, page, block = shape
+    gen = torch.Generator().manual_seed(2000 + sum(counts) + sum(lens))
+    tokens, streams = sum(counts), len(counts)
+    keys, values, weights, _, table = make_pool(gen, streams, max(max(lens), 1) + page, kv, page, dim, dtype)
+    poison_unused(keys, values, weights, table, lens, page)
+    q = (1.5 * torch.randn(tokens, heads, dim, generator=gen)).to(dtype)
+    ragged, starts = len(set(counts)) > 1, starts_of(counts)
+    for b, n in enumerate(lens):
+        table[b, -(-n // page):] = -12345
+    wide = widened(table, page, tokens, heads, kv)
+    lens_t = torch.tensor(lens, dtype=torch.int32)
+    out, tol, lse, lse_tol, ww, w_tol = ref.attention(q, keys, values, wide, lens_t, starts, None, block, weights, 0.75)
+    w = weights.to(DEV)
+    got, got_lse = hk.paged_attention(*(t.to(DEV) for t in (q, keys, values, wide, lens_t)), starts=starts.to(DEV) if ragged else None,
+                                      causal_block=block, weights=w, decay=0.75, return_lse=True)
+    ref.assert_within(got, out, tol, "out")
+    ref.assert_within(got_lse, lse, lse_tol, "lse")
+    ref.assert_within(w, ww, w_tol, "weights")
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.float32, 64), (torch.float16, 64), (torch.bfloat16, 128)], ids=str)
+def test_paged_attention_many_rows_in_pieces(lib, dtype, dim):
+    """So long a cache that 128 rows of it are joined from several pieces."""
+    from deltacnn_amd import hip_kernels as hk
+    gen = torch.Generator().manual_seed(31)
+    tokens, heads, page, n = 260, 8, 64, 13000
+    keys, values, _, _, table = make_pool(gen, 1, n, heads, page, dim, dtype)
+    q = (1.5 * torch.randn(tokens, heads, dim, generator=gen)).to(dtype)
+    lens_t = torch.tensor([n], dtype=torch.int32)
+    out, tol, lse, lse_tol, _, _ = ref.attention(q, keys, values, table, lens_t)
+    got, got_lse = hk.paged_attention(*(t.to(DEV) for t in (q, keys, values, table, lens_t)), return_lse=True)
+    ref.assert_within(got, out, tol, "out")
+    ref.assert_within(got_lse, lse, lse_tol, "lse")
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids)
 @pytest.mark.parametrize("scale", [-0.2, 0.0, 3.0])
 @pytest.mark.parametrize("tokens", [2, 70])
@@ -261,8 +321,8 @@ def test_paged_attention_scales(lib, dtype, scale, tokens):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids)
-@pytest.mark.parametrize("tokens", [3, 150])
-def test_paged_attention_masked_infinities(lib, dtype, tokens):
+@pytest.mark.parametrize("tokens,wide", [(3, False), (150, False), (150, True)])
+def test_paged_attention_masked_infinities(lib, dtype, tokens, wide):
     """Infinities and NaN in keys and values that a row does not see leave it alone; rows that see
     them get what the definition says."""
     from deltacnn_amd import hip_kernels as hk
@@ -270,6 +330,7 @@ def test_paged_attention_masked_infinities(lib, dtype, tokens):
     dim, page, past = 64, 32, 20
     n = past + tokens
     keys, values, weights, _, table = make_pool(gen, 1, n, 1, page, dim, dtype)
+    table = widened(table, page, tokens, 1, 1) if wide else table
     bad = n - max(1, tokens // 2)  # seen by the later rows alone
     pg, off = ref.place(table[0], bad, page)
     values[pg, 0, off, 3], values[pg, 0, off, 40], values[pg, 0, off, 41] = math.nan, math.inf, -math.inf
@@ -292,14 +353,15 @@ def test_paged_attention_masked_infinities(lib, dtype, tokens):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids)
-@pytest.mark.parametrize("tokens", [1, 3, 70])
+@pytest.mark.parametrize("tokens,wide", [(1, False), (3, False), (70, False), (70, True)])
 @pytest.mark.parametrize("block", [0, 1])
-def test_paged_attention_visible_infinity(lib, dtype, tokens, block):
+def test_paged_attention_visible_infinity(lib, dtype, tokens, wide, block):
     """A key that gives every row a score of -inf: as if the slot were not there, and no weight for it."""
     from deltacnn_amd import hip_kernels as hk
     gen = torch.Generator().manual_seed(15)
     dim, page, n, bad = 64, 32, 400, 127
     keys, values, weights, _, table = make_pool(gen, 1, n, 1, page, dim, dtype)
+    table = widened(table, page, tokens, 2, 1) if wide else table
     q = torch.randn(tokens, 2, dim, generator=gen).to(dtype)
     q[:, :, 0] = q[:, :, 0].abs() + 0.5
     lens_t = torch.tensor([n], dtype=torch.int32)
@@ -322,14 +384,16 @@ def test_paged_attention_visible_infinity(lib, dtype, tokens, block):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("tokens,page", [(2, 32), (2, 20), (80, 64), (80, 20), (2, 48), (80, 48), (2, 16), (80, 16)])
-def test_paged_attention_lost_page_and_rows_behind(lib, dtype, tokens, page):
+def test_paged_attention_lost_page_and_rows_behind(lib, dtype, tokens, page, wide):
     """A page outside the pool makes its own stream NaN and no other; rows behind the last stream stay."""
     from deltacnn_amd import hip_kernels as hk
     gen = torch.Generator().manual_seed(3)
     dim, lens = 32, [90, 130, 41]
     keys, values, weights, _, table = make_pool(gen, 3, 140, 1, page, dim, dtype)
     table[1, 1] = keys.shape[0] if page > 20 else -1
+    table = widened(table, page, 3 * tokens, 2, 1) if wide else table
     counts = [tokens, tokens, tokens - 1]
     starts = starts_of(counts)
     total = sum(counts) + 4
