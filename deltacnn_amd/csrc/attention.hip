@@ -4,6 +4,14 @@
 //   m' = max(m, s),  l' = l e^(m - m') + sum e^(s - m'),  o' = o e^(m - m') + sum e^(s - m') v.
 // The attention that a slot receives needs the finished log-sum of every row, so it is a second
 // launch: weight[s] = decay weight[s] + sum over rows of e^(s - lse).
+//
+// What bounds it, and what it reaches (MI355X; a large copy moves 5.2 TB/s, a large matrix product makes 1200 TFLOP/s in
+// bf16 and 150 in fp32):
+//   a token of 32 streams over 1 .. 32640 slots, 2 kv heads of 128, bf16: reading the cache; 146 + 6 us, 5.7 TB/s
+//   12240 tokens in 24 frames, 16 query and 4 kv heads of 128, bf16: the matrix cores; 630 us, 1.0 PFLOP/s
+//   510 tokens over 32640 slots, the same heads: the matrix cores; 148 us, joining 10 us, weights 107 us
+//   64 tokens of 4 streams over 4096 slots, 8 heads of 64, fp32: the matrix cores; 29 + 5 us, weights 22 us
+//   49 tokens over 3136 slots, 20 query and 4 kv heads of 64: its launches and the way through one tile; 9 + 5 us
 #include "cache.hpp"
 
 namespace dc {
@@ -723,8 +731,8 @@ __device__ __forceinline__ const AttnCall &call_again() {
 
 // How a workgroup goes about its slots.
 //   PIPE (16-bit types, many rows): 4 wavefronts own different rows and share blocks of 32 slots, rings of 3
-//   blocks of keys and 4 of values; see pipeline().
-//   KEYS (few rows): the wavefronts own the same rows and blocks of 32 slots each in turn, two stages of
+//   blocks of keys and 4 of values; see RowState::turn().
+//   KEYS (few rows, or little work): the wavefronts own the same rows and blocks of 32 slots each in turn, two stages of
 //   their own, without a barrier between them, and join their sums at the end.
 //   NARROW: 2 wavefronts, for streams of at most 64 rows whose tiles leave no room for KEYS' four.
 //   else (fp32, whose products take sixteen times as long as anything beside them): 4 wavefronts own
@@ -985,10 +993,15 @@ attention_mfma_kernel(AttnCall call) {
 }
 
 // The attention that slots receive, once every row's log-sum is known.  A wavefront keeps the keys of
-// 32 NB slots in registers as the first operand and walks over all rows of its stream and head, tiles
+// 32 slots in registers as the first operand and walks over all rows of its stream and head, tiles
 // of 64 at a time through LDS; a lane's scores are those of one row, so its sums over the rows stay
 // in place until the end, where the lanes of a half are added up in a fixed order.
-template <typename E, int DP, int NB>
+//
+// Bound by its vector work: an exponential, a multiplication and two sums for every score take as long as the
+// score's product.  2040 rows x 32640 slots x 4 heads of 128, bf16: 107 us, 0.64 PFLOP/s.  (64 slots a
+// wavefront, half of the reads from LDS: 109 us there, 455 instead of 437 us for 8 streams over 16320 slots, and
+// 1300 instead of 650 us for 8192 tokens in frames of 512, where the workgroups of the first slots have most rows.)
+template <typename E, int DP>
 __global__ void __launch_bounds__(256, DP * sizeof(E) <= 256 ? 2 : 1)
 attention_weights_kernel(AttnPlan p, FastDiv by_group, const E *__restrict__ q, const float *__restrict__ lse,
                          const E *__restrict__ keys, float *__restrict__ weights, const int32_t *__restrict__ lens,
@@ -999,22 +1012,20 @@ attention_weights_kernel(AttnPlan p, FastDiv by_group, const E *__restrict__ q, 
     extern __shared__ __attribute__((aligned(1024))) char lds[];  // whole rows of any tile: see kfrag()
     const int b = blockIdx.z, h = blockIdx.y, len = uniform(stream_len(p, lens, b));
     const int lane = lane_id(), wv = wave_id(), half = lane >> 5, col = lane & 31;
-    const int s_block = blockIdx.x * (4 * 32 * NB), s0 = s_block + wv * 32 * NB;
+    const int s_block = blockIdx.x * (4 * 32), s0 = s_block + wv * 32;
     if (s_block >= len) return;
     int first, count;
     stream_tokens(starts, b, p.streams, p.tokens, first, count);
     const int32_t *table = p.pool.table + int64_t(b) * p.pool.max_pages;
-    chunk k[NB][STEPS];
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-        const int s = s0 + 32 * i + col;
-        const int64_t row = s < len ? slot_row(p.pool, table, s, p.kv_heads, h) : -1;
+    chunk k[STEPS];
+    {
+        const int64_t row = s0 + col < len ? slot_row(p.pool, table, s0 + col, p.kv_heads, h) : -1;
 #pragma unroll
         for (int t = 0; t < STEPS; ++t) {
             const int e = (2 * t + half) * N;
             uint4 u = make_uint4(0, 0, 0, 0);
             if (row >= 0 && e < p.dim) u = *reinterpret_cast<const uint4 *>(keys + row * p.dim + e);
-            k[i][t] = __builtin_bit_cast(chunk, u);
+            k[t] = __builtin_bit_cast(chunk, u);
         }
     }
     // the first token that sees this workgroup's first slot
@@ -1060,11 +1071,9 @@ attention_weights_kernel(AttnPlan p, FastDiv by_group, const E *__restrict__ q, 
         }
     };
     const float scale = p.flip != 0 ? -p.scale : p.scale;
-    float16_t acc[NB];
+    float16_t acc;
 #pragma unroll
-    for (int i = 0; i < NB; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
+    for (int r = 0; r < 16; ++r) acc[r] = 0.f;
     // this lane's row of a tile: its log-sum (-inf: no row, or one that sees nothing) and what it sees
     struct Row {
         float lse;
@@ -1090,31 +1099,23 @@ attention_weights_kernel(AttnPlan p, FastDiv by_group, const E *__restrict__ q, 
         for (int t = 0; t < STEPS; ++t) qf[t] = lds_read<chunk>((qt + col * ROW + ((half ^ key_swizzle<E, DP>(col)) << 4)) ^ (t << 5));
         __builtin_amdgcn_sched_barrier(0);  // all requested before anything else
     };
-    auto scores = [&](float16_t(&s)[NB]) {
+    auto scores = [&](float16_t &s) {
 #pragma unroll
-        for (int i = 0; i < NB; ++i)
+        for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[i][r] = 0.f;
-#pragma unroll
-        for (int t = 0; t < STEPS; ++t)
-#pragma unroll
-            for (int i = 0; i < NB; ++i) s[i] = Chunk<E>::mma(k[i][t], qf[t], s[i]);
+        for (int t = 0; t < STEPS; ++t) s = Chunk<E>::mma(k[t], qf[t], s);
     };
-    auto add = [&](const float16_t(&s)[NB], Row x, bool whole) {
+    auto add = [&](const float16_t &s, Row x, bool whole) {
         const float less = x.lse == -INFINITY ? -INFINITY : x.lse * -1.44269504088896341f;
         if (whole) {
 #pragma unroll
-            for (int i = 0; i < NB; ++i)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) acc[i][r] += __builtin_amdgcn_exp2f(fmaf(s[i][r], scale, less));
+            for (int r = 0; r < 16; ++r) acc[r] += __builtin_amdgcn_exp2f(fmaf(s[r], scale, less));
         } else {
 #pragma unroll
-            for (int i = 0; i < NB; ++i)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const float e = __builtin_amdgcn_exp2f(fmaf(s[i][r], scale, less));
-                    acc[i][r] += s0 + 32 * i + 8 * (r / 4) + 4 * half + r % 4 < x.limit ? e : 0.f;
-                }
+            for (int r = 0; r < 16; ++r) {
+                const float e = __builtin_amdgcn_exp2f(fmaf(s[r], scale, less));
+                acc[r] += s0 + 8 * (r / 4) + 4 * half + r % 4 < x.limit ? e : 0.f;
+            }
         }
     };
     if (r_first < rows) {
@@ -1134,10 +1135,10 @@ attention_weights_kernel(AttnPlan p, FastDiv by_group, const E *__restrict__ q, 
 #pragma unroll
             for (int i = 0; i < BM / 32; ++i) y[i] = next_row(i);
             // (no row behind the last: its scores are zeros, or NaN of an infinite key that gives a real row a weight of 0)
-            const bool whole = r0 + BM <= rows && s0 + 32 * NB <= visible(len, count, int(by_group.quot(uint32_t(r0))), p.causal_block);
+            const bool whole = r0 + BM <= rows && s0 + 32 <= visible(len, count, int(by_group.quot(uint32_t(r0))), p.causal_block);
 #pragma unroll
             for (int i = 0; i < BM / 32; ++i) {
-                float16_t s[NB];
+                float16_t s;
                 scores(s);
                 if (i + 1 < BM / 32) rows_of(place + stage * TILE + 32 * (i + 1) * ROW);  // in time for the exponentials
                 add(s, x[i], whole);
@@ -1148,21 +1149,20 @@ attention_weights_kernel(AttnPlan p, FastDiv by_group, const E *__restrict__ q, 
     // sums over the 32 lanes of a half; lane `col` keeps sum number `col`
     float mine = 0.f;
 #pragma unroll
-    for (int i = 0; i < NB; ++i)
+    for (int r = 0; r < 16; ++r) {
+        float x = acc[r];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            float x = acc[i][r];
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) x += __shfl_xor(x, d, WAVE);
-            if (col == 16 * i + r) mine = x;
-        }
-    const int i = col >> 4, r = col & 15, s = s0 + 32 * i + 8 * (r / 4) + 4 * half + r % 4;
-    if (i >= NB || s >= len) return;
+        for (int d = 1; d < 32; d <<= 1) x += __shfl_xor(x, d, WAVE);
+        if (col == r) mine = x;
+    }
+    const int s = s0 + 8 * (col / 4) + 4 * half + col % 4;
+    if (col >= 16 || s >= len) return;
     const int64_t row = slot_row(p.pool, table, s, p.kv_heads, h);
     if (row >= 0) weights[row] = p.decay == 0.f ? mine : fmaf(p.decay, weights[row], mine);
 }
 
-// Joins the pieces of the slot axis: one wavefront per row.
+// Joins the pieces of the slot axis: one wavefront per row, a lane per piece for the maxima, then 16 lanes for each
+// of four pieces.  Bound by its launch and three dependent trips to memory: 4 .. 6 us up to 2000 rows.
 template <typename T>
 __global__ void __launch_bounds__(256)
 attention_join_kernel(AttnPlan p, AttnGrid g, T *__restrict__ out, float *__restrict__ lse, const int32_t *__restrict__ lens,
@@ -1322,14 +1322,14 @@ hipError_t attention_go(const dc_attention_args &a, const AttnPlan &p, const Att
     return hipGetLastError();
 }
 
-template <typename E, int DP, int NB>
+template <typename E, int DP>
 hipError_t weights_go(const dc_attention_args &a, const AttnPlan &p, const AttnGrid &g, const float *lse, hipStream_t s) {
-    auto kernel = attention_weights_kernel<E, DP, NB>;
+    auto kernel = attention_weights_kernel<E, DP>;
     constexpr int BM = DP * sizeof(E) <= 512 ? 64 : 32, LDS = 2 * BM * DP * int(sizeof(E));
     static thread_local uint64_t raised = 0;
     const hipError_t err = raise_lds((const void *)kernel, LDS, raised);
     if (err != hipSuccess) return err;
-    const int64_t blocks = ceil_div64(int64_t(a.max_pages) * a.page_size, 128 * NB);
+    const int64_t blocks = ceil_div64(int64_t(a.max_pages) * a.page_size, 128);
     note_kernel("attention_weights_kernel");
     kernel<<<dim3(uint32_t(blocks), p.kv_heads, p.streams), 256, LDS, s>>>(p, g.by_group, (const E *)a.q, lse, (const E *)a.keys, a.weights,
                                                                            a.lens, a.starts);
@@ -1365,9 +1365,7 @@ hipError_t attention_dp(const dc_attention_args &a, const AttnPlan &p, const Att
         e = hipGetLastError();
     }
     if (e != hipSuccess || a.weights == nullptr) return e;
-    // 64 slots a wavefront where that leaves a workgroup and more for every compute unit
-    const bool wide = ceil_div64(int64_t(a.max_pages) * a.page_size, 256) * p.kv_heads * p.streams >= 512;
-    return wide ? weights_go<E, DP, 2>(a, p, g, lse, s) : weights_go<E, DP, 1>(a, p, g, lse, s);
+    return weights_go<E, DP>(a, p, g, lse, s);
 }
 
 AttnPlan make_plan(const dc_attention_args &a) {
