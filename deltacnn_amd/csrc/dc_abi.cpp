@@ -985,7 +985,8 @@ struct RowSet {
     int64_t token_stride, head_stride;
     int dtype;
     Span span() const { return Span(p, rows_span(tokens, heads, dim, token_stride, head_stride, dtype)); }
-    int64_t width() const { return (heads - 1) * head_stride + dim; }
+    // of the columns that a token takes; heads that lie whole tokens apart share theirs
+    int64_t width() const { return heads > 1 && head_stride % token_stride != 0 ? (heads - 1) * head_stride + dim : dim; }
     bool meets(const RowSet &o) const {
         if (!span().meets(o.span())) return false;
         if (token_stride != o.token_stride) return true;

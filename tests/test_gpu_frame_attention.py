@@ -187,6 +187,32 @@ def test_rotary_append(lib, dtype, shape):
     assert torch.equal(d["stamps"].cpu(), ws2)
 
 
+@pytest.mark.parametrize("outer", ["tokens", "heads"])
+def test_rotary_append_in_place_of_a_fused_projection(lib, outer):
+    """q, k and v are columns of one buffer, token by token or head by head, and q is turned in place: the
+    same as with tensors of their own, and k and v stay."""
+    from deltacnn_amd import hip_kernels as hk
+    gen = torch.Generator().manual_seed(41)
+    tokens, heads, dim, page = 21, 3, 16, 8
+    own = [torch.randn(tokens, heads, dim, generator=gen).half().to(DEV) for _ in range(3)]
+    if outer == "tokens":
+        fused = torch.cat(own, 1)
+        q, k, v = fused.split(heads, 1)
+    else:
+        fused = torch.cat([t.transpose(0, 1) for t in own], 2).contiguous()
+        q, k, v = (t.transpose(0, 1) for t in fused.split(dim, 2))
+    pos = torch.randint(-40, 40, (tokens, 2), generator=gen, dtype=torch.int32).to(DEV)
+    freq = hk.rotary_frequencies((8, 8), device=DEV)
+    table = torch.arange(4, dtype=torch.int32, device=DEV)[None]
+    slots = torch.arange(tokens, dtype=torch.int32, device=DEV).expand(heads, tokens).contiguous()
+    pools = [[torch.zeros(4, heads, page, dim, dtype=torch.float16, device=DEV) for _ in range(2)] for _ in range(2)]
+    want = hk.rotary_append(*own, pos, freq, (8, 8), *pools[0], table, slots)
+    got = hk.rotary_append(q, k, v, pos, freq, (8, 8), *pools[1], table, slots, out=q)
+    assert got.data_ptr() == q.data_ptr() and torch.equal(got, want)
+    assert torch.equal(k, own[1]) and torch.equal(v, own[2])
+    assert all(torch.equal(a, b) for a, b in zip(*pools))
+
+
 # ---- paged_attention ----
 
 ATTEND = [  # counts, lens, q_heads, kv_heads, dim, page, causal_block
