@@ -7,10 +7,10 @@
 //
 // What bounds it, and what it reaches (MI355X; a large copy moves 5.2 TB/s, a large matrix product makes 1200 TFLOP/s in
 // bf16 and 150 in fp32):
-//   a token of 32 streams over 1 .. 32640 slots, 2 kv heads of 128, bf16: reading the cache; 146 + 6 us, 5.7 TB/s
+//   a token of 32 streams over 1 .. 32640 slots, 2 kv heads of 128, bf16: reading the cache; 144 + 6 us, 5.8 TB/s
 //   12240 tokens in 24 frames, 16 query and 4 kv heads of 128, bf16: the matrix cores; 630 us, 1.0 PFLOP/s
 //   510 tokens over 32640 slots, the same heads: the matrix cores; 148 us, joining 10 us, weights 107 us
-//   64 tokens of 4 streams over 4096 slots, 8 heads of 64, fp32: the matrix cores; 29 + 5 us, weights 22 us
+//   64 tokens of 4 streams over 4096 slots, 8 heads of 64, fp32: the matrix cores; 29 + 5 us, weights 21 us
 //   49 tokens over 3136 slots, 20 query and 4 kv heads of 64: its launches and the way through one tile; 9 + 5 us
 #include "cache.hpp"
 
