@@ -103,6 +103,21 @@ __device__ __forceinline__ float sum_halves(float x) {
 
 __device__ const uint4 zero_chunk = {0, 0, 0, 0};
 
+// Exponentials are formed as 2^(score - m) with m up to LIFT below a row's largest score.  The second product's
+// operand in fp16 has no value between 0 and 2^-24, so many small probabilities beside a large one would
+// leave the sum of values and stay in the normaliser (2^19 slots 17.4 below one: off by 0.015); formed from 2^7 down, what
+// is lost begins at 2^-32 of a row's largest.
+template <typename E>
+constexpr float LIFT = __is_same(E, half_t) ? 7.f : 0.f;
+
+// Log-sum of a row from its m and the sum l of its exponentials; LIFT cancels first, which leaves a single term exact.
+template <typename E>
+__device__ __forceinline__ float log_sum(float m, float l) {
+    if (l == 0.f) return -INFINITY;
+    const float top = m == -INFINITY ? 0.f : m + LIFT<E>;
+    return (top + __builtin_amdgcn_logf(l * (1.f / float(1 << int(LIFT<E>))))) * 0.693147180559945309f;
+}
+
 // Where a workgroup's rows and slots are.  A ROW is one (token, head of the group) pair of a stream and
 // kv head: row r is token r / group, query head h * group + r % group, so the heads that share keys
 // share their tiles too.
@@ -559,11 +574,20 @@ struct RowState {
         }
     }
 
-    // The reference of the exponentials follows the maximum only when that outgrows it by 2^8: any reference
-    // gives the same quotient, and a step without a new one leaves the sums alone.
+    // The reference of the exponentials follows the maximum only when that outgrows it by 2^8 (fp16: by 2^15, from
+    // 2^7 on): any reference gives the same quotient, and a step without a new one leaves the sums alone.
     __device__ __forceinline__ void follow(float top) {
-        if (ballot(top > m + 8.f) != 0) {
-            const float m2 = fmaxf(m, top), fade = m2 == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - m2);
+        bool more;
+        // `top` is off by half a step, |top| 2^-24, which counts as soon as that is not small: fp16 overflows at 2^16
+        if constexpr (LIFT<E> > 0.f) more = fmaf(fabsf(top), 0x1p-22f, top) - m > LIFT<E> + 8.f;
+        else more = top > m + 8.f;
+        if (ballot(more) != 0) {
+            float next = top - LIFT<E>;
+            if constexpr (LIFT<E> > 0.f) {  // half a step is more than 2^-1, or, from 2^28 on, may be more than 2^4
+                const float size = fabsf(top);
+                if (size >= 0x1p24f) next = size < 0x1p28f ? top : fmaf(size, 0x1p-23f, top);
+            }
+            const float m2 = fmaxf(m, next), fade = m2 == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - m2);
             m = m2;
             l *= fade;
 #pragma unroll
@@ -650,8 +674,9 @@ struct RowState {
         bool odd = false;
         if constexpr (MASK) odd = any_odd(vt);
         if constexpr (sizeof(E) == 2) {
-            // the sum above is of the probabilities in fp32; the product's operand is rounded to the 16-bit type
-            // (half a step of it relative to each, as much as the values that it multiplies carry)
+            // the sum above is of the probabilities in fp32; the product's operand is rounded to the 16-bit type (half a
+            // step of it relative to each, as much as the values that it multiplies carry; fp16: or 2^-32 of the
+            // row's largest, see LIFT)
             chunk pr[BLK][2];
 #pragma unroll
             for (int b = 0; b < BLK; ++b)
@@ -956,7 +981,7 @@ attention_mfma_kernel(AttnCall call) {
                 E *dst = out + int64_t(w.first + tk) * tp.ot + hd * tp.oh + c;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) dst[j] = v.v[j];
-                if (c == 0 && lse != nullptr) lse[gr] = ll == 0.f ? -INFINITY : (ref + __builtin_amdgcn_logf(ll)) * 0.693147180559945309f;
+                if (c == 0 && lse != nullptr) lse[gr] = log_sum<E>(mm, ll);
             }
         }
     } else {
@@ -987,8 +1012,7 @@ attention_mfma_kernel(AttnCall call) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) dst[32 * d + 8 * j + 4 * half + i] = E(st.o[d][4 * j + i] * inv);
             }
-        if (half == 0 && lse != nullptr)
-            lse[grow] = l == 0.f ? -INFINITY : ((st.m == -INFINITY ? 0.f : st.m) + __builtin_amdgcn_logf(l)) * 0.693147180559945309f;
+        if (half == 0 && lse != nullptr) lse[grow] = log_sum<E>(st.m, l);
     }
 }
 
@@ -1230,7 +1254,7 @@ attention_join_kernel(AttnPlan p, AttnGrid g, T *__restrict__ out, float *__rest
             for (int i = 0; i < 4; ++i) dst[i] = T(o[k][i] * inv);
         }
     }
-    if (lane == 0 && lse != nullptr) lse[row] = l == 0.f ? -INFINITY : (ref + __builtin_amdgcn_logf(l)) * 0.693147180559945309f;
+    if (lane == 0 && lse != nullptr) lse[row] = log_sum<T>(top, l);
 }
 
 // Rows of a workgroup.  32 (KEYS) where a stream has no more, and, as long as four wavefronts' blocks have room in LDS

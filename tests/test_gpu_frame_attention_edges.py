@@ -1,0 +1,70 @@
+"""Frame attention where its operators can go wrong beside the ordinary cases: long caches with one dominant
+slot, scores far from zero."""
+import math
+
+import pytest
+import torch
+
+import frame_reference as ref
+from test_gpu_frame_attention import make_pool, widened
+from util import DEV
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("streams,tokens", [(32, 1), (64, 70)], ids=["rows of 32", "rows of 128"])
+def test_paged_attention_many_small_probabilities_beside_a_large_one(lib, streams, tokens):
+    """One slot scores 17.375 above 130559 equal ones (each 2^-25.07 of it) whose values are 1, its own are 0; so many
+    workgroups that none shares its slots.  out = n e / (1 + n e), e = exp(-17.375).
+
+    A probability in fp16 is off by 2^-11 of itself or by 2^-32 of the largest, whichever is more: n 2^-32 in all.
+    Their sum is exact: equal multiples of 2^-24 below 2^7, at most 2^6 units each and 2^23 together.  The
+    normaliser adds up n / 32 blocks and 4 pieces: 2 (n / 32 + 16) w; exponentials and quotient 16 w; the result 2^-11."""
+    from deltacnn_amd import hip_kernels as hk
+    n, kv, dim, page, gap = 130560, 8, 64, 64, 17.375
+    keys = torch.zeros(n // page, kv, page, dim, dtype=torch.float16, device=DEV)
+    values = torch.ones_like(keys)
+    keys[0, :, 3, 0] = gap
+    values[0, :, 3] = 0
+    table = torch.arange(n // page, dtype=torch.int32, device=DEV).expand(streams, n // page).contiguous()  # read by all
+    q = torch.zeros(streams * tokens, kv, dim, dtype=torch.float16, device=DEV)
+    q[..., 0] = 1
+    lens = torch.full((streams,), n, dtype=torch.int32, device=DEV)
+    got, lse = hk.paged_attention(q, keys, values, table, lens, scale=1.0, return_lse=True)
+    assert b"join" not in lib.dc_last_kernels()
+    mass = (n - 1) * math.exp(-gap)
+    want = mass / (1 + mass)
+    u = ref.half_step(torch.float16)
+    tol = n * 2.0 ** -32 + want * (2 * u + (2 * (n / 32 + 16) + 16) * ref.W)
+    assert float((got.double() - want).abs().max()) <= tol
+    assert float((lse.double() - gap - math.log1p(mass)).abs().max()) <= (n / 32 + 16 + 8 * (gap + 2)) * ref.W
+
+
+@pytest.mark.parametrize("tokens,wide", [(1, False), (150, False), (150, True)])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_paged_attention_equal_scores_far_from_zero(lib, tokens, wide, sign):
+    """Scores of one value up to 2^32, where a step of fp32 is 2^8 and more: every slot counts the same, and nothing
+    overflows fp16.  All probabilities are one number, rounded once: (u + 2 n w + 16 w) mean |v| + u |out|.
+
+    That holds where the number is a normal one in fp16.  The maximum that is subtracted, in powers of two, is
+    off by half a step at most, 2^3 below 2^28: the number is 2^-8 or more.  From 2^28 on half a step is 2^4 and more, a
+    score is good to no power of two, and any weights of the slots are as good: what is left is |out| <= max |v|."""
+    from deltacnn_amd import hip_kernels as hk
+    gen = torch.Generator().manual_seed(50)
+    n, dim, page = 300, 64, 32
+    keys, values, _, _, table = make_pool(gen, 1, n, 1, page, dim, torch.float16)
+    table = widened(table, page, tokens, 1, 1) if wide else table
+    v = ref.gather(values, table[0], n, 0, page)
+    want, u = v.mean(0), ref.half_step(torch.float16)
+    tol = (u + (2 * n + 16) * ref.W) * v.abs().mean(0) + u * want.abs()
+    q = torch.zeros(tokens, 1, dim, dtype=torch.float16)
+    lens = torch.tensor([n], dtype=torch.int32, device=DEV)
+    keys.zero_()
+    for power in range(10, 32):
+        q[..., 0] = min(1.37 * 2.0 ** (power // 2), 61000.0)
+        keys[..., 0] = sign * min(1.23 * 2.0 ** (power - power // 2), 63000.0)
+        got = hk.paged_attention(q.to(DEV), keys.to(DEV), values.to(DEV), table.to(DEV), lens, scale=1.0)
+        if float(q[0, 0, 0]) * abs(float(keys[0, 0, 0, 0])) * math.log2(math.e) < 2.0 ** 28:
+            ref.assert_within(got[:, 0], want.expand(tokens, dim), tol.expand(tokens, dim), f"2^{power}")
+        else:
+            assert float(got.abs().nan_to_num(math.inf).max()) <= float(v.abs().max()), f"2^{power}"
