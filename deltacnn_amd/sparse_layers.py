@@ -1118,7 +1118,9 @@ class DCFrameAttention(DCModule):
 
     Parameters: ``qkv`` and ``proj``, plain linear layers.  Returns a new ``[B, C, H, W]`` tensor in
     channels_last; no residual.  Inference only.  Nothing depends on the host's count of frames, so a
-    frame behind the first can be captured (FrameGraph, VideoGraph) like the other layers' frames."""
+    frame behind the first can be captured (FrameGraph, VideoGraph) like the other layers' frames.  A frame of
+    another shape or type starts a new state; a graph goes on with the one it was captured with, until ``reset``
+    ends both."""
 
     def __init__(self, channels, heads, kv_heads=None, head_dim=None, frames=64, keep_frames=1, decay=1.0, sections=None,
                  base=10000.0, page_size=64, bias=True, name=""):
@@ -1138,6 +1140,7 @@ class DCFrameAttention(DCModule):
         self.qkv = Linear(channels, (heads + 2 * self.kv_heads) * self.head_dim, bias=bias)
         self.proj = Linear(heads * self.head_dim, channels, bias=bias)
         self._state = None
+        self._captured = []  # states that captured graphs write to: they live on beside a new one, until reset()
 
     def _start(self, x):
         b, _, h, w = x.shape
@@ -1166,6 +1169,8 @@ class DCFrameAttention(DCModule):
         if self._state is None or self._state["key"] != (tuple(input.shape), input.dtype, input.device):
             self._state = self._start(input)
         s = self._state
+        if input.is_cuda and torch.cuda.is_current_stream_capturing() and all(c is not s for c in self._captured):
+            self._captured.append(s)
         tokens = b * h * w
         q_end, k_end = self.heads * self.head_dim, (self.heads + self.kv_heads) * self.head_dim
         fused = self.qkv(input.permute(0, 2, 3, 1).reshape(tokens, c))
@@ -1184,6 +1189,7 @@ class DCFrameAttention(DCModule):
     def reset(self):
         super().reset()
         self._state = None
+        self._captured = []
 
 
 class DCUpsamplingNearest2d(DCModule):

@@ -1,12 +1,12 @@
-"""Frame attention where its operators can go wrong beside the ordinary cases: long caches with one dominant
-slot, scores far from zero."""
+"""Frame attention where its operators and its layer can go wrong beside the ordinary cases: long caches with one
+dominant slot, scores far from zero, graphs and eager frames of one layer."""
 import math
 
 import pytest
 import torch
 
 import frame_reference as ref
-from test_gpu_frame_attention import make_pool, widened
+from test_gpu_frame_attention import _layer, make_pool, widened
 from util import DEV
 
 pytestmark = pytest.mark.gpu
@@ -68,3 +68,30 @@ def test_paged_attention_equal_scores_far_from_zero(lib, tokens, wide, sign):
             ref.assert_within(got[:, 0], want.expand(tokens, dim), tol.expand(tokens, dim), f"2^{power}")
         else:
             assert float(got.abs().nan_to_num(math.inf).max()) <= float(v.abs().max()), f"2^{power}"
+
+
+# ---- the layer ----
+
+def frames_of(shape, count, seed, dtype=torch.float16):
+    gen = torch.Generator().manual_seed(seed)
+    return [torch.randn(shape, generator=gen).to(dtype).to(DEV).contiguous(memory_format=torch.channels_last) for _ in range(count)]
+
+
+def test_a_graph_keeps_its_state_beside_eager_frames_of_another_size(lib):
+    """A frame of another size starts a new state; the graph goes on with its own, and what is allocated in
+    between is not written to."""
+    from deltacnn_amd.graph import FrameGraph
+    video, other = frames_of((2, 48, 3, 3), 7, 60), frames_of((1, 48, 5, 4), 7, 61)
+    layer, eager, eager_other = (_layer(torch.float16) for _ in range(3))
+    with torch.no_grad():
+        wanted, wanted_other = [eager(x).clone() for x in video], [eager_other(x).clone() for x in other]
+        assert torch.equal(layer(video[0]), wanted[0])
+        graph = FrameGraph(layer, video[0])
+        kept = []
+        for t in range(1, 7):
+            assert torch.equal(layer(other[t - 1]), wanted_other[t - 1])
+            kept += [torch.full((n,), 77, dtype=torch.int32, device=DEV) for n in (1, 2, 4, 8, 54, 128, 1024, 4096)]
+            got = graph(video[t]).clone()
+            torch.cuda.synchronize()
+            assert torch.equal(got, wanted[t]), f"frame {t}"
+            assert all(bool((k == 77).all()) for k in kept)
