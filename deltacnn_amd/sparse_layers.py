@@ -1166,10 +1166,13 @@ class DCFrameAttention(DCModule):
         if not isinstance(input, Tensor):
             raise TypeError("DCFrameAttention attends over dense maps: put a DCDensify in front of it")
         b, c, h, w = input.shape
+        capturing = input.is_cuda and torch.cuda.is_current_stream_capturing()
         if self._state is None or self._state["key"] != (tuple(input.shape), input.dtype, input.device):
+            if capturing:  # every replay would start anew, from memory of the host that is gone by then
+                raise RuntimeError("DCFrameAttention: the first frame of a shape and type cannot be captured, run it before the capture")
             self._state = self._start(input)
         s = self._state
-        if input.is_cuda and torch.cuda.is_current_stream_capturing() and all(c is not s for c in self._captured):
+        if capturing and all(x is not s for x in self._captured):
             self._captured.append(s)
         tokens = b * h * w
         q_end, k_end = self.heads * self.head_dim, (self.heads + self.kv_heads) * self.head_dim

@@ -95,3 +95,20 @@ def test_a_graph_keeps_its_state_beside_eager_frames_of_another_size(lib):
             torch.cuda.synchronize()
             assert torch.equal(got, wanted[t]), f"frame {t}"
             assert all(bool((k == 77).all()) for k in kept)
+
+
+def test_the_first_frame_of_a_size_is_not_captured(lib):
+    """The state has to be there before the capture; a refused capture leaves layer and stream usable."""
+    from deltacnn_amd.graph import FrameGraph
+    video, other = frames_of((2, 48, 3, 3), 3, 62), frames_of((1, 48, 5, 4), 1, 63)
+    layer, eager = _layer(torch.float16), _layer(torch.float16)
+    with torch.no_grad():
+        with pytest.raises(RuntimeError, match="before the capture"):
+            FrameGraph(layer, video[0])
+        wanted = [eager(x).clone() for x in video]
+        assert torch.equal(layer(video[0]), wanted[0])
+        with pytest.raises(RuntimeError, match="before the capture"):
+            FrameGraph(layer, other[0])
+        assert torch.equal(layer(video[1]), wanted[1])  # the refused frame has changed nothing
+        graph = FrameGraph(layer, video[0])
+        assert torch.equal(graph(video[2]), wanted[2])
