@@ -1114,7 +1114,7 @@ class DCFrameAttention(DCModule):
     frame.  Every position of a ``[B, C, H, W]`` map is a token; the layer keeps the keys and values of
     ``frames * H * W`` tokens of each of the B streams.  Once that is used up, the tokens that have
     received the least attention (``decay`` per frame) give way, separately for each kv head; those of
-    the last ``keep_frames`` frames give way last.  Positions are rotary over (time, row, column).
+    the ``keep_frames`` frames in front of the arriving one give way last.  Positions are rotary over (time, row, column).
 
     Parameters: ``qkv`` and ``proj``, plain linear layers.  Returns a new ``[B, C, H, W]`` tensor in
     channels_last; no residual.  Inference only.  Nothing depends on the host's count of frames, so a
@@ -1158,7 +1158,7 @@ class DCFrameAttention(DCModule):
             "table": torch.arange(pages, dtype=torch.int32, device=dev).view(b, per),
             "lens": torch.zeros(b, dtype=torch.int32, device=dev),
             "positions": grid.reshape(-1, 3).contiguous().to(dev),  # column 0: the frame, counted on the device
-            "keep_from": torch.full((b,), 1 - self.keep_frames, dtype=torch.int32, device=dev),
+            "keep_from": torch.full((b,), -self.keep_frames, dtype=torch.int32, device=dev),
             "frequencies": hk.rotary_frequencies(self.sections, self.base, device=dev),
         }
 

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import frame_reference as ref
-from test_gpu_frame_attention import _layer, make_pool, widened
+from test_gpu_frame_attention import PlainFrames, _layer, make_pool, widened
 from util import DEV
 
 pytestmark = pytest.mark.gpu
@@ -112,3 +112,49 @@ def test_the_first_frame_of_a_size_is_not_captured(lib):
         assert torch.equal(layer(video[1]), wanted[1])  # the refused frame has changed nothing
         graph = FrameGraph(layer, video[0])
         assert torch.equal(graph(video[2]), wanted[2])
+
+
+class Protecting:
+    """A layer as PlainFrames wants to see it, which counts the frame that arrives among `keep_frames`: one more."""
+
+    def __init__(self, layer):
+        self.layer, self.keep_frames = layer, layer.keep_frames + 1
+
+    def __getattr__(self, name):
+        return getattr(self.layer, name)
+
+
+@pytest.mark.parametrize("keep", [0, 1, 2])
+def test_layer_protects_the_last_frames(lib, keep):
+    """fp32, two streams, eight frames of which four fit: the tokens of the last `keep` frames stay whatever attention
+    they have received, in every kv head, and outputs, slots and stamps are those of the 64-bit statement.
+
+    Its numbers are sums of at most 48 (projections) and 80 (slots) terms of magnitude about 1 in fp32 behind two
+    projections: 10 (48 + 80) w relative to outputs below 1; weights that decide have to differ by twice that."""
+    from deltacnn_amd.sparse_layers import DCFrameAttention
+    torch.manual_seed(4)
+    layer = DCFrameAttention(48, 4, kv_heads=2, head_dim=24, frames=4, keep_frames=keep, decay=0.5, page_size=16).eval().to(DEV)
+    shape = (2, 48, 4, 5)
+    plain = PlainFrames(Protecting(layer), shape)
+    gen = torch.Generator().manual_seed(8)
+    rescued = 0
+    with torch.no_grad():
+        for t in range(8):
+            x = torch.randn(shape, generator=gen)
+            before = [[[(c, c[2]) for c in cells] for cells in heads] for heads in plain.kept]
+            want = plain.frame(x)
+            got = layer(x.to(DEV).contiguous(memory_format=torch.channels_last))
+            assert float((got.double().cpu() - want).abs().max()) < 10 * 128 * ref.W, f"frame {t}"
+            s = layer._state
+            for b in range(2):
+                for h in range(2):
+                    cells = plain.kept[b][h]
+                    stamps = ref.gather(s["stamps"].cpu()[..., None], s["table"].cpu()[b], len(cells), h, 16)[:, 0]
+                    assert stamps.tolist() == [c[3] for c in cells], f"frame {t}: other tokens were kept"
+                    for back in range(min(keep, t) + 1):
+                        assert int((stamps == t - back).sum()) == 20, f"frame {t}: tokens of frame {t - back} went"
+                    gone = [w for c, w in before[b][h] if not any(c is d for d in cells)]
+                    if gone:
+                        rescued += sum(w < max(gone) for c, w in before[b][h] if t - keep <= c[3])
+    assert 20 * 128 * ref.W < plain.gap < math.inf
+    assert (rescued > 0) == (keep > 0)  # without the protection other tokens would have gone
