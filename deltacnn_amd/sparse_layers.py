@@ -1116,13 +1116,18 @@ class DCFrameAttention(DCModule):
     received the least attention (``decay`` per frame) give way, separately for each kv head; those of
     the ``keep_frames`` frames in front of the arriving one give way last.  Positions are rotary over (time, row, column).
 
+    ``decay`` decides how far back the choice looks.  A token that has received r per frame for long counts
+    r / (1 - decay), a token of one frame what it received there: with the default 0.5 a new token stays that receives
+    more than twice as much per frame as an old one.  From 0.9 on few do, and the cache keeps mostly the first
+    frames it has seen; 1 never forgets any attention; 0 goes by the last frame alone.
+
     Parameters: ``qkv`` and ``proj``, plain linear layers.  Returns a new ``[B, C, H, W]`` tensor in
     channels_last; no residual.  Inference only.  Nothing depends on the host's count of frames, so a
     frame behind the first can be captured (FrameGraph, VideoGraph) like the other layers' frames.  A frame of
     another shape or type starts a new state; a graph goes on with the one it was captured with, until ``reset``
     ends both."""
 
-    def __init__(self, channels, heads, kv_heads=None, head_dim=None, frames=64, keep_frames=1, decay=1.0, sections=None,
+    def __init__(self, channels, heads, kv_heads=None, head_dim=None, frames=64, keep_frames=1, decay=0.5, sections=None,
                  base=10000.0, page_size=64, bias=True, name=""):
         super().__init__()
         self.name = name

@@ -158,3 +158,31 @@ def test_layer_protects_the_last_frames(lib, keep):
                         rescued += sum(w < max(gone) for c, w in before[b][h] if t - keep <= c[3])
     assert 20 * 128 * ref.W < plain.gap < math.inf
     assert (rescued > 0) == (keep > 0)  # without the protection other tokens would have gone
+
+
+def test_layer_lets_go_of_an_earlier_scene(lib):
+    """With the constructor's own decay and protection, 40 frames of one scene are gone after as many frames of
+    another as the cache holds.
+
+    Queries and keys are 4 x and 4 x (but for the one pair that turns with the position), x is +1 or -1: a score is +-34,
+    so that a frame attends to its own scene alone, evenly.  With decay d a token of the first scene has at most
+    1 (its first frame) + 1 / (F (1 - d)), F = 4 frames in the cache; d = 0.5 makes that 1.5 and halves it with every
+    frame of the second scene, whose j-th frame gives each of its j n tokens 1 / j.  When frame j = 3, 4 chooses, the first
+    scene's tokens are below 1.5 / 2^(j - 1) < 1 / 2, the second's in front of the protected frame above 1 / 2 + 1 / 2."""
+    from deltacnn_amd.sparse_layers import DCFrameAttention
+    layer = DCFrameAttention(8, 1, frames=4, sections=(2, 0, 0), page_size=16).eval()
+    with torch.no_grad():
+        layer.qkv.weight.zero_()
+        layer.qkv.bias.zero_()
+        for e in range(2, 8):
+            layer.qkv.weight[e, e] = layer.qkv.weight[8 + e, e] = 4.0
+        layer.qkv.weight[16:24] = torch.eye(8)
+        layer.to(DEV)
+        x = torch.ones(1, 8, 3, 3, device=DEV).contiguous(memory_format=torch.channels_last)
+        for _ in range(40):
+            layer(x)
+        for _ in range(4):
+            layer(-x)
+    s = layer._state
+    stamps = ref.gather(s["stamps"].cpu()[..., None], s["table"].cpu()[0], 36, 0, 16)[:, 0]
+    assert sorted(stamps.tolist()) == [t for t in range(40, 44) for _ in range(9)]
