@@ -1167,6 +1167,12 @@ class DCFrameAttention(DCModule):
             "frequencies": hk.rotary_frequencies(self.sections, self.base, device=dev),
         }
 
+    def _drop(self):
+        """Give up the present state; its tensors leave the list of all layers' caches unless a graph uses them."""
+        s, self._state = self._state, None
+        if s is not None and all(x is not s for x in self._captured):
+            DCModule.temp_buffers = [t for t in DCModule.temp_buffers if all(t is not x for x in s.values())]
+
     def forward(self, input):
         if not isinstance(input, Tensor):
             raise TypeError("DCFrameAttention attends over dense maps: put a DCDensify in front of it")
@@ -1175,6 +1181,7 @@ class DCFrameAttention(DCModule):
         if self._state is None or self._state["key"] != (tuple(input.shape), input.dtype, input.device):
             if capturing:  # every replay would start anew, from memory of the host that is gone by then
                 raise RuntimeError("DCFrameAttention: the first frame of a shape and type cannot be captured, run it before the capture")
+            self._drop()
             self._state = self._start(input)
         s = self._state
         if capturing and all(x is not s for x in self._captured):

@@ -186,3 +186,17 @@ def test_layer_lets_go_of_an_earlier_scene(lib):
     s = layer._state
     stamps = ref.gather(s["stamps"].cpu()[..., None], s["table"].cpu()[0], 36, 0, 16)[:, 0]
     assert sorted(stamps.tolist()) == [t for t in range(40, 44) for _ in range(9)]
+
+
+def test_alternating_sizes_do_not_grow_memory(lib):
+    from deltacnn_amd.sparse_layers import DCModule
+    layer = _layer(torch.float16)
+    one, two = frames_of((1, 48, 3, 3), 1, 64)[0], frames_of((2, 48, 3, 3), 1, 65)[0]
+    before, seen = DCModule.get_temp_buffer_numel(), []
+    with torch.no_grad():
+        for _ in range(4):
+            layer(one)
+            layer(two)
+            torch.cuda.synchronize()
+            seen.append((DCModule.get_temp_buffer_numel() - before, torch.cuda.memory_allocated()))
+    assert seen[0][0] > 0 and all(x == seen[0] for x in seen)
