@@ -3,6 +3,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <numeric>
 
 #include "common.hpp"
 
@@ -978,21 +979,41 @@ int check_apart(const char *fn, const char *what, int32_t tokens, int32_t heads,
     return DC_OK;
 }
 
-// Do rows x and y share an element?  Columns of one wider buffer may interleave.
+// Rows [tokens][heads] of `dim` elements, and whether two sets of them share an element.  Columns of one wider
+// buffer may interleave.
 struct RowSet {
     const void *p;
     int32_t tokens, heads, dim;
     int64_t token_stride, head_stride;
     int dtype;
     Span span() const { return Span(p, rows_span(tokens, heads, dim, token_stride, head_stride, dtype)); }
-    // of the columns that a token takes; heads that lie whole tokens apart share theirs
-    int64_t width() const { return heads > 1 && head_stride % token_stride != 0 ? (heads - 1) * head_stride + dim : dim; }
+    // Elements between the first and the last of the rows that `folded` dimensions alone span (bit 0: tokens, 1: heads);
+    // the strides of the others are counted into `step`, their greatest common divisor.
+    int64_t width(int folded, int64_t &step) const {
+        int64_t w = dim;
+        for (int d = 0; d < 2; ++d) {
+            const int32_t n = d == 0 ? tokens : heads;
+            const int64_t stride = d == 0 ? token_stride : head_stride;
+            if (n == 1) continue;
+            if (folded >> d & 1) w += (n - 1) * stride;
+            else step = std::gcd(step, stride);
+        }
+        return w;
+    }
+    // Apart, if the spans are or if there is a way to see both sets as columns: modulo a step that divides the strides
+    // of some dimensions of both, each set lies in a window as wide as its other dimensions span.
     bool meets(const RowSet &o) const {
         if (!span().meets(o.span())) return false;
-        if (token_stride != o.token_stride) return true;
         const int64_t off = (static_cast<const char *>(p) - static_cast<const char *>(o.p)) / (int64_t)esize(dtype);
-        const int64_t column = (off % token_stride + token_stride) % token_stride;
-        return column < o.width() || column + width() > token_stride;
+        for (int mine = 0; mine < 4; ++mine)
+            for (int its = 0; its < 4; ++its) {
+                int64_t step = 0;
+                const int64_t w = width(mine, step), ow = o.width(its, step);
+                if (step == 0) continue;  // nothing but the spans
+                const int64_t column = (off % step + step) % step;
+                if (column >= ow && column + w <= step) return false;
+            }
+        return true;
     }
 };
 

@@ -70,6 +70,32 @@ def test_paged_attention_equal_scores_far_from_zero(lib, tokens, wide, sign):
             assert float(got.abs().nan_to_num(math.inf).max()) <= float(v.abs().max()), f"2^{power}"
 
 
+# ---- one buffer for all ----
+
+@pytest.mark.parametrize("tokens", [1, 2, 21])
+@pytest.mark.parametrize("order", ["t x h d", "t h x d", "h t x d", "h x t d", "x t h d", "x h t d"])
+def test_rotary_append_in_place_of_any_projection(lib, tokens, order):
+    """q, k and v in one buffer, dimensions in any order, q turned in place: as with tensors of their own."""
+    from deltacnn_amd import hip_kernels as hk
+    gen = torch.Generator().manual_seed(70)
+    heads, dim, page = 3, 16, 8
+    own = torch.randn(3, tokens, heads, dim, generator=gen).half().to(DEV)
+    names = order.split()
+    at = [("x", "t", "h", "d").index(n) for n in names]
+    fused = own.permute(at).contiguous()
+    q, k, v = fused.permute([names.index(n) for n in ("x", "t", "h", "d")])
+    pos = torch.randint(-40, 40, (tokens, 2), generator=gen, dtype=torch.int32).to(DEV)
+    freq = hk.rotary_frequencies((8, 8), device=DEV)
+    table = torch.arange(4, dtype=torch.int32, device=DEV)[None]
+    slots = torch.arange(tokens, dtype=torch.int32, device=DEV).expand(heads, tokens).contiguous()
+    pools = [[torch.zeros(4, heads, page, dim, dtype=torch.float16, device=DEV) for _ in range(2)] for _ in range(2)]
+    want = hk.rotary_append(*own, pos, freq, (8, 8), *pools[0], table, slots)
+    got = hk.rotary_append(q, k, v, pos, freq, (8, 8), *pools[1], table, slots, out=q)
+    assert got.data_ptr() == q.data_ptr() and torch.equal(got, want)
+    assert torch.equal(k, own[1]) and torch.equal(v, own[2])
+    assert all(torch.equal(a, b) for a, b in zip(*pools))
+
+
 # ---- the layer ----
 
 def frames_of(shape, count, seed, dtype=torch.float16):
