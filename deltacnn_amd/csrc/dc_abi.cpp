@@ -1149,11 +1149,11 @@ int dc_paged_attention(const dc_attention_args *a, int dtype, void *stream) {
     const int64_t vec = 16 / int64_t(esize(dtype));
     if (a->q_token_stride % vec || a->q_head_stride % vec)
         return fail(DC_ERR_ALIGN, "%s: rows of q are not aligned to 16 bytes", fn);
-    const Span q(a->q, rows_span(a->tokens, a->q_heads, a->dim, a->q_token_stride, a->q_head_stride, dtype));
-    const Span out(a->out, rows_span(a->tokens, a->q_heads, a->dim, a->out_token_stride, a->out_head_stride, dtype));
+    const RowSet q = {a->q, a->tokens, a->q_heads, a->dim, a->q_token_stride, a->q_head_stride, dtype};
+    const RowSet out = {a->out, a->tokens, a->q_heads, a->dim, a->out_token_stride, a->out_head_stride, dtype};
     const size_t pool = size_t(a->num_pages) * a->kv_heads * a->page_size * a->dim * esize(dtype);
     if ((rc = check_apart(fn, "out", a->tokens, a->q_heads, a->dim, a->out_token_stride, a->out_head_stride)) != DC_OK) return rc;
-    if (out.meets(q) || out.meets(Span(a->keys, pool)) || out.meets(Span(a->values, pool)))
+    if (out.meets(q) || out.span().meets(Span(a->keys, pool)) || out.span().meets(Span(a->values, pool)))
         return fail(DC_ERR_UNSUPPORTED, "%s: out overlaps an operand", fn);
     const int64_t need = dc::paged_attention_workspace(*a, dtype);
     if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need))

@@ -565,7 +565,8 @@ typedef struct dc_attention_args {
  * whatever they hold.  A stream with a page outside the pool among the slots it reads gets NaN.
  * With weights, every slot below lens receives, summed over the tokens and the heads that share it,
  *   weights[s] = decay * weights[s] + sum p[s]          (decay 0: the old weight is not read);
- * pages then belong to one stream each.  out must not overlap the operands.  Results do not depend
+ * pages then belong to one stream each.  out must not share an element with q (columns of one buffer
+ * may lie side by side) or lie in the cache.  Results do not depend
  * on the order in which workgroups run. */
 int dc_paged_attention(const dc_attention_args *args, int dtype, void *stream);
 /* Bytes of workspace that the call needs (0: none; negative: a dc_status). */

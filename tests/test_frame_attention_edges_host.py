@@ -4,7 +4,7 @@ import random
 import pytest
 import torch
 
-from test_frame_attention_host import rotary_args
+from test_frame_attention_host import attention_args, rotary_args
 
 
 # ---- the layer's state ----
@@ -102,3 +102,14 @@ def test_rows_that_share_an_element_are_never_taken_for_apart(lib):
     # the other way round a few layouts are refused that would do: none of those above, and not many
     assert sum(s for s, _ in verdicts) > 300 and sum(not s for s, _ in verdicts) > 300
     assert sum(r for s, r in verdicts if not s) < 0.2 * sum(not s for s, _ in verdicts)
+
+
+def test_out_may_lie_beside_q_in_one_buffer(lib):
+    """Rows of 2 heads of 16 in a buffer of 64 columns: q in the first 32, out in the others.  (What is not refused for
+    its place is refused for a missing workspace.)"""
+    big = dict(max_pages=4096, page_size=64, num_pages=1, keys=BASE + (1 << 24), values=BASE + (1 << 26), workspace=None, q=BASE,
+               q_token_stride=64, out_token_stride=64)
+    assert lib.dc_paged_attention(attention_args(BASE, out=BASE + 2 * 32, **big), 1, None) == -4
+    for column in (0, 8, 16, 24, 40, 48, 56):  # the last ones reach into the next token's q
+        assert lib.dc_paged_attention(attention_args(BASE, out=BASE + 2 * column, **big), 1, None) == -3, column
+        assert b"overlaps an operand" in lib.dc_last_error()

@@ -96,6 +96,24 @@ def test_rotary_append_in_place_of_any_projection(lib, tokens, order):
     assert all(torch.equal(a, b) for a, b in zip(*pools))
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=["float16", "float32"])
+@pytest.mark.parametrize("tokens", [1, 90])
+def test_paged_attention_beside_its_queries(lib, dtype, tokens):
+    """q and out as columns of one buffer: as with a tensor of its own, and q stays."""
+    from deltacnn_amd import hip_kernels as hk
+    gen = torch.Generator().manual_seed(71)
+    heads, dim, n = 4, 64, 500
+    keys, values, weights, _, table = (t.to(DEV) for t in make_pool(gen, 1, n, 2, 64, dim, dtype))
+    both = torch.randn(tokens, 2 * heads, dim, generator=gen).to(dtype).to(DEV)
+    q, out = both.split(heads, 1)
+    own = q.clone()
+    lens = torch.tensor([n], dtype=torch.int32, device=DEV)
+    w = weights.clone()
+    want = hk.paged_attention(own, keys, values, table, lens, weights=w)
+    got = hk.paged_attention(q, keys, values, table, lens, weights=weights, out=out)
+    assert got.data_ptr() == out.data_ptr() and torch.equal(got, want) and torch.equal(q, own) and torch.equal(weights, w)
+
+
 # ---- the layer ----
 
 def frames_of(shape, count, seed, dtype=torch.float16):
