@@ -1278,7 +1278,9 @@ AttnGrid plan_grid(const AttnPlan &p, bool ragged, int bm) {
     AttnGrid g = {};
     g.block_rows = bm;
     const int64_t rows = int64_t(p.tokens) * p.group;
-    g.stream_blocks = int(ceil_div64(rows / p.streams, bm));
+    // (with starts there may be fewer rows than streams: a token each of 20 of 32 streams over 32640 slots, one head of 128
+    // in bf16, 63 us in pieces, 284 us without)
+    g.stream_blocks = max(1, int(ceil_div64(rows / p.streams, bm)));
     g.flat = ragged ? int(rows / bm) + p.streams : g.stream_blocks * p.streams;
     const int64_t cap = int64_t(p.pool.max_pages) * p.pool.page_size;
     const int64_t base = int64_t(g.flat) * p.kv_heads;

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import frame_reference as ref
-from test_gpu_frame_attention import PlainFrames, _layer, make_pool, widened
+from test_gpu_frame_attention import PlainFrames, _layer, make_pool, starts_of, widened
 from util import DEV
 
 pytestmark = pytest.mark.gpu
@@ -68,6 +68,31 @@ def test_paged_attention_equal_scores_far_from_zero(lib, tokens, wide, sign):
             ref.assert_within(got[:, 0], want.expand(tokens, dim), tol.expand(tokens, dim), f"2^{power}")
         else:
             assert float(got.abs().nan_to_num(math.inf).max()) <= float(v.abs().max()), f"2^{power}"
+
+
+# ---- streams without tokens ----
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bfloat16", "float32"])
+@pytest.mark.parametrize("active", [1, 20])
+def test_paged_attention_where_most_streams_wait(lib, dtype, active):
+    """Fewer rows than streams: the slot axis is still cut into pieces."""
+    from deltacnn_amd import hip_kernels as hk
+    gen = torch.Generator().manual_seed(80 + active)
+    streams, n, dim, page = 32, 2000, 64, 64
+    chosen = sorted(torch.randperm(streams, generator=gen)[:active].tolist())
+    counts = [int(b in chosen) for b in range(streams)]
+    lens = [n - 7 * b if counts[b] else 5 for b in range(streams)]
+    keys, values, weights, _, table = make_pool(gen, streams, n, 1, page, dim, dtype)
+    q = (1.5 * torch.randn(active, 1, dim, generator=gen)).to(dtype)
+    lens_t, starts = torch.tensor(lens, dtype=torch.int32), starts_of(counts)
+    out, tol, lse, lse_tol, ww, w_tol = ref.attention(q, keys, values, table, lens_t, starts, None, 0, weights, 0.75)
+    w = weights.to(DEV)
+    got, got_lse = hk.paged_attention(*(t.to(DEV) for t in (q, keys, values, table, lens_t)), starts=starts.to(DEV), weights=w,
+                                      decay=0.75, return_lse=True)
+    assert b"attention_join_kernel" in lib.dc_last_kernels()
+    ref.assert_within(got, out, tol, "out")
+    ref.assert_within(got_lse, lse, lse_tol, "lse")
+    ref.assert_within(w, ww, w_tol, "weights")
 
 
 # ---- one buffer for all ----
