@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import frame_reference as ref
-from test_gpu_frame_attention import PlainFrames, _layer, make_pool, starts_of, widened
+from test_gpu_frame_attention import DTYPES, PlainFrames, _layer, ids, make_pool, poison_unused, starts_of, widened
 from util import DEV
 
 pytestmark = pytest.mark.gpu
@@ -93,6 +93,55 @@ def test_paged_attention_where_most_streams_wait(lib, dtype, active):
     ref.assert_within(got, out, tol, "out")
     ref.assert_within(got_lse, lse, lse_tol, "lse")
     ref.assert_within(w, ww, w_tol, "weights")
+
+
+# ---- rows of more than 256 bytes, 33 .. 64 a stream and head: two wavefronts a workgroup ----
+
+NARROW = [  # counts, lens, q_heads, kv_heads, page, causal_block
+    ([40], [300], 1, 1, 64, 0), ([64], [333], 1, 1, 33, 1), ([33], [200], 1, 1, 13, 0), ([25, 20], [190, 90], 2, 1, 16, 5),
+    ([50, 0, 20, 64], [77, 9, 150, 64], 2, 2, 64, 16), ([50, 3, 64], [40, 3, 300], 1, 1, 13, 1), ([64], [1], 3, 3, 1, 0),
+    ([45], [31], 1, 1, 33, 7),
+]
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.float16, 256), (torch.bfloat16, 256), (torch.bfloat16, 136), (torch.float32, 256),
+                                       (torch.float32, 136), (torch.float32, 96)], ids=str)
+@pytest.mark.parametrize("shape", NARROW, ids=str)
+def test_paged_attention_two_wavefronts(lib, dtype, dim, shape):
+    from deltacnn_amd import hip_kernels as hk
+    counts, lens, heads, kv, page, block = shape
+    gen = torch.Generator().manual_seed(3000 + sum(counts) + sum(lens))
+    streams = len(counts)
+    assert 32 * streams < sum(counts) * (heads // kv) <= 64 * streams
+    keys, values, weights, _, table = make_pool(gen, streams, max(lens) + page, kv, page, dim, dtype)
+    poison_unused(keys, values, weights, table, lens, page)
+    q = (1.5 * torch.randn(sum(counts), heads, dim, generator=gen)).to(dtype)
+    for b, n in enumerate(lens):
+        table[b, -(-n // page):] = -12345
+    lens_t, starts = torch.tensor(lens, dtype=torch.int32), starts_of(counts)
+    out, tol, lse, lse_tol, ww, w_tol = ref.attention(q, keys, values, table, lens_t, starts, None, block, weights, 0.75)
+    w = weights.to(DEV)
+    got, got_lse = hk.paged_attention(*(t.to(DEV) for t in (q, keys, values, table, lens_t)),
+                                      starts=starts.to(DEV) if len(set(counts)) > 1 else None, causal_block=block, weights=w, decay=0.75, return_lse=True)
+    ref.assert_within(got, out, tol, "out")
+    ref.assert_within(got_lse, lse, lse_tol, "lse")
+    ref.assert_within(w, ww, w_tol, "weights")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("block", [0, 1])
+def test_paged_attention_two_wavefronts_over_long_pieces(lib, dtype, block):
+    """Four streams of 8 heads share the card: pieces of more blocks than the rings of tiles hold."""
+    from deltacnn_amd import hip_kernels as hk
+    gen = torch.Generator().manual_seed(90)
+    tokens, kv, dim, page, lens = 40, 8, 256, 64, [6400, 3333, 1, 5001]
+    keys, values, _, _, table = make_pool(gen, 4, max(lens), kv, page, dim, dtype)
+    q = (1.5 * torch.randn(4 * tokens, kv, dim, generator=gen)).to(dtype)
+    lens_t = torch.tensor(lens, dtype=torch.int32)
+    out, tol, lse, lse_tol, _, _ = ref.attention(q, keys, values, table, lens_t, None, None, block)
+    got, got_lse = hk.paged_attention(*(t.to(DEV) for t in (q, keys, values, table, lens_t)), causal_block=block, return_lse=True)
+    ref.assert_within(got, out, tol, "out")
+    ref.assert_within(got_lse, lse, lse_tol, "lse")
 
 
 # ---- one buffer for all ----
