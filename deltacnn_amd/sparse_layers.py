@@ -1139,8 +1139,11 @@ class DCFrameAttention(DCModule):
             rest = (self.head_dim - time) // 4 * 2
             sections = (time, rest, rest)
         self.sections = tuple(int(n) for n in sections)
-        if len(self.sections) != 3 or heads % self.kv_heads or self.head_dim % 8 or not 0 < sum(self.sections) <= self.head_dim:
+        if (len(self.sections) != 3 or heads % self.kv_heads or self.head_dim % 8 or not 0 < sum(self.sections) <= self.head_dim <= 256
+                or any(n < 0 or n % 2 for n in self.sections)):
             raise ValueError(f"DCFrameAttention: {heads} heads over {self.kv_heads}, head_dim {self.head_dim}, sections {self.sections}")
+        if frames < 1 or keep_frames < 0 or page_size < 1:
+            raise ValueError(f"DCFrameAttention: frames {frames}, keep_frames {keep_frames}, page_size {page_size}")
         self.frames, self.keep_frames, self.decay, self.base, self.page_size = frames, keep_frames, decay, base, page_size
         self.qkv = Linear(channels, (heads + 2 * self.kv_heads) * self.head_dim, bias=bias)
         self.proj = Linear(heads * self.head_dim, channels, bias=bias)

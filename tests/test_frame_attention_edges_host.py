@@ -32,6 +32,15 @@ def test_a_replaced_state_leaves_the_list_of_caches():
         DCModule.temp_buffers = saved
 
 
+@pytest.mark.parametrize("change", [dict(head_dim=264), dict(head_dim=12), dict(sections=(3, 5, 8)), dict(sections=(-2, 8, 8)),
+                                    dict(sections=(8, 8)), dict(sections=(0, 0, 0)), dict(kv_heads=3), dict(frames=0), dict(keep_frames=-1),
+                                    dict(page_size=0)], ids=str)
+def test_the_layer_refuses_what_its_operators_refuse(change):
+    from deltacnn_amd.sparse_layers import DCFrameAttention
+    with pytest.raises(ValueError, match="DCFrameAttention"):
+        DCFrameAttention(64, 4, **change)
+
+
 # ---- rows that share a buffer ----
 
 BASE = 1 << 20  # addresses that are compared and never read: every call here is refused before it would launch
