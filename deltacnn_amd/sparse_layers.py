@@ -1185,7 +1185,8 @@ class DCFrameAttention(DCModule):
             if capturing:  # every replay would start anew, from memory of the host that is gone by then
                 raise RuntimeError("DCFrameAttention: the first frame of a shape and type cannot be captured, run it before the capture")
             self._drop()
-            self._state = self._start(input)
+            with torch.inference_mode(False):  # later frames may run in another mode and count on in it
+                self._state = self._start(input)
         s = self._state
         if capturing and all(x is not s for x in self._captured):
             self._captured.append(s)

@@ -318,3 +318,13 @@ def test_alternating_sizes_do_not_grow_memory(lib):
             torch.cuda.synchronize()
             seen.append((DCModule.get_temp_buffer_numel() - before, torch.cuda.memory_allocated()))
     assert seen[0][0] > 0 and all(x == seen[0] for x in seen)
+
+
+def test_frames_in_inference_mode_and_out_of_it(lib):
+    video = frames_of((1, 48, 3, 3), 6, 66)
+    layer, eager = _layer(torch.float16), _layer(torch.float16)
+    with torch.no_grad():
+        wanted = [eager(x).clone() for x in video]
+    for t, x in enumerate(video):
+        with torch.inference_mode() if t % 2 == 0 else torch.no_grad():
+            assert torch.equal(layer(x), wanted[t]), f"frame {t}"
