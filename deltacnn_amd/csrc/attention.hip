@@ -6,10 +6,10 @@
 // launch: weight[s] = decay weight[s] + sum over rows of e^(s - lse).
 //
 // What bounds it, and what it reaches (MI355X; a large copy moves 5.2 TB/s, a large matrix product makes 1200 TFLOP/s in
-// bf16 and 150 in fp32):
-//   a token of 32 streams over 1 .. 32640 slots, 2 kv heads of 128, bf16: reading the cache; 144 + 6 us, 5.8 TB/s
-//   12240 tokens in 24 frames, 16 query and 4 kv heads of 128, bf16: the matrix cores; 630 us, 1.0 PFLOP/s
-//   510 tokens over 32640 slots, the same heads: the matrix cores; 148 us, joining 10 us, weights 107 us
+// bf16 and 150 in fp32; single kernels: medians under the profiler, where those bound by the matrix cores run slower):
+//   a token of 32 streams over 18360 .. 32640 slots, 2 kv heads of 128, bf16: reading the cache; 145 + 7 us, 5.8 TB/s
+//   12240 tokens in 24 frames, 16 query and 4 kv heads of 128, bf16: the matrix cores; a call 612 us, 1.04 PFLOP/s
+//   510 tokens over 32640 slots, the same heads: the matrix cores; 160 us, joining 12 us, weights 119 us, a call 247 us
 //   64 tokens of 4 streams over 4096 slots, 8 heads of 64, fp32: the matrix cores; 29 + 5 us, weights 21 us
 //   49 tokens over 3136 slots, 20 query and 4 kv heads of 64: its launches and the way through one tile; 9 + 5 us
 #include "cache.hpp"
@@ -1021,10 +1021,13 @@ attention_mfma_kernel(AttnCall call) {
 // of 64 at a time through LDS; a lane's scores are those of one row, so its sums over the rows stay
 // in place until the end, where the lanes of a half are added up in a fixed order.
 //
-// Bound by its vector work: an exponential, a multiplication and two sums for every score take as long as the
-// score's product.  2040 rows x 32640 slots x 4 heads of 128, bf16: 107 us, 0.64 PFLOP/s.  (64 slots a
-// wavefront, half of the reads from LDS: 109 us there, 455 instead of 437 us for 8 streams over 16320 slots, and
-// 1300 instead of 650 us for 8192 tokens in frames of 512, where the workgroups of the first slots have most rows.)
+// Bound by its products and its vector work one after the other: an exponential, a multiplication and two sums for
+// every score take about as long as the score's product, and the full wait and the barrier in front of every tile of rows
+// keep the two wavefronts of a SIMD in step.  2040 rows x 32640 slots x 4 heads of 128, bf16: 112 .. 127 us under the
+// profiler, 0.6 PFLOP/s.  A workgroup walks over all rows by itself, so few slots fill the card poorly: 8160 rows of one kv
+// head over 2040 slots 145 us.  (64 slots a wavefront, half of the reads from LDS: alike in the first case, 455 instead of
+// 437 us for 8 streams over 16320 slots, and 1300 instead of 650 us for 8192 tokens in frames of 512, where the workgroups
+// of the first slots have most rows.)
 template <typename E, int DP>
 __global__ void __launch_bounds__(256, DP * sizeof(E) <= 256 ? 2 : 1)
 attention_weights_kernel(AttnPlan p, FastDiv by_group, const E *__restrict__ q, const float *__restrict__ lse,
@@ -1284,7 +1287,7 @@ AttnGrid plan_grid(const AttnPlan &p, bool ragged, int bm) {
     g.flat = ragged ? int(rows / bm) + p.streams : g.stream_blocks * p.streams;
     const int64_t cap = int64_t(p.pool.max_pages) * p.pool.page_size;
     const int64_t base = int64_t(g.flat) * p.kv_heads;
-    // Pieces of the slot axis until every compute unit has two workgroups, or one with few rows, whose LDS it
+    // Pieces of the slot axis (by the table's capacity: the lengths are the device's) until every compute unit has two workgroups, or one with few rows, whose LDS it
     // takes (a token of 32 streams over 32640 slots: 146 us, with two 159 us and twice as much to join), and
     // not more than are resident at once; none below 128 slots, in whole turns of a workgroup's blocks.
     const bool few = bm == 32;

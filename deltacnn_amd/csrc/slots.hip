@@ -14,7 +14,7 @@
 // (cache_slots_kernel).  Longer caches are cut into pieces, a workgroup each, and the selection becomes
 // four launches that meet in histograms in the workspace (cache_slots_piece_kernel): one workgroup
 // alone draws too little from memory (130560 slots x 4 heads: 389 us that way, 8 + 13 + 10 + 12 us in pieces).
-// 1568 slots x 8 heads x 32 streams, 256 workgroups at once: 22 us; 3136 slots x 4 heads: 11 us.
+// 12544 slots x 8 heads x 32 streams, 256 workgroups at once: 21 us; 3136 slots x 4 heads: 11 us.
 #include "cache.hpp"
 
 namespace dc {

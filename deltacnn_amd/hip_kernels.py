@@ -928,6 +928,7 @@ def paged_attention(q, keys, values, page_table, lens, *, starts=None, scale=Non
     A token sees every slot in use of its stream, ``lens[b]`` of them; with ``causal_block = c`` the
     new tokens are the last ``n`` slots in order, and token ``i`` sees slots below ``lens[b] - n +
     (i // c + 1) * c`` (1: causal; the tokens of a frame: a frame sees itself and those before it).
+    (In order they are until :func:`cache_slots` hands them slots of earlier tokens; then only 0 is meaningful.)
     A token that sees nothing gets zeros (and a log-sum of -inf); what is not visible has no influence,
     NaN included; a stream that reads a page outside the pool gets NaN.  ``scale`` defaults to
     ``dim ** -0.5``.  With ``weights`` [pages, kv_heads, page_size] float32 every slot in use also

@@ -559,7 +559,8 @@ typedef struct dc_attention_args {
 /* Attention of new tokens over a paged cache that already holds them:
  *   out = sum_s p[s] values[s],  p = softmax over the visible slots s of scale * <q, keys[s]>.
  * Token i of a stream's n sees slots [0, lens) or, with causal_block = c > 0 (the new tokens being
- * the last n slots in order), slots below lens - n + (i / c + 1) * c: 1 is causal by tokens, the
+ * the last n slots in order, which they no longer are once dc_cache_slots has given slots of
+ * earlier tokens to them), slots below lens - n + (i / c + 1) * c: 1 is causal by tokens, the
  * tokens of a frame make frames see themselves and the frames before them.  A token that sees
  * nothing gets zeros and lse = -infinity.  Slots that are not visible never influence anything,
  * whatever they hold.  A stream with a page outside the pool among the slots it reads gets NaN.
